@@ -2,6 +2,9 @@
 HIPCC ?= /opt/rocm/bin/hipcc
 ARCH ?= gfx950
 HIPFLAGS ?= -O3 -std=c++17 -fPIC --offload-arch=$(ARCH) -munsafe-fp-atomics -Wno-unused-result
+# no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on these cards. The
+# host pass warns that it does not know the feature: harmless
+HIPFLAGS += -Xclang -target-feature -Xclang -packed-fp32-ops
 CXXFLAGS ?= -O3 -std=c++17 -fPIC -Wall -Wno-unused-result
 PKG := homebrewnlp_mtf_amd
 KSRC := $(wildcard csrc/kernels/*.hip)
