@@ -1,0 +1,420 @@
+// A key-value cache in pages: block tables and slot maps from request lengths, and the attention of one new token per
+// request over its pages.
+//
+// K cache [P][Hk][page][D]; V cache [P][Hk][page / 8][D][8]: eight tokens of one dimension side by side, so that V^T,
+// the matrix operand of P V that wants tokens along its contraction, loads 16 bytes a lane like K does -- no transpose
+// in shared memory on the path that reads the whole cache for every token (the append writes two bytes at a time
+// instead, once a token).
+#include "common.h"
+
+struct PlanDesc {
+  const int *cached, *nnew;            // [B] tokens held, tokens to append
+  int* table;                          // [B][ld] page ids, entries of new pages are written
+  const int *free, *nfree;             // [P] stack of unused page ids, its height
+  int *slots;                          // [T] out: page id * page + offset, -1: none
+  long long* pos;                      // [T] out: position of each token in its request
+  int *start, *lens, *nfree_out;       // [B + 1], [B], [1] out
+  int B, W, ld, page, T, P;
+};
+
+struct PagedDesc {
+  const void *q, *k, *v;
+  void* o;
+  const int *table, *lens;
+  float* part;                         // [B][Hq][nsplit][D + 2] partial outputs, maxima, sums
+  long long q_bs, q_hs;                // strides of q's batch and head, in elements
+  int B, Hq, Hk, D, P, cap, ld, shift, dtype, nsplit, split;   // cap: lengths count up to it; page = 1 << shift
+  float scale;
+};
+
+namespace {
+constexpr int NTH = 256;
+
+// ---- block tables and slot maps
+// Requests are served in order. Request b holds c tokens in ceil(c / page) pages and wants n more. It is refused -- no
+// slots, its length stays -- where its pages pass the table's width, its tokens pass the step's buffer, or the pages
+// asked for up to and including it pass the stack. Its i-th new page is the stack's entry nfree - 1 - (pages asked for
+// before it) - i. Sums over the requests before b are all that a group needs, so every block forms them itself from
+// the lengths (a few KB out of the caches) and one launch does it all: the call's latency is what matters here.
+struct Want { long long n, need; bool fits; };
+
+__device__ __forceinline__ Want want_of(const PlanDesc& d, int b, int& c) {
+  c = max(d.cached[b], 0);
+  const int n = max(d.nnew[b], 0);
+  const long long old = (c + (long long)d.page - 1) / d.page, all = ((long long)c + n + d.page - 1) / d.page;
+  const bool fits = all <= d.W;
+  return {n, fits ? all - old : 0, fits};
+}
+
+__device__ __forceinline__ long long wave_sum_ll(long long v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// grid (request groups, token segments): 8 requests a block, 32 lanes each
+constexpr int GR = 8, GL = NTH / GR;
+
+__global__ __launch_bounds__(NTH) void page_plan_kernel(const PlanDesc d) {
+  __shared__ long long red[3][NTH / 64];
+  __shared__ long long s_n[GR], s_need[GR];
+  const int tid = threadIdx.x, r0 = blockIdx.x * GR;
+  long long n0 = 0, need0 = 0, total = 0;        // tokens and pages before the block's requests; all tokens
+  for (int j = tid; j < d.B; j += NTH) {
+    int c;
+    const Want w = want_of(d, j, c);
+    total += w.n;
+    if (j < r0) { n0 += w.n; need0 += w.need; }
+  }
+  n0 = wave_sum_ll(n0);
+  need0 = wave_sum_ll(need0);
+  total = wave_sum_ll(total);
+  if ((tid & 63) == 0) { red[0][tid >> 6] = n0; red[1][tid >> 6] = need0; red[2][tid >> 6] = total; }
+  const int g = tid / GL, l = tid % GL, b = r0 + g;
+  int c = 0;
+  Want w = {0, 0, false};
+  if (b < d.B) w = want_of(d, b, c);
+  if (l == 0) { s_n[g] = w.n; s_need[g] = w.need; }
+  __syncthreads();
+  n0 = need0 = total = 0;
+#pragma unroll
+  for (int i = 0; i < NTH / 64; ++i) { n0 += red[0][i]; need0 += red[1][i]; total += red[2][i]; }
+  for (int i = 0; i < g; ++i) { n0 += s_n[i]; need0 += s_need[i]; }
+  const int avail = min(max(*d.nfree, 0), d.P);
+  const bool first = blockIdx.y == 0;
+  if (b < d.B) {
+    const bool room = w.fits && n0 + w.n <= d.T;
+    const bool ok = room && (w.need == 0 || need0 + w.need <= avail);
+    const long long old = (c + (long long)d.page - 1) / d.page;
+    if (first && l == 0) {
+      d.lens[b] = ok ? (int)(c + w.n) : c;
+      d.start[b] = (int)min(n0, (long long)0x7fffffff);
+    }
+    if (first && ok)
+      for (long long i = l; i < w.need; i += GL) d.table[(long long)b * d.ld + old + i] = d.free[avail - 1 - need0 - i];
+    for (long long i = (long long)blockIdx.y * GL + l; i < w.n && n0 + i < d.T; i += (long long)gridDim.y * GL) {
+      const long long p = c + i, e = p / d.page;
+      int slot = -1;
+      if (ok) {
+        const int id = e < old ? d.table[(long long)b * d.ld + e] : d.free[avail - 1 - need0 - (e - old)];
+        if ((unsigned)id < (unsigned)d.P) slot = id * d.page + (int)(p % d.page);
+      }
+      d.slots[n0 + i] = slot;
+      d.pos[n0 + i] = p;
+    }
+  }
+  // places of the step's buffer behind the last token
+  for (long long t = total + (blockIdx.y * (long long)gridDim.x + blockIdx.x) * NTH + tid; t < d.T;
+       t += (long long)gridDim.x * gridDim.y * NTH) {
+    d.slots[t] = -1;
+    d.pos[t] = 0;
+  }
+  if (!first || blockIdx.x != gridDim.x - 1) return;
+  // what is left of the stack: the pages asked for up to the last request that got some. Thread t takes its run of
+  // requests; the runs' sums are joined in order
+  __shared__ long long sn[NTH], sneed[NTH], top[NTH / 64];
+  const int per = (d.B + NTH - 1) / NTH, j0 = tid * per, j1 = min(d.B, j0 + per);
+  long long n = 0;
+  for (int j = j0; j < j1; ++j) {
+    int cc;
+    n += want_of(d, j, cc).n;
+  }
+  sn[tid] = n;
+  __syncthreads();
+  long long at = 0;
+  for (int i = 0; i < tid; ++i) at += sn[i];
+  long long need = 0, a2 = at;
+  for (int j = j0; j < j1; ++j) {
+    int cc;
+    const Want x = want_of(d, j, cc);
+    a2 += x.n;
+    if (a2 <= d.T) need += x.need;
+  }
+  sneed[tid] = need;
+  __syncthreads();
+  long long asked = 0, taken = 0;
+  for (int i = 0; i < tid; ++i) asked += sneed[i];
+  for (int j = j0; j < j1; ++j) {
+    int cc;
+    const Want x = want_of(d, j, cc);
+    at += x.n;
+    if (at > d.T) continue;
+    asked += x.need;
+    if (x.need > 0 && asked <= avail) taken = asked;
+  }
+  for (int o = 32; o > 0; o >>= 1) taken = max(taken, (long long)__shfl_xor(taken, o, 64));
+  if ((tid & 63) == 0) top[tid >> 6] = taken;
+  __syncthreads();
+  if (tid == 0) {
+    for (int i = 0; i < NTH / 64; ++i) taken = max(taken, top[i]);
+    *d.nfree_out = (int)(avail - taken);
+    d.start[d.B] = (int)min(total, (long long)0x7fffffff);
+  }
+}
+
+// pages of the requests that are done go back onto the stack, in request order; their lengths become 0. One block
+__global__ __launch_bounds__(1024) void page_release_kernel(const unsigned char* __restrict__ done, int* lens,
+                                                           const int* __restrict__ table, int* stack, int* nfree, int B,
+                                                           int W, int ld, int page, int P) {
+  __shared__ int cnt[1024];
+  __shared__ int base;
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (tid == 0) base = min(max(*nfree, 0), P);
+  for (int b0 = 0; b0 < B; b0 += 1024) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < B && done[b]) n = (int)min(((long long)max(lens[b], 0) + page - 1) / page, (long long)W);
+    __syncthreads();                              // the piece before this one has read cnt and base
+    cnt[tid] = n;
+    __syncthreads();
+    for (int o = 1; o < 1024; o <<= 1) {          // inclusive prefix sums
+      const int v = tid >= o ? cnt[tid - o] : 0;
+      __syncthreads();
+      cnt[tid] += v;
+      __syncthreads();
+    }
+    if (b < B && done[b]) lens[b] = 0;
+    // one wave a request: 16 waves copy the rows of the piece
+    const int at0 = base;
+    for (int r = tid >> 6; r < 1024 && b0 + r < B; r += 16) {
+      const int e = r ? cnt[r - 1] : 0, m = cnt[r] - e;
+      for (int i = lane; i < m; i += 64)
+        if ((long long)at0 + e + i < P) stack[at0 + e + i] = table[(long long)(b0 + r) * ld + i];
+    }
+    __syncthreads();
+    if (tid == 0) base = (int)min((long long)at0 + cnt[1023], (long long)P);
+  }
+  __syncthreads();
+  if (tid == 0) *nfree = base;
+}
+
+// ---- attention of one token per request
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+
+template <int TYPE> struct Mat;
+template <> struct Mat<1> {
+  typedef bf16x8_t v;
+  static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint16_t bits(float f) { return f2bf(f); }
+  static __device__ __forceinline__ float back(uint16_t b) { return bf2f(b); }
+};
+template <> struct Mat<2> {
+  typedef f16x8_t v;
+  static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint16_t bits(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
+  static __device__ __forceinline__ float back(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
+};
+
+// o[b][h] = sum_j softmax_j(scale q[b][h] . k_j) v_j over the lens[b] tokens of request b; 0 where it holds none.
+//
+// A block takes one request, one key head and its (up to 16) query heads, and one split of the length; a wave takes
+// every fourth tile of 32 keys. S^T = K Q^T: 16x16x32 products with 16 keys as rows, the query heads as columns. Row m
+// of the two products of a tile is key 8 (m / 4) + 4 t + m % 4, so a lane ends up with the scores of eight
+// neighbouring keys 8 (lane / 16) + 0..7 of one query head: just what the P operand of O^T = V^T P takes from it. P
+// never leaves its lane. With one query head per key head 15 of the 16 columns are idle: the products' time is
+// still a small part of the loads' (16 x 16-cycle products to 16 KB a tile and wave).
+//
+// Softmax in one pass with the running maximum; P enters the product as two summands of the cache's type (its value
+// and what that rounding left), so the weights keep at least 16 bits. Waves, then splits, are joined by their maxima and sums.
+//
+// Keys past the length, and pages whose id is not one, have weight 0 and a value of 0 whatever the cache holds there.
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float NEG = -3.0e38f;                   // a running maximum before any key
+
+template <int TYPE, int D>
+__global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
+  typedef typename Mat<TYPE>::v vec;
+  constexpr int NK = D / 32, NV = D / 16;
+  __shared__ float sm[4][16], sl[4][16];
+  __shared__ float sacc[4][16][D + 4];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+  const int G = d.Hq / d.Hk, ng = (G + 15) / 16;
+  const int hk = blockIdx.y / ng, gi = blockIdx.y % ng, b = blockIdx.z, sp = blockIdx.x;
+  const int h0 = hk * G + gi * 16, gc = min(16, G - gi * 16);
+  const int len = min(max(d.lens[b], 0), d.cap);
+  const int k0 = sp * d.split, k1 = min(len, k0 + d.split);
+  if (k0 >= k1 && sp > 0) return;
+
+  const uint16_t* qp = (const uint16_t*)d.q + b * d.q_bs + (long long)(h0 + min(n, gc - 1)) * d.q_hs + 8 * g;
+  vec q[NK];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) q[j] = *reinterpret_cast<const vec*>(qp + 32 * j);
+  f32x4_t acc[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float m = NEG, l = 0.f;
+  const float sc = d.scale * LOG2E;
+  const int* tb = d.table + (long long)b * d.ld;
+  const uint16_t *K = (const uint16_t*)d.k, *V = (const uint16_t*)d.v;
+  const int in_page = (1 << d.shift) - 1;
+  const long long row = (long long)D << d.shift, pst = d.Hk * row, hoff = hk * row;
+
+  for (int t0 = k0 + 32 * w; t0 < k1; t0 += 128) {
+    // this lane's key rows (one per product) and the first of its eight value tokens, kept inside the length
+    const int ka = min(t0 + 8 * (n >> 2) + (n & 3), len - 1), kb = min(t0 + 8 * (n >> 2) + 4 + (n & 3), len - 1);
+    const int kv = min(t0 + 8 * g, (len - 1) & ~7);
+    int ia = tb[ka >> d.shift], ib = tb[kb >> d.shift], iv = tb[kv >> d.shift];
+    const bool bad_v = (unsigned)iv >= (unsigned)d.P;
+    ia = (unsigned)ia < (unsigned)d.P ? ia : 0;
+    ib = (unsigned)ib < (unsigned)d.P ? ib : 0;
+    iv = bad_v ? 0 : iv;
+    const uint16_t* pa = K + ia * pst + hoff + (ka & in_page) * D + 8 * g;
+    const uint16_t* pb = K + ib * pst + hoff + (kb & in_page) * D + 8 * g;
+    const uint16_t* pv = V + iv * pst + hoff + (kv & in_page) * D + 8 * n;
+    f32x4_t s0{0.f, 0.f, 0.f, 0.f}, s1{0.f, 0.f, 0.f, 0.f};
+    vec a[NK], c[NK], v[NV];
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      a[j] = *reinterpret_cast<const vec*>(pa + 32 * j);
+      c[j] = *reinterpret_cast<const vec*>(pb + 32 * j);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = *reinterpret_cast<const vec*>(pv + 128 * j);
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      s0 = Mat<TYPE>::mul(a[j], q[j], s0);
+      s1 = Mat<TYPE>::mul(c[j], q[j], s1);
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { p[i] = s0[i] * sc; p[4 + i] = s1[i] * sc; }
+    const int left = bad_v ? 0 : k1 - (t0 + 8 * g);         // how many of the lane's eight keys count
+    if (__any(left < 8)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = i < left ? p[i] : -INFINITY;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        u32x4_t x = __builtin_bit_cast(u32x4_t, v[j]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = left >= 2 * i + 2 ? x[i] : left == 2 * i + 1 ? x[i] & 0xffffu : 0u;
+        v[j] = __builtin_bit_cast(vec, x);
+      }
+    }
+    float mx = p[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, p[i]);
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
+    const float f = __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) acc[i] *= f;
+    u32x4_t hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint16_t h2[2], l2[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float x = __builtin_amdgcn_exp2f(p[2 * i + e] - m);
+        l += x;
+        h2[e] = Mat<TYPE>::bits(x);
+        l2[e] = Mat<TYPE>::bits(x - Mat<TYPE>::back(h2[e]));
+      }
+      hi[i] = h2[0] | (uint32_t)h2[1] << 16;
+      lo[i] = l2[0] | (uint32_t)l2[1] << 16;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, hi), acc[j]);
+      acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, lo), acc[j]);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  if (g == 0) { sm[w][n] = m; sl[w][n] = l; }
+#pragma unroll
+  for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[w][n][16 * j + 4 * g]) = acc[j];
+  __syncthreads();
+  const bool whole = len <= d.split;
+  for (int e = threadIdx.x; e < gc * D; e += NTH) {
+    const int h = e / D, i = e % D;
+    const float M = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
+    float L = 0.f, o = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = __builtin_amdgcn_exp2f(sm[x][h] - M);
+      L += f * sl[x][h];
+      o += f * sacc[x][h][i];
+    }
+    if (whole) {
+      ((uint16_t*)d.o)[((long long)b * d.Hq + h0 + h) * D + i] = Mat<TYPE>::bits(L != 0.f ? o / L : 0.f);
+    } else {
+      float* pt = d.part + (((long long)b * d.Hq + h0 + h) * d.nsplit + sp) * (D + 2);
+      pt[i] = o;
+      if (i == 0) { pt[D] = M; pt[D + 1] = L; }
+    }
+  }
+}
+
+// the splits of one query head: block (Hq, B), thread = dim
+template <int TYPE>
+__global__ __launch_bounds__(NTH) void paged_join_kernel(const PagedDesc d) {
+  const int h = blockIdx.x, b = blockIdx.y, i = threadIdx.x;
+  const int len = min(max(d.lens[b], 0), d.cap);
+  if (len <= d.split || i >= d.D) return;
+  const int ns = (len + d.split - 1) / d.split;
+  const float* pt = d.part + ((long long)b * d.Hq + h) * d.nsplit * (d.D + 2);
+  float M = NEG;
+  for (int s = 0; s < ns; ++s) M = fmaxf(M, pt[(long long)s * (d.D + 2) + d.D]);
+  float L = 0.f, o = 0.f;
+  for (int s = 0; s < ns; ++s) {
+    const float* x = pt + (long long)s * (d.D + 2);
+    const float f = __builtin_amdgcn_exp2f(x[d.D] - M);
+    L += f * x[d.D + 1];
+    o += f * x[i];
+  }
+  ((uint16_t*)d.o)[((long long)b * d.Hq + h) * d.D + i] = Mat<TYPE>::bits(L != 0.f ? o / L : 0.f);
+}
+
+template <int TYPE>
+int attn(const PagedDesc& d, hipStream_t st) {
+  const int ng = (d.Hq / d.Hk + 15) / 16;
+  const dim3 grid(d.nsplit, d.Hk * ng, d.B), blk(NTH);
+  switch (d.D) {
+    case 32: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 32>), grid, blk, 0, st, d); break;
+    case 64: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 64>), grid, blk, 0, st, d); break;
+    case 96: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 96>), grid, blk, 0, st, d); break;
+    case 128: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 128>), grid, blk, 0, st, d); break;
+    case 256: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 256>), grid, blk, 0, st, d); break;
+    default: return -2;
+  }
+  int rc = (int)hipGetLastError();
+  if (rc || d.nsplit == 1) return rc;
+  hipLaunchKernelGGL(paged_join_kernel<TYPE>, dim3(d.Hq, d.B), dim3(d.D <= 64 ? 64 : d.D <= 128 ? 128 : 256), 0, st, d);
+  return (int)hipGetLastError();
+}
+}  // namespace
+
+OBST_API int obst_page_plan(const PlanDesc* d, hipStream_t st) {
+  if (!d || d->B < 1 || d->W < 1 || d->ld < d->W || d->page < 1 || d->T < 0 || d->P < 1) return -1;
+  const int gx = (d->B + GR - 1) / GR;
+  long long gy = d->T / ((long long)d->B * GL * 4);      // a few rounds of a request's tokens per lane
+  gy = gy < 1 ? 1 : gy > 64 ? 64 : gy;
+  hipLaunchKernelGGL(page_plan_kernel, dim3(gx, (unsigned)gy), dim3(NTH), 0, st, *d);
+  return (int)hipGetLastError();
+}
+
+OBST_API int obst_page_release(const void* done, void* lens, const void* table, void* stack, void* nfree, int B, int W,
+                               int ld, int page, int P, hipStream_t st) {
+  if (B < 1 || W < 1 || ld < W || page < 1 || P < 1) return -1;
+  hipLaunchKernelGGL(page_release_kernel, dim3(1), dim3(1024), 0, st, (const unsigned char*)done, (int*)lens,
+                     (const int*)table, (int*)stack, (int*)nfree, B, W, ld, page, P);
+  return (int)hipGetLastError();
+}
+
+OBST_API int obst_paged_attn(const PagedDesc* d, hipStream_t st) {
+  if (!d || d->B < 1 || d->B > 65535 || d->Hk < 1 || d->Hq < 1 || d->Hq % d->Hk || d->P < 1 || d->cap < 0 ||
+      d->nsplit < 1 || d->split < 32 || d->split % 32 || (d->nsplit > 1 && !d->part))
+    return -1;
+  if (d->shift < 4 || d->shift > 8 || (long long)d->ld << d->shift < d->cap) return -3;
+  if (d->cap > (long long)d->nsplit * d->split) return -4;
+  if (d->dtype == 1) return attn<1>(*d, st);
+  if (d->dtype == 2) return attn<2>(*d, st);
+  return -5;
+}

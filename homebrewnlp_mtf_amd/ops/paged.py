@@ -1,0 +1,315 @@
+"""A key-value cache in pages, and single-token attention over it (csrc/kernels/paged.hip, rotary.hip; torch oracles on
+the CPU).
+
+A pool of ``P`` pages of ``page`` tokens is shared by all requests (one pool per layer, one set of page ids for all
+layers). Request b's tokens lie in the pages ``table[b, 0], table[b, 1], ...``; unused ids wait on a stack. One step of
+a serving loop, without a read-back to the host:
+
+    plan = page_plan(lens, new, table, stack, height, page, tokens=T)     # pages and slots of the new tokens
+    q = rotary_append(q, k, v, k_cache, v_cache, plan.slots, plan.pos, freqs)   # per layer
+    o = paged_attn(q, k_cache, v_cache, table, plan.lens, scale)                # per layer, one new token a request
+
+Layouts: keys [P, kv heads, page, D], values [P, kv heads, page / 8, D, 8] (eight tokens of one dim side by side: the
+order in which the attention's second product reads them); a token's slot is ``page id * page + offset``.
+Ids outside the pool and tokens without a slot are passed over, never followed.
+"""
+from __future__ import annotations
+
+import typing
+
+import torch
+
+from . import _lib as L
+from . import raw
+from .rotary import (DTYPES, _tokens, check_heads, check_turn, kernel_weights, rotary_t, tokens_view)
+
+HEAD_DIMS = (32, 64, 96, 128, 256)
+PAGES = (16, 32, 64, 128, 256)
+_MAX_SLOTS = 2 ** 31 - 1
+
+
+def page_pools(pages: int, page: int, kv_heads: int, dim: int, dtype: torch.dtype,
+               device: typing.Union[str, torch.device]) -> typing.Tuple[torch.Tensor, torch.Tensor]:
+    """uninitialised (key, value) caches of one layer"""
+    if pages < 1 or kv_heads < 1 or dim < 1 or page not in PAGES or pages * page > _MAX_SLOTS:
+        raise L.KernelError(f"page_pools: {pages} pages of {page} tokens x {kv_heads} heads x {dim}: pages hold "
+                            f"{PAGES} tokens, a pool up to {_MAX_SLOTS}")
+    return (torch.empty(pages, kv_heads, page, dim, dtype=dtype, device=device),
+            torch.empty(pages, kv_heads, page // 8, dim, 8, dtype=dtype, device=device))
+
+
+class PagePlan(typing.NamedTuple):
+    slots: torch.Tensor     # int32 [T]: slot of each new token, -1: none (refused, or behind the last token)
+    pos: torch.Tensor       # int64 [T]: its position in its request (0 behind the last token)
+    start: torch.Tensor     # int32 [B + 1]: first token of each request, then all tokens
+    lens: torch.Tensor      # int32 [B]: tokens held after the step (unchanged where refused)
+    nfree: torch.Tensor     # int32 [1]: height of the stack after the step
+
+
+def plan_buffers(requests: int, tokens: int, device: typing.Union[str, torch.device]) -> PagePlan:
+    """buffers for ``page_plan(out=...)``, for a program that keeps them (a captured graph)"""
+    if requests < 1 or tokens < 0:
+        raise L.KernelError(f"plan_buffers: {requests} requests, {tokens} tokens")
+
+    def i32(n):
+        return torch.empty(n, dtype=torch.int32, device=device)
+    return PagePlan(i32(tokens), torch.empty(tokens, dtype=torch.int64, device=device), i32(requests + 1),
+                    i32(requests), i32(1))
+
+
+def _ints(what: str, dev, **ts):
+    for name, t in ts.items():
+        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+            raise L.KernelError(f"{what}: {name} must be contiguous int32 on {dev}, got {t.dtype} on {t.device}")
+
+
+def _table(what: str, table, B: int, dev):
+    if (table.dtype != torch.int32 or table.device != dev or table.dim() != 2 or table.shape[0] != B
+            or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1)
+            or (B > 1 and not table.shape[1] <= table.stride(0) < 2 ** 31)):
+        raise L.KernelError(f"{what}: the table must be int32 [{B}, pages] with dense rows on {dev}, got {table.dtype} "
+                            f"{list(table.shape)} strides {list(table.stride())} on {table.device}")
+
+
+def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stack: torch.Tensor, nfree: torch.Tensor,
+              page: int, tokens: typing.Optional[int] = None, out: typing.Optional[PagePlan] = None) -> PagePlan:
+    """Pages, slots and positions of a step's new tokens, on the device: request b holds ``cached[b]`` tokens and
+    appends ``new[b]`` (int32 [B], negative counts as 0); the step's tokens lie one request after the other in a buffer
+    of ``tokens`` places. New pages come off the top of ``stack`` (int32 [P], ``nfree`` int32 [1] of them unused) and
+    are entered into ``table`` (int32 [B, W]) in place.
+
+    Requests are served in order. One is refused -- no slots, its length unchanged -- if its pages pass W, its tokens
+    the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request that needs no new
+    page goes on). ``cached`` and ``nfree`` are not written: the plan holds their new values, and the same call again
+    gives the same plan. ``out`` must not share memory with them."""
+    dev, B = cached.device, cached.numel()
+    _ints("page_plan", dev, cached=cached, new=new, stack=stack, nfree=nfree)
+    if cached.dim() != 1 or B < 1 or new.shape != cached.shape or nfree.numel() != 1 or stack.dim() != 1:
+        raise L.KernelError(f"page_plan: cached {list(cached.shape)}, new {list(new.shape)}, stack "
+                            f"{list(stack.shape)}, nfree {list(nfree.shape)}")
+    _table("page_plan", table, B, dev)
+    P = stack.numel()
+    if page < 1 or P < 1 or P * page > _MAX_SLOTS:
+        raise L.KernelError(f"page_plan: a pool of {P} pages of {page} tokens (at most {_MAX_SLOTS} tokens)")
+    if out is None:
+        if tokens is None:
+            raise L.KernelError("page_plan: tokens or out")
+        out = plan_buffers(B, tokens, dev)
+    else:
+        _ints("page_plan", dev, slots=out.slots, start=out.start, lens=out.lens, nfree_out=out.nfree)
+        if (out.pos.dtype != torch.int64 or out.pos.device != dev or not out.pos.is_contiguous()
+                or out.pos.shape != out.slots.shape or out.slots.dim() != 1 or out.start.numel() != B + 1
+                or out.lens.numel() != B or out.nfree.numel() != 1
+                or (tokens is not None and tokens != out.slots.numel())):
+            raise L.KernelError("page_plan: out does not fit (plan_buffers)")
+        if out.lens.data_ptr() in (cached.data_ptr(), new.data_ptr()) or out.nfree.data_ptr() == nfree.data_ptr():
+            raise L.KernelError("page_plan: out shares memory with cached, new or nfree")
+    T = out.slots.numel()
+    if T >= 2 ** 31:
+        raise L.KernelError(f"page_plan: {T} tokens")
+    if dev.type == "cuda":
+        d = L.PlanDesc(cached.data_ptr(), new.data_ptr(), table.data_ptr(), stack.data_ptr(), nfree.data_ptr(),
+                       out.slots.data_ptr(), out.pos.data_ptr(), out.start.data_ptr(), out.lens.data_ptr(),
+                       out.nfree.data_ptr(), B, table.shape[1], max(table.stride(0), table.shape[1]), page, T, P)
+        L.launch(L.lib().obst_page_plan, cached, "page_plan", d)
+        return out
+    # ---- torch oracle
+    W, avail = table.shape[1], min(max(int(nfree), 0), P)
+    out.slots.fill_(-1)
+    out.pos.zero_()
+    at = asked = taken = 0
+    for b, (c, n) in enumerate(zip(cached.clamp(min=0).tolist(), new.clamp(min=0).tolist())):
+        out.start[b] = min(at, 2 ** 31 - 1)
+        old, want = -(-c // page), -(-(c + n) // page)
+        ok = want <= W and at + n <= T
+        if ok:
+            asked += want - old
+            ok = want == old or asked <= avail
+            if ok and want > old:
+                taken = asked
+                ids = stack[avail - asked:avail - asked + want - old].flip(0)
+                table[b, old:want] = ids
+        out.lens[b] = c + n if ok else c
+        m = min(n, T - at)
+        if m > 0:
+            p = torch.arange(c, c + m)
+            out.pos[at:at + m] = p
+            if ok:
+                ids = table[b, p // page].long()
+                slot = torch.where((ids >= 0) & (ids < P), ids * page + p % page, -1)
+                out.slots[at:at + m] = slot.int()
+        at += n
+    out.start[B] = min(at, 2 ** 31 - 1)
+    out.nfree[0] = avail - taken
+    return out
+
+
+def page_release(done: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, stack: torch.Tensor, nfree: torch.Tensor,
+                 page: int) -> None:
+    """Requests that are ``done`` (bool [B]) give their pages back: pushed onto ``stack`` in request order, ``nfree``
+    raised and their ``lens`` zeroed, all in place. (A stack that is full takes no more.)"""
+    dev, B = lens.device, lens.numel()
+    _ints("page_release", dev, lens=lens, stack=stack, nfree=nfree)
+    if lens.dim() != 1 or B < 1 or done.shape != lens.shape or done.dtype != torch.bool or done.device != dev \
+            or not done.is_contiguous() or nfree.numel() != 1 or stack.dim() != 1 or stack.numel() < 1 or page < 1:
+        raise L.KernelError(f"page_release: done bool {list(done.shape)}, lens {list(lens.shape)}, page {page}")
+    _table("page_release", table, B, dev)
+    P, W = stack.numel(), table.shape[1]
+    if dev.type == "cuda":
+        L.launch(L.lib().obst_page_release, lens, "page_release", done.data_ptr(), lens.data_ptr(), table.data_ptr(),
+                 stack.data_ptr(), nfree.data_ptr(), B, W, max(table.stride(0), W), page, P)
+        return
+    at = min(max(int(nfree), 0), P)
+    for b in done.nonzero().flatten().tolist():
+        n = min(-(-max(int(lens[b]), 0) // page), W, P - at)
+        stack[at:at + n] = table[b, :n]
+        at += n
+        lens[b] = 0
+    nfree[0] = at
+
+
+# ----------------------------------------------------------------------------------------------------------------
+def _pools(what: str, k_cache, v_cache, q, heads: typing.Optional[int] = None) -> typing.Tuple[int, int, int]:
+    """(pages, kv heads, page) of a layer's caches"""
+    if k_cache.dim() != 4 or v_cache.dim() != 5:
+        raise L.KernelError(f"{what}: caches [P, heads, page, D] and [P, heads, page / 8, D, 8] (page_pools), got "
+                            f"{list(k_cache.shape)}, {list(v_cache.shape)}")
+    P, H, page, D = k_cache.shape
+    if (tuple(v_cache.shape) != (P, H, page // 8, D, 8) or page not in PAGES or P < 1 or D != q.shape[-1]
+            or (heads is not None and H != heads) or P * page > _MAX_SLOTS):
+        raise L.KernelError(f"{what}: caches {list(k_cache.shape)}, {list(v_cache.shape)} for heads {heads} x "
+                            f"{q.shape[-1]}, pages of {PAGES} tokens")
+    for t in (k_cache, v_cache):
+        if t.dtype != q.dtype or t.device != q.device or not t.is_contiguous():
+            raise L.KernelError(f"{what}: caches must be contiguous {q.dtype} on {q.device}")
+    return P, H, page
+
+
+def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slots: torch.Tensor, pos: torch.Tensor, freqs: typing.Optional[torch.Tensor],
+                  interleaved: bool = False, mscale: float = 1.0, q_weight: typing.Optional[torch.Tensor] = None,
+                  k_weight: typing.Optional[torch.Tensor] = None, eps: float = 1e-5,
+                  out: typing.Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``rotary.rotary`` of a step's tokens with the turned keys and the values written into the cache: q [T, Hq, D],
+    k and v [T, Hk, D] (any token and head strides), ``slots`` int32 [T] (outside the pool: neither key nor value is
+    written), ``pos`` int64 [T]. Returns the turned queries [T, Hq, D]. ``freqs`` None and no weights: a plain append.
+    One launch, no gradient. Tokens of one call must have different slots."""
+    check_heads("rotary_append", q, k)
+    if q.dim() != 3 or v.shape != k.shape or v.dtype != q.dtype or v.device != q.device:
+        raise L.KernelError(f"rotary_append: q [T, Hq, D], k and v [T, Hk, D] of one type, got {list(q.shape)}, "
+                            f"{list(k.shape)}, {list(v.shape)}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise L.KernelError("rotary_append has no gradient: call it under torch.no_grad()")
+    T, Hq, D = q.shape
+    P, Hk, page = _pools("rotary_append", k_cache, v_cache, q, k.shape[1])
+    _ints("rotary_append", q.device, slots=slots)
+    if slots.dim() != 1 or slots.numel() != T:
+        raise L.KernelError(f"rotary_append: slots {list(slots.shape)} for {T} tokens")
+    pos, freqs, rot = check_turn("rotary_append", q, pos, freqs, (q_weight, k_weight), eps)
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise L.KernelError(f"rotary_append: out must be contiguous {q.dtype} {list(q.shape)}")
+    if q.device.type == "meta" or T == 0:
+        return out
+    if raw.on_gpu(q):
+        q, q_ts, q_hs = tokens_view(q)
+        k, k_ts, k_hs = tokens_view(k)
+        v, v_ts, v_hs = tokens_view(v)
+        wq, wk, wt = kernel_weights(q_weight, k_weight)
+        d = L.RotDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, out.data_ptr(), k_cache.data_ptr(),
+                      v_cache.data_ptr(), L.ptr(wq), L.ptr(wk), L.ptr(freqs), pos.data_ptr(), slots.data_ptr(), 0, 0,
+                      0, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, 0, 0, 0, 0, T, P * page, Hq, Hk, D, rot,
+                      int(interleaved), DTYPES[q.dtype], wt, 0, 0, page, mscale, eps)
+        L.launch(L.lib().obst_rotary_fwd, q, "rotary_append", d)
+        return out
+    # ---- torch oracle
+    ko = rotary_t(k, None if k_weight is None else k_weight.detach(), pos, freqs, interleaved, mscale, eps)
+    live = (slots >= 0) & (slots < P * page)
+    s = slots[live].long()
+    k_cache[s // page, :, s % page] = ko[live]
+    v_cache[s // page, :, s % page // 8, :, s % 8] = v[live]
+    out.copy_(rotary_t(q, None if q_weight is None else q_weight.detach(), pos, freqs, interleaved, mscale, eps))
+    return out
+
+
+# ----------------------------------------------------------------------------------------------------------------
+def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+               scale: float, max_len: typing.Optional[int] = None, out: typing.Optional[torch.Tensor] = None
+               ) -> torch.Tensor:
+    """Attention of one new token per request over its pages: q [B, Hq, D] (batch and head strides free), caches as
+    ``page_pools`` makes them with Hq a multiple of their heads (query heads h * G .. h * G + G - 1 read key head h),
+    ``table`` int32 [B, W], ``lens`` int32 [B] the tokens that count, the new one among them:
+
+        out[b, h] = softmax_j(scale * q[b, h] . k_j) @ v,  j < min(lens[b], max_len);  0 for a request without tokens
+
+    ``max_len`` (default: what the table's width holds) is a bound on lens that the host knows; it sizes the launch, so
+    a close one helps a wide table. A page id outside the pool hides its tokens. What the cache holds behind a length
+    is never looked at. No gradient."""
+    if q.dim() != 3 or q.shape[0] < 0 or q.numel() == 0 and q.shape[0] > 0:
+        raise L.KernelError(f"paged_attn: q must be [B, heads, D], got {list(q.shape)}")
+    B, Hq, D = q.shape
+    P, Hk, page = _pools("paged_attn", k_cache, v_cache, q)
+    if Hk < 1 or Hq < 1 or Hq % Hk:
+        raise L.KernelError(f"paged_attn: {Hq} query heads over {Hk} key heads")
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
+        raise L.KernelError("paged_attn has no gradient: call it under torch.no_grad()")
+    _table("paged_attn", table, B, q.device)
+    _ints("paged_attn", q.device, lens=lens)
+    if lens.dim() != 1 or lens.numel() != B:
+        raise L.KernelError(f"paged_attn: lens {list(lens.shape)} for {B} requests")
+    W = table.shape[1]
+    cap = min(W * page, _MAX_SLOTS // page * page)
+    if max_len is not None:
+        if max_len < 0:
+            raise L.KernelError(f"paged_attn: max_len {max_len}")
+        cap = min(cap, max_len)
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise L.KernelError(f"paged_attn: out must be contiguous {q.dtype} {list(q.shape)}")
+    if B == 0 or q.device.type == "meta":
+        return out
+    if raw.on_gpu(q):
+        if D not in HEAD_DIMS or q.dtype not in (torch.bfloat16, torch.float16):
+            raise L.KernelError(f"paged_attn: heads of {HEAD_DIMS} in bf16 or fp16 on the GPU, got {D} in {q.dtype}")
+        if B > 65535 or Hk * (-(-Hq // Hk // 16)) > 65535:
+            raise L.KernelError(f"paged_attn: {B} requests x {Hk} heads (at most 65535 each)")
+        if q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 8 or q.data_ptr() % 16:
+            q = q.contiguous()
+            if q.data_ptr() % 16:
+                q = q.clone()
+        for t in (k_cache, v_cache):
+            if t.data_ptr() % 16:
+                raise L.KernelError("paged_attn: caches must be 16-byte aligned")
+        nsplit, split = _splits(B * Hk * (-(-Hq // Hk // 16)), cap)
+        part = torch.empty(B * Hq * nsplit * (D + 2), dtype=torch.float32, device=q.device) if nsplit > 1 else None
+        d = L.PagedDesc(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(),
+                        lens.data_ptr(), L.ptr(part), q.stride(0), q.stride(1), B, Hq, Hk, D, P, cap,
+                        max(table.stride(0), W), page.bit_length() - 1, DTYPES[q.dtype], nsplit, split, scale)
+        L.launch(L.lib().obst_paged_attn, q, "paged_attn", d)
+        return out
+    # ---- torch oracle
+    G = Hq // Hk
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), cap)
+        ids = table[b, :-(-n // page)].long()
+        ok = (ids >= 0) & (ids < P)
+        live = ok.repeat_interleave(page)[:n]
+        ids = torch.where(ok, ids, 0)
+        kk = k_cache[ids].transpose(1, 2).reshape(-1, Hk, D)[:n][live]
+        vv = v_cache[ids].permute(0, 2, 4, 1, 3).reshape(-1, Hk, D)[:n][live]
+        if kk.shape[0] == 0:
+            out[b] = 0
+            continue
+        s = torch.einsum("hgd,jhd->hgj", raw._f(q[b]).reshape(Hk, G, D), raw._f(kk)) * scale
+        out[b] = torch.einsum("hgj,jhd->hgd", torch.softmax(s, -1), raw._f(vv)).reshape(Hq, D)
+    return out
+
+
+def _splits(rows: int, cap: int) -> typing.Tuple[int, int]:
+    """(splits, tokens a split) of the length for ``rows`` blocks without one: enough blocks to fill the card"""
+    want = max(1, -(-2048 // rows))
+    split = max(256, -(-cap // want))
+    split = -(-split // 128) * 128
+    return max(1, -(-cap // split)), split

@@ -1,0 +1,295 @@
+"""Rotary positions of queries and keys, with an optional norm of each head in the same pass (csrc/kernels/rotary.hip;
+a torch oracle on the CPU).
+
+For one head x of one token, D wide: ``n = x / sqrt(mean(x^2) + eps) * weight`` (only where a weight is given), then the
+first ``R = 2 * len(freqs)`` dims of n turn in pairs by ``angle_i = pos * freqs[i]``:
+
+    a' = mscale (a cos - b sin),  b' = mscale (b cos + a sin),  (a, b) = dims (i, i + R/2), interleaved: (2i, 2i + 1)
+
+and the other dims pass through. ``rotary`` is differentiable in q, k and both weights; ``paged.rotary_append`` is the
+serving form that writes keys and values into a paged cache.
+"""
+from __future__ import annotations
+
+import math
+import typing
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import raw
+from .functional import _acc_grad, _done, _param32
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_DIM = 512
+
+
+def rotary_freqs(rot_dim: int, theta: float = 10000.0, scaling: typing.Optional[dict] = None,
+                 device: typing.Union[str, torch.device, None] = None) -> typing.Tuple[torch.Tensor, float]:
+    """(frequencies in radians per position, float64 [rot_dim / 2]; the factor ``mscale`` of the turned dims).
+
+    Plain: ``theta ** (-2 i / rot_dim)``, mscale 1. ``scaling`` stretches them for contexts ``factor`` times as long as
+    the trained one: ``{"type": ..., "factor": s}`` with
+
+    * ``"linear"``: positions are divided by s;
+    * ``"base"``: theta grows by ``s ** (rot_dim / (rot_dim - 2))``: the slowest pair turns s times slower, the fastest
+      as before;
+    * ``"ramp"``: pairs that turn more than ``fast`` (32) times over the trained ``length`` (2048) keep their frequency,
+      those under ``slow`` (1) turns are divided by s, linear in between over the pair's index; mscale is
+      ``0.1 ln s + 1``, sharpening the scores that the longer context flattens."""
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rotary needs an even number of dims, got {rot_dim}")
+    if not theta > 0:
+        raise ValueError(f"rotary base must be positive, got {theta}")
+    i = torch.arange(rot_dim // 2, dtype=torch.float64)
+    mscale = 1.0
+    kind, s = None, 1.0
+    if scaling:
+        unknown = set(scaling) - {"type", "factor", "length", "fast", "slow"}
+        if unknown:
+            raise ValueError(f"unknown rotary scaling keys {sorted(unknown)}")
+        kind, s = scaling["type"], float(scaling["factor"])
+        if not s >= 1:
+            raise ValueError(f"rotary scaling factor must be at least 1, got {s}")
+    if kind == "base":
+        if rot_dim < 4:
+            raise ValueError("rotary scaling 'base' needs at least 4 dims")
+        theta = theta * s ** (rot_dim / (rot_dim - 2))
+    freqs = theta ** (-2.0 * i / rot_dim)
+    if kind == "linear":
+        freqs = freqs / s
+    elif kind == "ramp":
+        length, fast, slow = (float(scaling.get(k, v)) for k, v in (("length", 2048), ("fast", 32), ("slow", 1)))
+        if not (length > 0 and fast > slow > 0 and theta > 1):
+            raise ValueError("rotary scaling 'ramp' needs length > 0, fast > slow > 0 and a base above 1")
+
+        def pair_of(turns):     # the (fractional) pair that makes `turns` turns over the trained length
+            return rot_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim // 2 - 1)
+        far = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        freqs = freqs * (1 - far) + freqs / s * far
+        mscale = 0.1 * math.log(s) + 1.0
+    elif kind not in (None, "base"):
+        raise ValueError(f"unknown rotary scaling type {kind!r} (linear, base, ramp)")
+    return freqs.to(device) if device is not None else freqs, mscale
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# argument checks and layouts shared with the serving form
+def tokens_view(t: torch.Tensor) -> typing.Tuple[torch.Tensor, int, int]:
+    """[..., H, D] -> (the tensor, token stride, head stride); a copy only where the leading dims are no single stride
+    or the last one is not dense"""
+    shape, st = t.shape, t.stride()
+    n = len(shape)
+    ok = st[-1] == 1 or shape[-1] == 1
+    for i in range(n - 3):
+        if shape[i] != 1 and st[i] != st[i + 1] * shape[i + 1]:
+            # a leading dim whose inner one is 1 wide takes its stride from further in
+            ok = ok and all(shape[j] == 1 for j in range(i + 1, n - 2))
+    if not ok:
+        t = t.contiguous()
+        st = t.stride()
+    ts = 0
+    for i in range(n - 3, -1, -1):
+        if shape[i] != 1:
+            ts = st[i]
+            break
+    return t, ts, st[-2]
+
+
+def check_heads(what: str, q, k):
+    if q.dim() < 3 or k.dim() != q.dim() or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
+        raise L.KernelError(f"{what}: q {list(q.shape)} and k {list(k.shape)} must be [..., heads, dim] over the same "
+                            "tokens")
+    if q.shape[-2] < 1 or k.shape[-2] < 1 or not 1 <= q.shape[-1] <= MAX_DIM:
+        raise L.KernelError(f"{what}: at least one head of 1 to {MAX_DIM} dims, got {list(q.shape)}, {list(k.shape)}")
+    if k.dtype != q.dtype or k.device != q.device:
+        raise L.KernelError(f"{what}: q and k must share type and device")
+    if q.device.type == "cuda" and q.dtype not in DTYPES:
+        raise L.KernelError(f"{what}: bf16, fp16 or fp32 on the GPU, got {q.dtype}")
+
+
+def check_turn(what: str, q, pos, freqs, weights, eps: float):
+    """(positions [tokens] contiguous, rotated dims)"""
+    lead = q.shape[:-2]
+    if pos.dtype != torch.int64 or pos.device != q.device:
+        raise L.KernelError(f"{what}: positions must be int64 on the device of q")
+    if pos.shape != lead:
+        try:
+            pos = pos.expand(lead)
+        except RuntimeError:
+            raise L.KernelError(f"{what}: positions {list(pos.shape)} for tokens {list(lead)}") from None
+    rot = 0
+    if freqs is not None:
+        rot = 2 * freqs.numel()
+        if freqs.dtype != torch.float64 or freqs.dim() != 1 or freqs.device != q.device or rot > q.shape[-1]:
+            raise L.KernelError(f"{what}: freqs must be float64 [pairs] on the device of q with 2 * pairs <= "
+                                f"{q.shape[-1]}, got {freqs.dtype} {list(freqs.shape)} on {freqs.device}")
+        freqs = freqs.contiguous()
+    for w in weights:
+        if w is not None and (w.numel() != q.shape[-1] or w.device != q.device or not w.is_floating_point()):
+            raise L.KernelError(f"{what}: norm weights must be [{q.shape[-1]}] on the device of q")
+    if not eps > 0:
+        raise L.KernelError(f"{what}: eps must be positive, got {eps}")
+    return pos.contiguous(), freqs, rot
+
+
+def kernel_weights(wq, wk):
+    """(wq, wk, type code) as the kernels read them: the fp32 master copy of a model parameter, else the tensor itself;
+    of two types, both in fp32"""
+    wq, wk = (None if w is None else (_param32(w) if hasattr(w, "master") else w).detach().contiguous()
+              for w in (wq, wk))
+    types = {w.dtype for w in (wq, wk) if w is not None}
+    if len(types) > 1 or (types and not types <= set(DTYPES)):
+        wq, wk = (None if w is None else w.float() for w in (wq, wk))
+        types = {torch.float32}
+    return wq, wk, DTYPES[types.pop()] if types else 0
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# torch oracle
+def turn_t(x, pos, freqs, inter: bool, mscale: float, sign: float = 1.0):
+    """[T, H, D] in 32 or 64 bits: the pairs turned by sign * angle, scaled"""
+    if freqs is None or freqs.numel() == 0:
+        return x
+    R = 2 * freqs.numel()
+    ang = pos.reshape(-1, 1).to(torch.float64) * freqs
+    c, s = ((f(ang) * mscale).to(x.dtype).unsqueeze(1) for f in (torch.cos, torch.sin))
+    s = s * sign
+    a, b = (x[..., 0:R:2], x[..., 1:R:2]) if inter else (x[..., :R // 2], x[..., R // 2:R])
+    u, v = a * c - b * s, b * c + a * s
+    y = torch.stack((u, v), -1).flatten(-2) if inter else torch.cat((u, v), -1)
+    return torch.cat((y, x[..., R:]), -1)
+
+
+def rotary_t(x, w, pos, freqs, inter: bool, mscale: float, eps: float):
+    x2 = raw._f(x).reshape(-1, *x.shape[-2:])
+    if w is not None:
+        x2 = x2 * torch.rsqrt((x2 * x2).mean(-1, keepdim=True) + eps) * w.to(x2.dtype).reshape(-1)
+    return turn_t(x2, pos, freqs, inter, mscale).reshape(x.shape).to(x.dtype)
+
+
+def rotary_bwd_t(x, w, g, pos, freqs, inter: bool, mscale: float, eps: float):
+    g2 = turn_t(raw._f(g).reshape(-1, *g.shape[-2:]), pos, freqs, inter, mscale, -1.0)
+    if w is None:
+        return g2.reshape(g.shape).to(g.dtype), None
+    x2 = raw._f(x).reshape(-1, *x.shape[-2:])
+    r = torch.rsqrt((x2 * x2).mean(-1, keepdim=True) + eps)
+    u = x2 * r
+    dw = (g2 * u).sum((0, 1))
+    h = g2 * w.to(g2.dtype).reshape(-1)
+    return (r * (h - u * (h * u).mean(-1, keepdim=True))).reshape(g.shape).to(g.dtype), dw
+
+
+# ----------------------------------------------------------------------------------------------------------------
+def _tokens(q) -> int:
+    return q.numel() // (q.shape[-1] * q.shape[-2])
+
+
+def _forward(q, k, pos, freqs, rot, wq, wk, inter, mscale, eps):
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.device.type == "meta" or q.numel() == 0:
+        return qo, ko
+    if not raw.on_gpu(q):
+        w = [None if x is None else _param32(x).detach() for x in (wq, wk)]
+        qo.copy_(rotary_t(q, w[0], pos, freqs, inter, mscale, eps))
+        ko.copy_(rotary_t(k, w[1], pos, freqs, inter, mscale, eps))
+        return qo, ko
+    q, q_ts, q_hs = tokens_view(q)
+    k, k_ts, k_hs = tokens_view(k)
+    wq, wk, wt = kernel_weights(wq, wk)
+    d = L.RotDesc(q.data_ptr(), k.data_ptr(), 0, 0, 0, qo.data_ptr(), ko.data_ptr(), 0, L.ptr(wq), L.ptr(wk),
+                  L.ptr(freqs), pos.data_ptr(), 0, 0, 0, 0, q_ts, q_hs, k_ts, k_hs, 0, 0, 0, 0, 0, 0, _tokens(q), 0,
+                  q.shape[-2], k.shape[-2], q.shape[-1], rot, int(inter), DTYPES[q.dtype], wt, 0, 0, 0, mscale, eps)
+    L.launch(L.lib().obst_rotary_fwd, q, "rotary", d)
+    return qo, ko
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, pos, freqs, rot, inter, mscale, eps):
+        normed = wq is not None or wk is not None
+        ctx.save_for_backward(q if normed else None, k if normed else None, wq, wk, pos, freqs)
+        ctx.cfg = (rot, inter, mscale, eps)
+        return _forward(q, k, pos, freqs, rot, wq, wk, inter, mscale, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, pos, freqs = ctx.saved_tensors
+        rot, inter, mscale, eps = ctx.cfg
+        dq = torch.empty(gq.shape, dtype=gq.dtype, device=gq.device)
+        dk = torch.empty(gk.shape, dtype=gk.dtype, device=gk.device)
+        ws = (wq, wk)
+        # model parameters accumulate into their fp32 main gradient; other weights get theirs back in their own type
+        main = any(getattr(w, "main_grad", None) is not None for w in ws if w is not None)
+        dws, kept = [None, None], [True, True]
+        for i, w in enumerate(ws):
+            if w is None:
+                continue
+            if main:
+                dws[i], kept[i] = _acc_grad(w)
+            elif raw.on_gpu(w) and wt_direct(ws):
+                dws[i], kept[i] = torch.empty(w.shape, dtype=w.dtype, device=w.device), False
+            else:
+                dws[i] = torch.zeros(w.shape, device=w.device, dtype=torch.float64 if w.dtype == torch.float64
+                                     else torch.float32)
+                kept[i] = False
+        into = list(dws)
+        if main and wq is not None and wk is not None and dws[0].data_ptr() == dws[1].data_ptr():
+            into[1] = torch.zeros(wk.shape, dtype=torch.float32, device=wk.device)   # one parameter for both
+        if not raw.on_gpu(gq):
+            for i, (x, w, g, o) in enumerate(((q, wq, gq, dq), (k, wk, gk, dk))):
+                dx, dw = rotary_bwd_t(x, None if w is None else _param32(w).detach(), g, pos, freqs, inter, mscale, eps)
+                o.copy_(dx)
+                if dw is not None:
+                    into[i].add_(dw.reshape(into[i].shape))
+        else:
+            gq, gq_ts, gq_hs = tokens_view(gq)
+            gk, gk_ts, gk_hs = tokens_view(gk)
+            q_ts = q_hs = k_ts = k_hs = 0
+            part = None
+            lib = L.lib()
+            if q is not None:
+                q, q_ts, q_hs = tokens_view(q)
+                k, k_ts, k_hs = tokens_view(k)
+                part = torch.empty(lib.obst_rotary_part(gq.shape[-1]), dtype=torch.float32, device=gq.device)
+            vq, vk, wt = kernel_weights(wq, wk)
+            typed = [x for x in into if x is not None]
+            d = L.RotDesc(L.ptr(q), L.ptr(k), 0, gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), 0,
+                          L.ptr(vq), L.ptr(vk), L.ptr(freqs), pos.data_ptr(), 0, L.ptr(part), L.ptr(into[0]),
+                          L.ptr(into[1]), q_ts, q_hs, k_ts, k_hs, 0, 0, gq_ts, gq_hs, gk_ts, gk_hs, _tokens(gq), 0,
+                          gq.shape[-2], gk.shape[-2], gq.shape[-1], rot, int(inter), DTYPES[gq.dtype], wt,
+                          DTYPES[typed[0].dtype] if typed else 0, int(main), 0, mscale, eps)
+            L.launch(lib.obst_rotary_bwd, gq, "rotary_bwd", d)
+        if into[1] is not dws[1]:
+            dws[1].add_(into[1])
+        out = []
+        for w, g, keep in zip(ws, dws, kept):
+            if w is not None:
+                _done(w)
+            out.append(None if w is None or keep else g.to(w.dtype))
+        return dq, dk, out[0], out[1], None, None, None, None, None, None
+
+
+def wt_direct(ws) -> bool:
+    """both weights of one kernel type: the kernel writes their gradients in it"""
+    return len({w.dtype for w in ws if w is not None}) == 1 and all(w is None or w.dtype in DTYPES for w in ws)
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, freqs: typing.Optional[torch.Tensor],
+           interleaved: bool = False, mscale: float = 1.0, q_weight: typing.Optional[torch.Tensor] = None,
+           k_weight: typing.Optional[torch.Tensor] = None, eps: float = 1e-5
+           ) -> typing.Tuple[torch.Tensor, torch.Tensor]:
+    """Queries [..., Hq, D] and keys [..., Hk, D] of the same tokens, normed (each where its weight [D] is given) and
+    turned (module docstring); any token and head strides. ``pos`` int64 over the tokens (or broadcastable to them, any
+    value), ``freqs`` float64 from ``rotary_freqs`` (None: no rotation). Returns new contiguous tensors; differentiable
+    in q, k and the weights, sums in fp32, weight gradients in a fixed order (the same bits each run)."""
+    check_heads("rotary", q, k)
+    pos, freqs, rot = check_turn("rotary", q, pos, freqs, (q_weight, k_weight), eps)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
+        return _Rotary.apply(q, k, q_weight, k_weight, pos, freqs, rot, bool(interleaved), float(mscale), float(eps))
+    return _forward(q, k, pos, freqs, rot, q_weight, k_weight, bool(interleaved), float(mscale), float(eps))
