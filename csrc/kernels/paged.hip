@@ -21,7 +21,7 @@ struct PagedDesc {
   const void *q, *k, *v;
   void* o;
   const int *table, *lens;
-  float* part;                         // [B][Hq][nsplit][D + 2] partial outputs, maxima, sums
+  float* part;                         // partial outputs [B][Hq][nsplit][D], then maxima and sums [B][Hq][nsplit][2]
   long long q_bs, q_hs;                // strides of q's batch and head, in elements
   int B, Hq, Hk, D, P, cap, ld, shift, dtype, nsplit, split;   // cap: lengths count up to it; page = 1 << shift
   float scale;
@@ -254,18 +254,23 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   const int in_page = (1 << d.shift) - 1;
   const long long row = (long long)D << d.shift, pst = d.Hk * row, hoff = hk * row;
 
+  // this lane's key rows (one per product) and the first of its eight value tokens of a tile; their page ids are loaded
+  // one tile ahead (never past the table: a tile behind the length reads whatever ids stand there, none is followed
+  // outside the pool)
+  const int ra = 8 * (n >> 2) + (n & 3), rv = 8 * g;
+  int ia, ib, iv;
+  auto ids = [&](int t0) {
+    ia = tb[min(t0 + ra, d.cap - 1) >> d.shift];
+    ib = tb[min(t0 + ra + 4, d.cap - 1) >> d.shift];
+    iv = tb[min(t0 + rv, d.cap - 1) >> d.shift];
+  };
+  if (d.cap > 0) ids(k0 + 32 * w);
   for (int t0 = k0 + 32 * w; t0 < k1; t0 += 128) {
-    // this lane's key rows (one per product) and the first of its eight value tokens, kept inside the length
-    const int ka = min(t0 + 8 * (n >> 2) + (n & 3), len - 1), kb = min(t0 + 8 * (n >> 2) + 4 + (n & 3), len - 1);
-    const int kv = min(t0 + 8 * g, (len - 1) & ~7);
-    int ia = tb[ka >> d.shift], ib = tb[kb >> d.shift], iv = tb[kv >> d.shift];
     const bool bad_v = (unsigned)iv >= (unsigned)d.P;
-    ia = (unsigned)ia < (unsigned)d.P ? ia : 0;
-    ib = (unsigned)ib < (unsigned)d.P ? ib : 0;
-    iv = bad_v ? 0 : iv;
-    const uint16_t* pa = K + ia * pst + hoff + (ka & in_page) * D + 8 * g;
-    const uint16_t* pb = K + ib * pst + hoff + (kb & in_page) * D + 8 * g;
-    const uint16_t* pv = V + iv * pst + hoff + (kv & in_page) * D + 8 * n;
+    const long long ja = (unsigned)ia < (unsigned)d.P ? ia : 0, jb = (unsigned)ib < (unsigned)d.P ? ib : 0, jv = bad_v ? 0 : iv;
+    const uint16_t* pa = K + ja * pst + hoff + ((t0 + ra) & in_page) * D + 8 * g;
+    const uint16_t* pb = K + jb * pst + hoff + ((t0 + ra + 4) & in_page) * D + 8 * g;
+    const uint16_t* pv = V + jv * pst + hoff + ((t0 + rv) & in_page) * D + 8 * n;
     f32x4_t s0{0.f, 0.f, 0.f, 0.f}, s1{0.f, 0.f, 0.f, 0.f};
     vec a[NK], c[NK], v[NV];
 #pragma unroll
@@ -275,6 +280,7 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) v[j] = *reinterpret_cast<const vec*>(pv + 128 * j);
+    ids(t0 + 128);
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
       s0 = Mat<TYPE>::mul(a[j], q[j], s0);
@@ -328,8 +334,10 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   if (g == 0) { sm[w][n] = m; sl[w][n] = l; }
+  if (n < gc) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[w][n][16 * j + 4 * g]) = acc[j];
+    for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[w][n][16 * j + 4 * g]) = acc[j];
+  }
   __syncthreads();
   const bool whole = len <= d.split;
   for (int e = threadIdx.x; e < gc * D; e += NTH) {
@@ -345,31 +353,63 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
     if (whole) {
       ((uint16_t*)d.o)[((long long)b * d.Hq + h0 + h) * D + i] = Mat<TYPE>::bits(L != 0.f ? o / L : 0.f);
     } else {
-      float* pt = d.part + (((long long)b * d.Hq + h0 + h) * d.nsplit + sp) * (D + 2);
-      pt[i] = o;
-      if (i == 0) { pt[D] = M; pt[D + 1] = L; }
+      const long long at = ((long long)b * d.Hq + h0 + h) * d.nsplit + sp;
+      d.part[at * D + i] = o;
+      if (i == 0) {
+        float* ml = d.part + (long long)d.B * d.Hq * d.nsplit * D + at * 2;
+        ml[0] = M;
+        ml[1] = L;
+      }
     }
   }
 }
 
-// the splits of one query head: block (Hq, B), thread = dim
+// the splits of one query head: block (Hq, B). The weights of the splits first, each by a thread; then D / 4 threads a
+// split row, 1024 / D rows side by side, joined in a fixed order
+constexpr int MAX_SPLITS = 1024;
+
 template <int TYPE>
 __global__ __launch_bounds__(NTH) void paged_join_kernel(const PagedDesc d) {
-  const int h = blockIdx.x, b = blockIdx.y, i = threadIdx.x;
+  __shared__ float wt[MAX_SPLITS], red[2][NTH / 64];
+  __shared__ f32x4_t so[NTH];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int len = min(max(d.lens[b], 0), d.cap);
-  if (len <= d.split || i >= d.D) return;
+  if (len <= d.split) return;
   const int ns = (len + d.split - 1) / d.split;
-  const float* pt = d.part + ((long long)b * d.Hq + h) * d.nsplit * (d.D + 2);
+  const long long at = ((long long)b * d.Hq + h) * d.nsplit;
+  const float* ml = d.part + (long long)d.B * d.Hq * d.nsplit * d.D + at * 2;
   float M = NEG;
-  for (int s = 0; s < ns; ++s) M = fmaxf(M, pt[(long long)s * (d.D + 2) + d.D]);
-  float L = 0.f, o = 0.f;
-  for (int s = 0; s < ns; ++s) {
-    const float* x = pt + (long long)s * (d.D + 2);
-    const float f = __builtin_amdgcn_exp2f(x[d.D] - M);
-    L += f * x[d.D + 1];
-    o += f * x[i];
+  for (int s = tid; s < ns; s += NTH) M = fmaxf(M, ml[2 * s]);
+  M = wave_max(M);
+  if ((tid & 63) == 0) red[0][tid >> 6] = M;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NTH / 64; ++i) M = fmaxf(M, red[0][i]);
+  float L = 0.f;
+  for (int s = tid; s < ns; s += NTH) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - M);
+    wt[s] = f;
+    L += f * ml[2 * s + 1];
   }
-  ((uint16_t*)d.o)[((long long)b * d.Hq + h) * d.D + i] = Mat<TYPE>::bits(L != 0.f ? o / L : 0.f);
+  L = wave_sum(L);
+  if ((tid & 63) == 0) red[1][tid >> 6] = L;
+  __syncthreads();
+  L = 0.f;
+#pragma unroll
+  for (int i = 0; i < NTH / 64; ++i) L += red[1][i];
+  const int per = d.D / 4, rows = NTH / per, r = tid / per, c = tid % per;
+  const f32x4_t* pt = reinterpret_cast<const f32x4_t*>(d.part) + at * per + c;
+  f32x4_t o{0.f, 0.f, 0.f, 0.f};
+  if (r < rows)
+#pragma unroll 4
+    for (int s = r; s < ns; s += rows) o += pt[(long long)s * per] * wt[s];
+  so[tid] = o;
+  __syncthreads();
+  if (r != 0) return;
+  for (int i = 1; i < rows; ++i) o += so[i * per + c];
+  uint16_t* out = (uint16_t*)d.o + ((long long)b * d.Hq + h) * d.D + 4 * c;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[i] = Mat<TYPE>::bits(L != 0.f ? o[i] / L : 0.f);
 }
 
 template <int TYPE>
@@ -386,7 +426,7 @@ int attn(const PagedDesc& d, hipStream_t st) {
   }
   int rc = (int)hipGetLastError();
   if (rc || d.nsplit == 1) return rc;
-  hipLaunchKernelGGL(paged_join_kernel<TYPE>, dim3(d.Hq, d.B), dim3(d.D <= 64 ? 64 : d.D <= 128 ? 128 : 256), 0, st, d);
+  hipLaunchKernelGGL(paged_join_kernel<TYPE>, dim3(d.Hq, d.B), dim3(NTH), 0, st, d);
   return (int)hipGetLastError();
 }
 }  // namespace
@@ -410,7 +450,7 @@ OBST_API int obst_page_release(const void* done, void* lens, const void* table, 
 
 OBST_API int obst_paged_attn(const PagedDesc* d, hipStream_t st) {
   if (!d || d->B < 1 || d->B > 65535 || d->Hk < 1 || d->Hq < 1 || d->Hq % d->Hk || d->P < 1 || d->cap < 0 ||
-      d->nsplit < 1 || d->split < 32 || d->split % 32 || (d->nsplit > 1 && !d->part))
+      d->nsplit < 1 || d->nsplit > MAX_SPLITS || d->split < 32 || d->split % 32 || (d->nsplit > 1 && !d->part))
     return -1;
   if (d->shift < 4 || d->shift > 8 || (long long)d->ld << d->shift < d->cap) return -3;
   if (d->cap > (long long)d->nsplit * d->split) return -4;

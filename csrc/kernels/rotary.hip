@@ -11,9 +11,11 @@
 // product is off by 10^-2 radians. sin and cos then see an argument within half a turn.
 //
 // A head's elements are cut into items of two chunks of VEC elements (16 bytes): one lane holds both members of its
-// pairs, so the rotation needs no exchange between lanes, and an angle is computed once per lane and token and used for
-// every head of the wave's unit. LPH lanes hold a head, a wave 64 / LPH heads. Memory-bound: each element is read once
-// and written once. VEC = 1 takes what 16-byte accesses cannot (odd head widths, strides or addresses).
+// pairs, so the rotation needs no exchange between lanes. LPH lanes hold a head, a wave 64 / LPH heads of one token.
+// VEC = 1 takes what 16-byte accesses cannot (odd head widths, strides or addresses).
+//
+// Bound by memory: every element is read once and written once. At 32768 tokens of 2 x 16 heads x 128 in bf16, normed:
+// forward 89 us (537 MB, 6.0 TB/s), backward 164 us (805 MB, 4.9 TB/s) and 4 us for the weight sums.
 #include <hip/hip_fp16.h>
 #include "common.h"
 
@@ -24,7 +26,7 @@ struct RotDesc {
   const double* freqs;                  // [R / 2]
   const long long* pos;                 // [T]
   const int* slots;                     // [T] or null
-  float* part;                          // backward: weight-gradient partials [blocks][2][D]
+  float* part;                          // backward: weight-gradient partials [blocks][D]
   void *dwq, *dwk;                      // backward: weight gradients
   long long q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, gq_ts, gq_hs, gk_ts, gk_hs;   // token / head strides, in elements
   long long T, nslots;
@@ -34,6 +36,7 @@ struct RotDesc {
 
 namespace {
 constexpr int NTH = 256;
+constexpr int NOTURN = 256;       // most pairs of a head
 
 template <int T> struct Elem;
 template <> struct Elem<0> { typedef float t; static constexpr int VEC = 4; };
@@ -50,19 +53,22 @@ __device__ __forceinline__ void from_f(float f, __half& o) { o = __float2half(f)
 template <typename E, int VEC>
 struct alignas(sizeof(E) * VEC) Chunk { E e[VEC]; };
 
-// lanes without an element read `safe` and see zeros: a load under a branch would be waited for inside it
-template <typename E, int VEC>
-__device__ __forceinline__ void load(const E* p, const E* safe, bool on, float* f) {
-  const Chunk<E, VEC> c = *reinterpret_cast<const Chunk<E, VEC>*>(on ? p : safe);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) f[i] = on ? to_f(c.e[i]) : 0.f;
-}
 template <typename E, int VEC>
 __device__ __forceinline__ void store(E* p, const float* f) {
   Chunk<E, VEC> c;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) from_f(f[i], c.e[i]);
   *reinterpret_cast<Chunk<E, VEC>*>(p) = c;
+}
+
+// the compiler no longer knows what a loaded chunk holds: what it derived from it is not kept
+template <typename E, int VEC>
+__device__ __forceinline__ void forget(Chunk<E, VEC>& c) {
+  if constexpr (sizeof(Chunk<E, VEC>) == 16) {
+    uint4 x = __builtin_bit_cast(uint4, c);
+    asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w));
+    c = __builtin_bit_cast(Chunk<E, VEC>, x);
+  }
 }
 
 __device__ __forceinline__ float load_w(const void* w, int type, int i) {
@@ -111,134 +117,250 @@ __device__ __forceinline__ void turn(float* a, float* b, const float* c, const f
   }
 }
 
-// the frequencies (in turns per position) of a lane's VEC pairs; -1 stands for "does not turn"
-template <int VEC, bool INSIDE>
-__device__ __forceinline__ void pair_freqs(const RotDesc& d, int a, int b, int item, double* f) {
+// One lane's share of a head: its items' chunks, which of them exist, and where their pairs' cos and sin lie in Staged
+template <int VEC, int ITEMS, bool INSIDE>
+struct Lane {
+  int ca[ITEMS], cb[ITEMS];              // first elements, 0 where there is no such chunk
+  bool ha[ITEMS], hb[ITEMS];
+  int fa[ITEMS], fb[ITEMS];              // first pair (INSIDE: of each chunk); NOTURN: these do not turn
+
+  __device__ __forceinline__ Lane(const RotDesc& d, int il, int lph) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    int p;
-    if (INSIDE) {
-      const int e = i < VEC / 2 ? a : b;
-      p = e >= 0 && e < d.R ? e / 2 + i % (VEC / 2) : -1;
-    } else {
-      p = a >= 0 && a < d.R ? (VEC == 1 ? item : a + i) : -1;
+    for (int it = 0; it < ITEMS; ++it) {
+      int a, b;
+      item_chunks<VEC>(il + it * lph, d.D, d.R, d.inter, a, b);
+      ha[it] = a >= 0;
+      hb[it] = b >= 0;
+      ca[it] = max(a, 0);
+      cb[it] = max(b, 0);
+      fa[it] = a < 0 || a >= d.R ? NOTURN : INSIDE ? a / 2 : VEC == 1 ? il + it * lph : a;
+      fb[it] = b < 0 || b >= d.R ? NOTURN : b / 2;
     }
-    f[i] = p >= 0 ? d.freqs[p] * 0.15915494309189535 : -1.0;
   }
+};
+
+// Shared memory of a block: norm weights (fp32), frequencies (turns per position), and each wave's cos and sin of the
+// pairs of its token, times mscale; behind them a pair that does not turn
+struct Staged {
+  float w[2][512];
+  double f[256];
+  float c[NTH / 64][NOTURN + 8], s[NTH / 64][NOTURN + 8];
+};
+
+// an offset of 0 that the compiler cannot see through: reads of Staged at it stay where they are written. Hoisted out of
+// the loops, as it would have them, they hold 32 to 48 registers a lane and spill
+__device__ __forceinline__ int here() {
+  int z = 0;
+  asm volatile("" : "+s"(z));
+  return z;
 }
 
-template <int VEC>
-__device__ __forceinline__ void angles(const double* f, double pos, float m, float sign, float* c, float* s) {
+__device__ __forceinline__ void stage(const RotDesc& d, Staged& s) {
+  for (int i = threadIdx.x; i < d.D; i += NTH) {
+    if (d.wq) s.w[0][i] = load_w(d.wq, d.wtype, i);
+    if (d.wk) s.w[1][i] = load_w(d.wk, d.wtype, i);
+  }
+  if ((int)threadIdx.x < d.R / 2) s.f[threadIdx.x] = d.freqs[threadIdx.x] * 0.15915494309189535;
+  if (threadIdx.x < 32) {
+    s.c[threadIdx.x >> 3][NOTURN + (threadIdx.x & 7)] = 1.f;
+    s.s[threadIdx.x >> 3][NOTURN + (threadIdx.x & 7)] = 0.f;
+  }
+  __syncthreads();
+}
+
+// cos and sin of a token's angles, a pair a lane, through shared memory for all of the wave's heads (each lane forming
+// those of its own pairs, eight times over in a wave of eight heads, took half of the forward's instructions). The angle is
+// reduced in 64 bits to a quarter turn r in [-1/2, 1/2] and its quadrant; there the Taylor polynomials of sin and
+// cos(pi r / 2) to the 9th and 10th power are off by less than 2^-28
+__device__ __forceinline__ void turn_angles(const RotDesc& d, Staged& sh, int w, double pos, float sign) {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the wave's reads of its last token's are done
+  for (int i = threadIdx.x & 63; i < d.R / 2; i += 64) {
+    double t = pos * sh.f[i];
+    t = 4.0 * (t - rint(t));
+    const double k = rint(t);
+    const float r = (float)(t - k), r2 = r * r;
+    const int q = (int)k;
+    const float sn = r * (1.5707963267948966f + r2 * (-0.6459640975062462f + r2 * (0.07969262624616704f +
+                     r2 * (-0.004681754135318688f + r2 * 0.00016044118478735982f))));
+    const float cs = 1.f + r2 * (-1.2337005501361697f + r2 * (0.2536695079010480f + r2 * (-0.02086348076335296f +
+                     r2 * (0.0009192602748394266f + r2 * -2.5202042373060605e-05f))));
+    const float u = q & 1 ? cs : sn, v = q & 1 ? sn : cs;
+    sh.c[w][i] = d.mscale * (q + 1 & 2 ? -v : v);
+    sh.s[w][i] = d.mscale * sign * (q & 2 ? -u : u);
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// a lane's VEC pairs of them
+template <int VEC, bool INSIDE>
+__device__ __forceinline__ void read_angles(const float* t, int fa, int fb, float* o) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    const double t = pos * f[i];
-    const float x = 2.f * (float)(t - rint(t));
-    float sn, cs;
-    sincospif(x, &sn, &cs);
-    const bool on = f[i] >= 0.0;
-    c[i] = on ? m * cs : 1.f;
-    s[i] = on ? sign * m * sn : 0.f;
-  }
+  for (int i = 0; i < VEC; ++i) o[i] = INSIDE && i >= VEC / 2 ? t[fb + i - VEC / 2] : t[fa + i];
 }
 
+template <int CTRL>
+__device__ __forceinline__ float dpp_mov(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, false));
+}
+// sum over the lph (a power of two) lanes of a head; every lane of the wave takes part
 __device__ __forceinline__ float sum_lanes(float v, int lph) {
-  for (int o = lph >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if (lph > 1) v += dpp_mov<0xB1>(v);    // lane ^ 1
+  if (lph > 2) v += dpp_mov<0x4E>(v);    // lane ^ 2
+  if (lph > 4) v += dpp_mov<0x141>(v);   // the other four of eight
+  if (lph > 8) v += dpp_mov<0x140>(v);   // the other eight of sixteen
+  if (lph > 16) v += __shfl_xor(v, 16, 64);
+  if (lph > 32) v += __shfl_xor(v, 32, 64);
   return v;
 }
 
-// ---- forward. A unit is U passes of 64 / LPH heads of one token; heads are q's, then k's, then (CACHE) v's.
-template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool CACHE>
-__global__ __launch_bounds__(NTH) void rotary_fwd_kernel(const RotDesc d, int lph, int npg) {
-  typedef typename Elem<TYPE>::t E;
-  const int lane = threadIdx.x & 63, hl = lane / lph, il = lane % lph, hpw = 64 / lph;
-  const int heads = d.Hq + d.Hk + (CACHE ? d.Hk : 0);
-  int ca[ITEMS], cb[ITEMS];
-  double f[ITEMS][VEC];
-  float wa[2][ITEMS][VEC], wb[2][ITEMS][VEC];
+// values into their columns of eight tokens: V cache [P][Hk][page / 8][D][8]. A wave takes one token and VCH pieces
+// of 64 * EV elements of its heads. Eight tokens of the step that fill one column block, slots 8 j .. 8 j + 7, are
+// written together by the first of them, 16 bytes (32) at a time; the others of the eight have nothing left to do.
+// Tokens outside such a run (a decode step's, a run's ragged ends) write their elements one by one.
+constexpr int VCH = 4;
+
+template <typename E, int EV>
+__device__ void append_values(const RotDesc& d, long long unit, int nvg) {
+  const int lane = threadIdx.x & 63;
+  const long long t = unit / nvg;
+  const long long slot = d.slots[t];
+  if (slot < 0 || slot >= d.nslots) return;
+  const int off = (int)(slot % 8);
+  const long long t0 = t - off;
+  bool mine = true;
+  if (lane < 8) mine = t0 + lane >= 0 && t0 + lane < d.T && d.slots[max(0LL, min(t0 + lane, d.T - 1))] == slot - off + lane;
+  const bool run = __all(mine);
+  if (run && off != 0) return;
+  const long long page = slot / d.page;
+  const int o8 = (int)(slot % d.page) / 8;
+  const E* v = (const E*)d.v + t * d.v_ts;
+  const int n = d.Hk * d.D, e0 = (int)(unit % nvg) * VCH * 64 * EV + lane * EV;
+  if (run) {
 #pragma unroll
-  for (int it = 0; it < ITEMS; ++it) {
-    item_chunks<VEC>(il + it * lph, d.D, d.R, d.inter, ca[it], cb[it]);
-    pair_freqs<VEC, INSIDE>(d, ca[it], cb[it], il + it * lph, f[it]);
+    for (int i = 0; i < VCH; ++i) {
+      const int e = e0 + i * 64 * EV;
+      if (e >= n) return;
+      const int h = e / d.D, c = e % d.D;
+      Chunk<E, EV> x[8];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
+      for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const Chunk<E, EV>*>(v + j * d.v_ts + h * d.v_hs + c);
+      E* o = (E*)d.vo + (((page * d.Hk + h) * (d.page / 8) + o8) * d.D + c) * 8;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const void* w = j ? d.wk : d.wq;
-        wa[j][it][i] = w && ca[it] >= 0 ? load_w(w, d.wtype, ca[it] + i) : 1.f;
-        wb[j][it][i] = w && cb[it] >= 0 ? load_w(w, d.wtype, cb[it] + i) : 1.f;
+      for (int k = 0; k < EV; ++k) {
+        Chunk<E, 8> y;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y.e[j] = x[j].e[k];
+        *reinterpret_cast<Chunk<E, 8>*>(o + 8 * k) = y;
       }
     }
+    return;
   }
+  Chunk<E, EV> x[VCH];
+#pragma unroll
+  for (int i = 0; i < VCH; ++i) {
+    const int e = min(e0 + i * 64 * EV, n - EV);
+    x[i] = *reinterpret_cast<const Chunk<E, EV>*>(v + e / d.D * d.v_hs + e % d.D);
+  }
+#pragma unroll
+  for (int i = 0; i < VCH; ++i) {
+    const int e = e0 + i * 64 * EV;
+    if (e >= n) return;
+    E* o = (E*)d.vo + (((page * d.Hk + e / d.D) * (d.page / 8) + o8) * d.D + e % d.D) * 8 + off;
+#pragma unroll
+    for (int k = 0; k < EV; ++k) o[8 * k] = x[i].e[k];
+  }
+}
+
+// ---- forward. A wave's unit is U passes of one token; a pass is 64 / lph heads, all of q or all of k. CACHE: k goes
+// into the pages, and the blocks behind the first `rot` write the values.
+template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool CACHE, int EV>
+__global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int lph, int pq, int pk, int rot, int nvg) {
+  typedef typename Elem<TYPE>::t E;
+  __shared__ Staged sh;
+  if (CACHE && (int)blockIdx.x >= rot) {
+    const long long units = d.T * nvg, nw = (long long)(gridDim.x - rot) * (NTH / 64);
+    for (long long u = (long long)(blockIdx.x - rot) * (NTH / 64) + (threadIdx.x >> 6); u < units; u += nw)
+      append_values<E, EV>(d, u, nvg);
+    return;
+  }
+  const int lane = threadIdx.x & 63, hl = lane / lph, il = lane % lph, hpw = 64 / lph;
+  const int np = pq + pk, npg = (np + U - 1) / U;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Lane<VEC, ITEMS, INSIDE> ln(d, il, lph);
+  stage(d, sh);
   const float inv_d = 1.f / d.D;
-  const long long units = d.T * npg, nw = (long long)gridDim.x * (NTH / 64);
-  for (long long u = (long long)blockIdx.x * (NTH / 64) + (threadIdx.x >> 6); u < units; u += nw) {
+  const long long units = d.T * npg, nw = (long long)rot * (NTH / 64);
+  for (long long u = (long long)blockIdx.x * (NTH / 64) + wave; u < units; u += nw) {
     const long long t = u / npg;
-    const int h0 = (int)(u % npg) * U * hpw + hl;
-    float a[U][ITEMS][VEC], b[U][ITEMS][VEC];
+    const int p0 = (int)(u % npg) * U;
+    Chunk<E, VEC> xa[U][ITEMS], xb[U][ITEMS];
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      const int h = h0 + p * hpw;
-      const E* x = h < d.Hq ? (const E*)d.q + t * d.q_ts + h * d.q_hs
-                   : h < d.Hq + d.Hk ? (const E*)d.k + t * d.k_ts + (h - d.Hq) * d.k_hs
-                                     : (const E*)d.v + t * d.v_ts + (h - d.Hq - d.Hk) * d.v_hs;
+      if (p0 + p >= np) break;
+      const bool isq = p0 + p < pq;
+      const int H = isq ? d.Hq : d.Hk, h = min((p0 + p - (isq ? 0 : pq)) * hpw + hl, H - 1);
+      const E* x = isq ? (const E*)d.q + t * d.q_ts + h * d.q_hs : (const E*)d.k + t * d.k_ts + h * d.k_hs;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
-        load<E, VEC>(x + ca[it], (const E*)d.q, h < heads && ca[it] >= 0, a[p][it]);
-        load<E, VEC>(x + cb[it], (const E*)d.q, h < heads && cb[it] >= 0, b[p][it]);
+        xa[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.ca[it]);
+        xb[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.cb[it]);
       }
     }
+    const double pos = (double)d.pos[t];
     const long long slot = CACHE ? d.slots[t] : 0;
-    const bool live = CACHE && slot >= 0 && slot < d.nslots;
+    const bool live = !CACHE || (slot >= 0 && slot < d.nslots);
     const long long page = CACHE ? slot / d.page : 0;
     const int off = CACHE ? (int)(slot % d.page) : 0;
-    float c[ITEMS][VEC], s[ITEMS][VEC];
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it) angles<VEC>(f[it], (double)d.pos[t], d.mscale, 1.f, c[it], s[it]);
+    turn_angles(d, sh, wave, pos, 1.f);
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      const int h = h0 + p * hpw;
-      const bool isq = h < d.Hq;
-      if (CACHE && h >= d.Hq + d.Hk) {             // a value head: as it is, into its column of eight tokens
-        if (h < heads && live) {
-          E* o = (E*)d.vo + ((page * d.Hk + (h - d.Hq - d.Hk)) * (d.page / 8) + off / 8) * 8LL * d.D + off % 8;
+      if (p0 + p >= np) break;
+      const bool isq = p0 + p < pq;
+      const int H = isq ? d.Hq : d.Hk, h = (p0 + p - (isq ? 0 : pq)) * hpw + hl;
+      float a[ITEMS][VEC], b[ITEMS][VEC];
 #pragma unroll
-          for (int it = 0; it < ITEMS; ++it) {
+      for (int it = 0; it < ITEMS; ++it)
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-              if (ca[it] >= 0) from_f(a[p][it][i], o[(ca[it] + i) * 8LL]);
-              if (cb[it] >= 0) from_f(b[p][it][i], o[(cb[it] + i) * 8LL]);
-            }
-          }
+        for (int i = 0; i < VEC; ++i) {
+          a[it][i] = to_f(xa[p][it].e[i]);
+          b[it][i] = to_f(xb[p][it].e[i]);
         }
-        continue;
-      }
       if (isq ? d.wq != nullptr : d.wk != nullptr) {
+        const float* w = sh.w[isq ? 0 : 1] + here();
         float ss = 0.f;
 #pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
+        for (int it = 0; it < ITEMS; ++it) {
+          float sa = 0.f, sb = 0.f;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) ss += a[p][it][i] * a[p][it][i] + b[p][it][i] * b[p][it][i];
-        ss = sum_lanes(ss, lph);
-        const float r = rsqrtf(ss * inv_d + d.eps);
+          for (int i = 0; i < VEC; ++i) {
+            sa += a[it][i] * a[it][i];
+            sb += b[it][i] * b[it][i];
+          }
+          ss += (ln.ha[it] ? sa : 0.f) + (ln.hb[it] ? sb : 0.f);
+        }
+        const float r = rsqrtf(sum_lanes(ss, lph) * inv_d + d.eps);
 #pragma unroll
         for (int it = 0; it < ITEMS; ++it)
 #pragma unroll
           for (int i = 0; i < VEC; ++i) {
-            a[p][it][i] *= r * (isq ? wa[0][it][i] : wa[1][it][i]);
-            b[p][it][i] *= r * (isq ? wb[0][it][i] : wb[1][it][i]);
+            a[it][i] *= r * w[ln.ca[it] + i];
+            b[it][i] *= r * w[ln.cb[it] + i];
           }
       }
-      if (h >= heads) continue;
+      if (h >= H || (!isq && !live)) continue;
       E* o;
       if (isq) o = (E*)d.qo + (t * d.Hq + h) * d.D;
-      else if (CACHE) o = (E*)d.ko + ((page * d.Hk + (h - d.Hq)) * d.page + off) * d.D;
-      else o = (E*)d.ko + (t * d.Hk + (h - d.Hq)) * d.D;
-      if (CACHE && !isq && !live) continue;
+      else if (CACHE) o = (E*)d.ko + ((page * d.Hk + h) * d.page + off) * d.D;
+      else o = (E*)d.ko + (t * d.Hk + h) * d.D;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
-        turn<VEC, INSIDE>(a[p][it], b[p][it], c[it], s[it]);
-        if (ca[it] >= 0) store<E, VEC>(o + ca[it], a[p][it]);
-        if (cb[it] >= 0) store<E, VEC>(o + cb[it], b[p][it]);
+        float c[VEC], s[VEC];
+        const int z = here();
+        read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
+        read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
+        turn<VEC, INSIDE>(a[it], b[it], c, s);
+        if (ln.ha[it]) store<E, VEC>(o + ln.ca[it], a[it]);
+        if (ln.hb[it]) store<E, VEC>(o + ln.cb[it], b[it]);
       }
     }
   }
@@ -247,149 +369,154 @@ __global__ __launch_bounds__(NTH) void rotary_fwd_kernel(const RotDesc d, int lp
 // ---- backward: as the forward, gradients in place of inputs; x is read again where it was normed. NORM: either of q
 // and k has a weight. Weight gradients: each lane sums its own elements over its units in 32 bits, a block adds its
 // lanes and waves in a fixed order into part[block], rotary_fold_kernel the blocks: no atomics, the same bits each run.
+// With sums to keep, a block works on one tensor (the first nbq on q): sums for both took 16 more registers a lane and
+// spilled.
 template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool NORM>
-__global__ __launch_bounds__(NTH) void rotary_bwd_kernel(const RotDesc d, int lph, int npg) {
+__global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int lph, int pq, int pk, int nbq) {
   typedef typename Elem<TYPE>::t E;
+  __shared__ Staged sh;
   const int lane = threadIdx.x & 63, hl = lane / lph, il = lane % lph, hpw = 64 / lph;
-  const int heads = d.Hq + d.Hk;
-  int ca[ITEMS], cb[ITEMS];
-  double f[ITEMS][VEC];
-  float wa[2][ITEMS][VEC], wb[2][ITEMS][VEC], da[2][ITEMS][VEC], db[2][ITEMS][VEC];
+  const bool block_q = (int)blockIdx.x < nbq;
+  const int pb = NORM && !block_q ? pq : 0, np = !NORM ? pq + pk : block_q ? pq : pk, npg = (np + U - 1) / U;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Lane<VEC, ITEMS, INSIDE> ln(d, il, lph);
+  stage(d, sh);
+  float da[ITEMS][VEC], db[ITEMS][VEC];
 #pragma unroll
-  for (int it = 0; it < ITEMS; ++it) {
-    item_chunks<VEC>(il + it * lph, d.D, d.R, d.inter, ca[it], cb[it]);
-    pair_freqs<VEC, INSIDE>(d, ca[it], cb[it], il + it * lph, f[it]);
-    if (NORM) {
+    for (int it = 0; it < ITEMS; ++it)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const void* w = j ? d.wk : d.wq;
-          wa[j][it][i] = w && ca[it] >= 0 ? load_w(w, d.wtype, ca[it] + i) : 1.f;
-          wb[j][it][i] = w && cb[it] >= 0 ? load_w(w, d.wtype, cb[it] + i) : 1.f;
-          da[j][it][i] = db[j][it][i] = 0.f;
-        }
-      }
-    }
-  }
+      for (int i = 0; i < VEC; ++i) da[it][i] = db[it][i] = 0.f;
   const float inv_d = 1.f / d.D;
-  const long long units = d.T * npg, nw = (long long)gridDim.x * (NTH / 64);
-  for (long long u = (long long)blockIdx.x * (NTH / 64) + (threadIdx.x >> 6); u < units; u += nw) {
+  const int b0 = NORM && !block_q ? nbq : 0, nb = !NORM ? gridDim.x : block_q ? nbq : gridDim.x - nbq;
+  const long long units = d.T * npg, nw = (long long)nb * (NTH / 64);
+  for (long long u = (long long)(blockIdx.x - b0) * (NTH / 64) + wave; u < units; u += nw) {
     const long long t = u / npg;
-    const int h0 = (int)(u % npg) * U * hpw + hl;
-    float a[U][ITEMS][VEC], b[U][ITEMS][VEC], xa[U][ITEMS][VEC], xb[U][ITEMS][VEC];
+    const int p0 = (int)(u % npg) * U;
+    Chunk<E, VEC> ga[U][ITEMS], gb[U][ITEMS], xa[U][ITEMS], xb[U][ITEMS];
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      const int h = h0 + p * hpw;
-      const bool isq = h < d.Hq, on = h < heads;
-      const E* g = isq ? (const E*)d.gq + t * d.gq_ts + h * d.gq_hs : (const E*)d.gk + t * d.gk_ts + (h - d.Hq) * d.gk_hs;
-      const E* x = isq ? (const E*)d.q + t * d.q_ts + h * d.q_hs : (const E*)d.k + t * d.k_ts + (h - d.Hq) * d.k_hs;
-      const bool nrm = NORM && on && (isq ? d.wq != nullptr : d.wk != nullptr);
+      if (p0 + p >= np) break;
+      const bool isq = NORM ? block_q : p0 + p < pq;
+      const int H = isq ? d.Hq : d.Hk, h = min((pb + p0 + p - (isq ? 0 : pq)) * hpw + hl, H - 1);
+      const E* g = isq ? (const E*)d.gq + t * d.gq_ts + h * d.gq_hs : (const E*)d.gk + t * d.gk_ts + h * d.gk_hs;
+      const E* x = isq ? (const E*)d.q + t * d.q_ts + h * d.q_hs : (const E*)d.k + t * d.k_ts + h * d.k_hs;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
-        load<E, VEC>(g + ca[it], (const E*)d.gq, on && ca[it] >= 0, a[p][it]);
-        load<E, VEC>(g + cb[it], (const E*)d.gq, on && cb[it] >= 0, b[p][it]);
+        ga[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(g + ln.ca[it]);
+        gb[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(g + ln.cb[it]);
         if (NORM) {
-          load<E, VEC>(x + ca[it], (const E*)d.q, nrm && ca[it] >= 0, xa[p][it]);
-          load<E, VEC>(x + cb[it], (const E*)d.q, nrm && cb[it] >= 0, xb[p][it]);
+          xa[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.ca[it]);
+          xb[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.cb[it]);
         }
       }
     }
-    float c[ITEMS][VEC], s[ITEMS][VEC];
-#pragma unroll
-    for (int it = 0; it < ITEMS; ++it) angles<VEC>(f[it], (double)d.pos[t], d.mscale, -1.f, c[it], s[it]);
+    const double pos = (double)d.pos[t];
+    turn_angles(d, sh, wave, pos, -1.f);
 #pragma unroll
     for (int p = 0; p < U; ++p) {
-      const int h = h0 + p * hpw;
-      const bool isq = h < d.Hq, on = h < heads;
-#pragma unroll
-      for (int it = 0; it < ITEMS; ++it) turn<VEC, INSIDE>(a[p][it], b[p][it], c[it], s[it]);
-      if (NORM) {
-        const bool nrm = on && (isq ? d.wq != nullptr : d.wk != nullptr);
-        float ss = 0.f;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) ss += xa[p][it][i] * xa[p][it][i] + xb[p][it][i] * xb[p][it][i];
-        ss = sum_lanes(ss, lph);
-        const float r = nrm ? rsqrtf(ss * inv_d + d.eps) : 0.f;
-        float hu = 0.f;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            xa[p][it][i] *= r;                        // u
-            xb[p][it][i] *= r;
-            const float ga = a[p][it][i] * xa[p][it][i], gb = b[p][it][i] * xb[p][it][i];   // 0 without a norm
-            da[0][it][i] += isq ? ga : 0.f;
-            da[1][it][i] += isq ? 0.f : ga;
-            db[0][it][i] += isq ? gb : 0.f;
-            db[1][it][i] += isq ? 0.f : gb;
-            const float va = isq ? wa[0][it][i] : wa[1][it][i], vb = isq ? wb[0][it][i] : wb[1][it][i];
-            hu += ga * va + gb * vb;
-            a[p][it][i] *= va;                        // h
-            b[p][it][i] *= vb;
-          }
-        hu = sum_lanes(hu, lph) * inv_d;
-        const float rr = nrm ? r : 1.f;
-#pragma unroll
-        for (int it = 0; it < ITEMS; ++it)
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            a[p][it][i] = rr * (a[p][it][i] - xa[p][it][i] * hu);
-            b[p][it][i] = rr * (b[p][it][i] - xb[p][it][i] * hu);
-          }
-      }
-      if (!on) continue;
-      E* o = isq ? (E*)d.qo + (t * d.Hq + h) * d.D : (E*)d.ko + (t * d.Hk + (h - d.Hq)) * d.D;
+      if (p0 + p >= np) break;
+      const bool isq = NORM ? block_q : p0 + p < pq;
+      const int H = isq ? d.Hq : d.Hk, h = (pb + p0 + p - (isq ? 0 : pq)) * hpw + hl;
+      float a[ITEMS][VEC], b[ITEMS][VEC];
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
-        if (ca[it] >= 0) store<E, VEC>(o + ca[it], a[p][it]);
-        if (cb[it] >= 0) store<E, VEC>(o + cb[it], b[p][it]);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          a[it][i] = to_f(ga[p][it].e[i]);
+          b[it][i] = to_f(gb[p][it].e[i]);
+        }
+        float c[VEC], s[VEC];
+        const int z = here();
+        read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
+        read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
+        turn<VEC, INSIDE>(a[it], b[it], c, s);
+      }
+      if (NORM && (isq ? d.wq != nullptr : d.wk != nullptr)) {
+        // with p = sum x^2 and e = sum g w x:  u = x r,  dx = r g w - (e r^3 / D) x,  dw += g x r
+        const float* w = sh.w[isq ? 0 : 1] + here();
+        float ss = 0.f, e = 0.f;
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+          float sa = 0.f, sb = 0.f, ea = 0.f, eb = 0.f;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float ya = to_f(xa[p][it].e[i]), yb = to_f(xb[p][it].e[i]);
+            sa += ya * ya;
+            sb += yb * yb;
+            ea += a[it][i] * w[ln.ca[it] + i] * ya;
+            eb += b[it][i] * w[ln.cb[it] + i] * yb;
+          }
+          ss += (ln.ha[it] ? sa : 0.f) + (ln.hb[it] ? sb : 0.f);
+          e += (ln.ha[it] ? ea : 0.f) + (ln.hb[it] ? eb : 0.f);
+        }
+        ss = sum_lanes(ss, lph);
+        e = sum_lanes(e, lph);
+        // lanes past the last head repeat it for their loads: nothing of theirs may reach the weight sums
+        const float r = rsqrtf(ss * inv_d + d.eps), rw = h < H ? r : 0.f, k = e * inv_d * r * r * r;
+        w = sh.w[isq ? 0 : 1] + here();
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+          forget(xa[p][it]);                          // x is widened again rather than kept in 32 bits
+          forget(xb[p][it]);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float ya = to_f(xa[p][it].e[i]), yb = to_f(xb[p][it].e[i]);
+            da[it][i] += a[it][i] * (ya * rw);
+            db[it][i] += b[it][i] * (yb * rw);
+            a[it][i] = a[it][i] * (r * w[ln.ca[it] + i]) - k * ya;
+            b[it][i] = b[it][i] * (r * w[ln.cb[it] + i]) - k * yb;
+          }
+        }
+      }
+      if (h >= H) continue;
+      E* o = isq ? (E*)d.qo + (t * d.Hq + h) * d.D : (E*)d.ko + (t * d.Hk + h) * d.D;
+#pragma unroll
+      for (int it = 0; it < ITEMS; ++it) {
+        if (ln.ha[it]) store<E, VEC>(o + ln.ca[it], a[it]);
+        if (ln.hb[it]) store<E, VEC>(o + ln.cb[it], b[it]);
       }
     }
   }
   if (!NORM) return;
-  __shared__ float red[NTH / 64][2][512];
+  __shared__ float red[NTH / 64][512];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int it = 0; it < ITEMS; ++it) {
 #pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        float x = da[j][it][i], y = db[j][it][i];
-        for (int o = lph; o < 64; o <<= 1) {
-          x += __shfl_xor(x, o, 64);
-          y += __shfl_xor(y, o, 64);
-        }
-        if (hl == 0 && ca[it] >= 0) red[threadIdx.x >> 6][j][ca[it] + i] = x;
-        if (hl == 0 && cb[it] >= 0) red[threadIdx.x >> 6][j][cb[it] + i] = y;
+    for (int i = 0; i < VEC; ++i) {
+      float x = da[it][i], y = db[it][i];
+      for (int o = lph; o < 64; o <<= 1) {
+        x += __shfl_xor(x, o, 64);
+        y += __shfl_xor(y, o, 64);
       }
+      if (hl == 0 && ln.ha[it]) red[threadIdx.x >> 6][ln.ca[it] + i] = x;
+      if (hl == 0 && ln.hb[it]) red[threadIdx.x >> 6][ln.cb[it] + i] = y;
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < 2 * d.D; e += NTH) {
-    const int j = e / d.D, i = e % d.D;
+  for (int i = threadIdx.x; i < d.D; i += NTH) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < NTH / 64; ++w) v += red[w][j][i];
-    d.part[((long long)blockIdx.x * 2 + j) * d.D + i] = v;
+    for (int w = 0; w < NTH / 64; ++w) v += red[w][i];
+    d.part[(long long)blockIdx.x * d.D + i] = v;
   }
 }
 
-// weight gradients from the blocks' partials: 64 columns a block, 16 waves each over every 16th row
-__global__ __launch_bounds__(1024) void rotary_fold_kernel(const RotDesc d, int nblocks) {
-  __shared__ float red[16][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, e = blockIdx.x * 64 + lane;
+// weight gradients from the blocks' partials: 16 columns a block, 64 rows of it side by side, in a fixed order
+__global__ __launch_bounds__(1024) void rotary_fold_kernel(const RotDesc d, int nbq, int nb) {
+  __shared__ float red[64][17];
+  const int col = threadIdx.x & 15, row = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
   float v = 0.f;
-  if (e < 2 * d.D)
-    for (int r = w; r < nblocks; r += 16) v += d.part[(long long)r * 2 * d.D + e];
-  red[w][lane] = v;
+  if (e < 2 * d.D) {
+#pragma unroll 4
+    for (int r = row + (e < d.D ? 0 : nbq); r < (e < d.D ? nbq : nb); r += 64)
+      v += d.part[(long long)r * d.D + (e < d.D ? e : e - d.D)];
+  }
+  red[row][col] = v;
   __syncthreads();
-  if (w != 0 || e >= 2 * d.D) return;
+  if (threadIdx.x >= 16 || e >= 2 * d.D) return;
   v = 0.f;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v += red[i][lane];
+  for (int i = 0; i < 64; ++i) v += red[i][col];
   void* o = e < d.D ? d.dwq : d.dwk;
   const int i = e < d.D ? e : e - d.D;
   if (!o) return;
@@ -421,30 +548,77 @@ int pow2_at_least(int n) {
   return p;
 }
 
-constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024;   // the backward's count also sizes its partials
+// the backward's block count also sizes its partials
+constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024;
+
+struct Passes {
+  int hpw, pq, pk;
+  Passes(const RotDesc& d, int lph) : hpw(64 / lph), pq((d.Hq + hpw - 1) / hpw), pk((d.Hk + hpw - 1) / hpw) {}
+  static int blocks(long long units, int most) {
+    const long long b = (units + 3) / 4;
+    return (int)(b < most ? b : most);
+  }
+};
 
 template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE>
-int launch(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
-  const int heads = d.Hq + d.Hk + (d.slots ? d.Hk : 0), per = (64 / lph) * U, npg = (heads + per - 1) / per;
-  const long long blocks = (d.T * npg + 3) / 4;
-  if (!bwd) {
-    const int grid = (int)(blocks < FWD_BLOCKS ? blocks : FWD_BLOCKS);
-    if (d.slots)
-      hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, true>), dim3(grid), dim3(NTH), 0, st, d, lph, npg);
-    else
-      hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false>), dim3(grid), dim3(NTH), 0, st, d, lph, npg);
+int forward(const RotDesc& d, int lph, hipStream_t st) {
+  const Passes p(d, lph);
+  const int grid = Passes::blocks(d.T * ((p.pq + p.pk + U - 1) / U), FWD_BLOCKS);
+  if (!d.slots) {
+    hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false, 1>), dim3(grid), dim3(NTH), 0, st, d, lph,
+                       p.pq, p.pk, grid, 0);
     return (int)hipGetLastError();
   }
-  const int grid = (int)(blocks < BWD_BLOCKS ? blocks : BWD_BLOCKS);
-  if (d.wq || d.wk) {
-    hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, true>), dim3(grid), dim3(NTH), 0, st, d, lph, npg);
-    const int rc = (int)hipGetLastError();
-    if (rc) return rc;
-    hipLaunchKernelGGL(rotary_fold_kernel, dim3((2 * d.D + 63) / 64), dim3(1024), 0, st, d, grid);
-  } else {
-    hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false>), dim3(grid), dim3(NTH), 0, st, d, lph, npg);
-  }
+  constexpr int EV = VEC == 1 ? 1 : 2;                     // VEC > 1: D and the strides are even
+  const int nvg = (d.Hk * d.D + VCH * 64 * EV - 1) / (VCH * 64 * EV), vgrid = Passes::blocks(d.T * nvg, FWD_BLOCKS);
+  hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, true, EV>), dim3(grid + vgrid), dim3(NTH), 0, st, d,
+                     lph, p.pq, p.pk, grid, nvg);
   return (int)hipGetLastError();
+}
+
+template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE>
+int backward(const RotDesc& d, int lph, hipStream_t st) {
+  const Passes p(d, lph);
+  const int grid = Passes::blocks(d.T * ((p.pq + p.pk + U - 1) / U), BWD_BLOCKS);
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false>), dim3(grid), dim3(NTH), 0, st, d, lph, p.pq,
+                     p.pk, 0);
+  return (int)hipGetLastError();
+}
+
+template <int TYPE, int VEC, int ITEMS, bool INSIDE>
+int backward_normed(const RotDesc& d, int lph, hipStream_t st) {
+  const Passes p(d, lph);
+  // blocks for q and for k, as many as their units ask for
+  const long long bq = (d.T * p.pq + 3) / 4, bk = (d.T * p.pk + 3) / 4;
+  int nq = (int)bq, nk = (int)bk;
+  if (bq + bk > BWD_BLOCKS) {
+    nq = BWD_BLOCKS * p.pq / (p.pq + p.pk);
+    nq = nq < 1 ? 1 : nq > BWD_BLOCKS - 1 ? BWD_BLOCKS - 1 : nq;
+    nk = BWD_BLOCKS - nq;
+  }
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, 1, INSIDE, true>), dim3(nq + nk), dim3(NTH), 0, st, d, lph, p.pq,
+                     p.pk, nq);
+  const int rc = (int)hipGetLastError();
+  if (rc) return rc;
+  hipLaunchKernelGGL(rotary_fold_kernel, dim3((2 * d.D + 15) / 16), dim3(1024), 0, st, d, nq, nq + nk);
+  return (int)hipGetLastError();
+}
+
+// Passes a unit. Four share one token's angles and keep four rows of loads in flight; under 1024 tokens one each spreads
+// them over more waves. The normed backward takes one: a second pass' loads and the sums leave it three waves a SIMD
+// (199 us where one pass takes 164, at 32768 tokens, 2 x 16 heads x 128 in bf16).
+template <int TYPE, int VEC, bool INSIDE>
+int by_tokens(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
+  const bool few = d.T < 1024;
+  if (!bwd) return few ? forward<TYPE, VEC, 1, 1, INSIDE>(d, lph, st) : forward<TYPE, VEC, 1, 4, INSIDE>(d, lph, st);
+  if (d.wq || d.wk) return backward_normed<TYPE, VEC, 1, INSIDE>(d, lph, st);
+  return few ? backward<TYPE, VEC, 1, 1, INSIDE>(d, lph, st) : backward<TYPE, VEC, 1, 4, INSIDE>(d, lph, st);
+}
+
+template <int TYPE, int ITEMS>
+int by_element(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
+  if (!bwd) return forward<TYPE, 1, ITEMS, 1, false>(d, lph, st);
+  return d.wq || d.wk ? backward_normed<TYPE, 1, ITEMS, false>(d, lph, st) : backward<TYPE, 1, ITEMS, 1, false>(d, lph, st);
 }
 
 template <int TYPE>
@@ -452,11 +626,10 @@ int dispatch(const RotDesc& d, bool bwd, hipStream_t st) {
   constexpr int V = Elem<TYPE>::VEC;
   if (vec_ok(d, V, bwd)) {
     const int lph = pow2_at_least(items_of(d, V));
-    return d.inter ? launch<TYPE, V, 1, 2, true>(d, bwd, lph, st) : launch<TYPE, V, 1, 2, false>(d, bwd, lph, st);
+    return d.inter ? by_tokens<TYPE, V, true>(d, bwd, lph, st) : by_tokens<TYPE, V, false>(d, bwd, lph, st);
   }
   const int n = items_of(d, 1);
-  if (n <= 64) return launch<TYPE, 1, 1, 1, false>(d, bwd, pow2_at_least(n), st);
-  return launch<TYPE, 1, 4, 1, false>(d, bwd, 64, st);
+  return n <= 64 ? by_element<TYPE, 1>(d, bwd, pow2_at_least(n), st) : by_element<TYPE, 4>(d, bwd, 64, st);
 }
 
 int run(const RotDesc* d, bool bwd, hipStream_t st) {
@@ -466,7 +639,7 @@ int run(const RotDesc* d, bool bwd, hipStream_t st) {
   if (d->slots && (d->page < 8 || d->page % 8 || d->nslots < 0)) return -2;
   if (d->T == 0) {                         // no tokens: the weight gradients are zero
     if (!bwd || !(d->wq || d->wk)) return 0;
-    hipLaunchKernelGGL(rotary_fold_kernel, dim3((2 * d->D + 63) / 64), dim3(1024), 0, st, *d, 0);
+    hipLaunchKernelGGL(rotary_fold_kernel, dim3((2 * d->D + 15) / 16), dim3(1024), 0, st, *d, 0, 0);
     return (int)hipGetLastError();
   }
   switch (d->dtype) {
@@ -481,4 +654,4 @@ int run(const RotDesc* d, bool bwd, hipStream_t st) {
 OBST_API int obst_rotary_fwd(const RotDesc* d, hipStream_t st) { return run(d, false, st); }
 OBST_API int obst_rotary_bwd(const RotDesc* d, hipStream_t st) { return run(d, true, st); }
 // floats of RotDesc.part
-OBST_API long long obst_rotary_part(int D) { return 2LL * BWD_BLOCKS * D; }
+OBST_API long long obst_rotary_part(int D) { return (long long)BWD_BLOCKS * D; }

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -83,27 +84,11 @@ class OptDesc(ctypes.Structure):
                 ("step_count", c_f), ("tp_size", c_i), ("dyn", c_p), ("part", c_p), ("part_base", c_i)]
 
 
-class RotDesc(ctypes.Structure):
-    _fields_ = [("q", c_p), ("k", c_p), ("v", c_p), ("gq", c_p), ("gk", c_p), ("qo", c_p), ("ko", c_p), ("vo", c_p),
-                ("wq", c_p), ("wk", c_p), ("freqs", c_p), ("pos", c_p), ("slots", c_p), ("part", c_p), ("dwq", c_p),
-                ("dwk", c_p),
-                ("q_ts", c_ll), ("q_hs", c_ll), ("k_ts", c_ll), ("k_hs", c_ll), ("v_ts", c_ll), ("v_hs", c_ll),
-                ("gq_ts", c_ll), ("gq_hs", c_ll), ("gk_ts", c_ll), ("gk_hs", c_ll), ("T", c_ll), ("nslots", c_ll),
-                ("Hq", c_i), ("Hk", c_i), ("D", c_i), ("R", c_i), ("inter", c_i), ("dtype", c_i), ("wtype", c_i),
-                ("dwtype", c_i), ("dwacc", c_i), ("page", c_i), ("mscale", c_f), ("eps", c_f)]
-
-
-class PlanDesc(ctypes.Structure):
-    _fields_ = [("cached", c_p), ("new", c_p), ("table", c_p), ("free", c_p), ("nfree", c_p), ("slots", c_p),
-                ("pos", c_p), ("start", c_p), ("lens", c_p), ("nfree_out", c_p),
-                ("B", c_i), ("W", c_i), ("ld", c_i), ("page", c_i), ("T", c_i), ("P", c_i)]
-
-
-class PagedDesc(ctypes.Structure):
-    _fields_ = [("q", c_p), ("k", c_p), ("v", c_p), ("o", c_p), ("table", c_p), ("lens", c_p), ("part", c_p),
-                ("q_bs", c_ll), ("q_hs", c_ll),
-                ("B", c_i), ("Hq", c_i), ("Hk", c_i), ("D", c_i), ("P", c_i), ("cap", c_i), ("ld", c_i),
-                ("shift", c_i), ("dtype", c_i), ("nsplit", c_i), ("split", c_i), ("scale", c_f)]
+# descriptors of the small latency-bound launches, packed in one call (a ctypes Structure of 40 fields takes 2.2 us to
+# fill, this 0.4): field order and types of the C structs in csrc/kernels/rotary.hip and paged.hip, natural alignment
+ROT_DESC = struct.Struct("@16P12q10i2f")      # RotDesc
+PLAN_DESC = struct.Struct("@10P6i")           # PlanDesc
+PAGED_DESC = struct.Struct("@7P2q11if")     # PagedDesc
 
 
 _SIGS = {
@@ -163,12 +148,12 @@ _SIGS = {
     "obst_skinny_ws": [c_i, c_i, c_i],
     "obst_calib_mfma": [c_p, c_i, c_p],
     "obst_calib_mfma_flops": [c_i],
-    "obst_rotary_fwd": [ctypes.POINTER(RotDesc), c_p],
-    "obst_rotary_bwd": [ctypes.POINTER(RotDesc), c_p],
+    "obst_rotary_fwd": [ctypes.c_char_p, c_p],
+    "obst_rotary_bwd": [ctypes.c_char_p, c_p],
     "obst_rotary_part": [c_i],
-    "obst_page_plan": [ctypes.POINTER(PlanDesc), c_p],
+    "obst_page_plan": [ctypes.c_char_p, c_p],
     "obst_page_release": [c_p, c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_p],
-    "obst_paged_attn": [ctypes.POINTER(PagedDesc), c_p],
+    "obst_paged_attn": [ctypes.c_char_p, c_p],
     "obst_decode_attn": [c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_i, c_i, c_i, c_i, c_f, c_i, c_p, c_p],
 }
 _RESTYPES = {"obst_rotary_part": c_ll, "obst_calib_mfma_flops": ctypes.c_double, "obst_norm_bwd_ws": c_ll, "obst_skinny_ws": c_ll, "obst_scatter_ws": c_ll}
@@ -209,7 +194,7 @@ def stream_ptr() -> int:
 def launch(fn, t: torch.Tensor, what: str, *args):
     """``fn(*args, stream)`` on the device that holds ``t`` (the current one or not), on its current stream"""
     dev = t.get_device()
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):

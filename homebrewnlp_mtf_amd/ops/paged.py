@@ -21,7 +21,7 @@ import torch
 
 from . import _lib as L
 from . import raw
-from .rotary import (DTYPES, _tokens, check_heads, check_turn, kernel_weights, rotary_t, tokens_view)
+from .rotary import DTYPES, check_args, kernel_weights, rotary_t, tokens_view
 
 HEAD_DIMS = (32, 64, 96, 128, 256)
 PAGES = (16, 32, 64, 128, 256)
@@ -57,18 +57,21 @@ def plan_buffers(requests: int, tokens: int, device: typing.Union[str, torch.dev
                     i32(requests), i32(1))
 
 
-def _ints(what: str, dev, **ts):
-    for name, t in ts.items():
-        if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
-            raise L.KernelError(f"{what}: {name} must be contiguous int32 on {dev}, got {t.dtype} on {t.device}")
+def _ints(what: str, dev: int, *named):
+    for name, t in named:
+        if t.dtype != torch.int32 or t.get_device() != dev or not t.is_contiguous():
+            raise L.KernelError(f"{what}: {name} must be contiguous int32 beside the other tensors, got {t.dtype} on "
+                                f"{t.device}")
 
 
-def _table(what: str, table, B: int, dev):
-    if (table.dtype != torch.int32 or table.device != dev or table.dim() != 2 or table.shape[0] != B
-            or table.shape[1] < 1 or (table.shape[1] > 1 and table.stride(1) != 1)
-            or (B > 1 and not table.shape[1] <= table.stride(0) < 2 ** 31)):
-        raise L.KernelError(f"{what}: the table must be int32 [{B}, pages] with dense rows on {dev}, got {table.dtype} "
-                            f"{list(table.shape)} strides {list(table.stride())} on {table.device}")
+def _table(what: str, table, B: int, dev: int) -> typing.Tuple[int, int]:
+    """(pages a row, row stride) of a block table"""
+    shape, st = table.shape, table.stride()
+    if (table.dtype != torch.int32 or table.get_device() != dev or len(shape) != 2 or shape[0] != B or shape[1] < 1
+            or (shape[1] > 1 and st[1] != 1) or (B > 1 and not shape[1] <= st[0] < 2 ** 31)):
+        raise L.KernelError(f"{what}: the table must be int32 [{B}, pages] with dense rows beside the other tensors, got "
+                            f"{table.dtype} {list(shape)} strides {list(st)} on {table.device}")
+    return shape[1], max(st[0], shape[1])
 
 
 def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stack: torch.Tensor, nfree: torch.Tensor,
@@ -82,22 +85,22 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
     the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request that needs no new
     page goes on). ``cached`` and ``nfree`` are not written: the plan holds their new values, and the same call again
     gives the same plan. ``out`` must not share memory with them."""
-    dev, B = cached.device, cached.numel()
-    _ints("page_plan", dev, cached=cached, new=new, stack=stack, nfree=nfree)
+    dev, B = cached.get_device(), cached.numel()
+    _ints("page_plan", dev, ("cached", cached), ("new", new), ("stack", stack), ("nfree", nfree))
     if cached.dim() != 1 or B < 1 or new.shape != cached.shape or nfree.numel() != 1 or stack.dim() != 1:
         raise L.KernelError(f"page_plan: cached {list(cached.shape)}, new {list(new.shape)}, stack "
                             f"{list(stack.shape)}, nfree {list(nfree.shape)}")
-    _table("page_plan", table, B, dev)
+    W, ld = _table("page_plan", table, B, dev)
     P = stack.numel()
     if page < 1 or P < 1 or P * page > _MAX_SLOTS:
         raise L.KernelError(f"page_plan: a pool of {P} pages of {page} tokens (at most {_MAX_SLOTS} tokens)")
     if out is None:
         if tokens is None:
             raise L.KernelError("page_plan: tokens or out")
-        out = plan_buffers(B, tokens, dev)
+        out = plan_buffers(B, tokens, cached.device)
     else:
-        _ints("page_plan", dev, slots=out.slots, start=out.start, lens=out.lens, nfree_out=out.nfree)
-        if (out.pos.dtype != torch.int64 or out.pos.device != dev or not out.pos.is_contiguous()
+        _ints("page_plan", dev, ("slots", out.slots), ("start", out.start), ("lens", out.lens), ("out.nfree", out.nfree))
+        if (out.pos.dtype != torch.int64 or out.pos.get_device() != dev or not out.pos.is_contiguous()
                 or out.pos.shape != out.slots.shape or out.slots.dim() != 1 or out.start.numel() != B + 1
                 or out.lens.numel() != B or out.nfree.numel() != 1
                 or (tokens is not None and tokens != out.slots.numel())):
@@ -107,14 +110,14 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
     T = out.slots.numel()
     if T >= 2 ** 31:
         raise L.KernelError(f"page_plan: {T} tokens")
-    if dev.type == "cuda":
-        d = L.PlanDesc(cached.data_ptr(), new.data_ptr(), table.data_ptr(), stack.data_ptr(), nfree.data_ptr(),
-                       out.slots.data_ptr(), out.pos.data_ptr(), out.start.data_ptr(), out.lens.data_ptr(),
-                       out.nfree.data_ptr(), B, table.shape[1], max(table.stride(0), table.shape[1]), page, T, P)
-        L.launch(L.lib().obst_page_plan, cached, "page_plan", d)
+    if dev >= 0:
+        L.launch(L.lib().obst_page_plan, cached, "page_plan", L.PLAN_DESC.pack(
+            cached.data_ptr(), new.data_ptr(), table.data_ptr(), stack.data_ptr(), nfree.data_ptr(),
+            out.slots.data_ptr(), out.pos.data_ptr(), out.start.data_ptr(), out.lens.data_ptr(), out.nfree.data_ptr(),
+            B, W, ld, page, T, P))
         return out
     # ---- torch oracle
-    W, avail = table.shape[1], min(max(int(nfree), 0), P)
+    avail = min(max(int(nfree), 0), P)
     out.slots.fill_(-1)
     out.pos.zero_()
     at = asked = taken = 0
@@ -148,16 +151,16 @@ def page_release(done: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, st
                  page: int) -> None:
     """Requests that are ``done`` (bool [B]) give their pages back: pushed onto ``stack`` in request order, ``nfree``
     raised and their ``lens`` zeroed, all in place. (A stack that is full takes no more.)"""
-    dev, B = lens.device, lens.numel()
-    _ints("page_release", dev, lens=lens, stack=stack, nfree=nfree)
-    if lens.dim() != 1 or B < 1 or done.shape != lens.shape or done.dtype != torch.bool or done.device != dev \
+    dev, B = lens.get_device(), lens.numel()
+    _ints("page_release", dev, ("lens", lens), ("stack", stack), ("nfree", nfree))
+    if lens.dim() != 1 or B < 1 or done.shape != lens.shape or done.dtype != torch.bool or done.get_device() != dev \
             or not done.is_contiguous() or nfree.numel() != 1 or stack.dim() != 1 or stack.numel() < 1 or page < 1:
         raise L.KernelError(f"page_release: done bool {list(done.shape)}, lens {list(lens.shape)}, page {page}")
-    _table("page_release", table, B, dev)
-    P, W = stack.numel(), table.shape[1]
-    if dev.type == "cuda":
+    W, ld = _table("page_release", table, B, dev)
+    P = stack.numel()
+    if dev >= 0:
         L.launch(L.lib().obst_page_release, lens, "page_release", done.data_ptr(), lens.data_ptr(), table.data_ptr(),
-                 stack.data_ptr(), nfree.data_ptr(), B, W, max(table.stride(0), W), page, P)
+                 stack.data_ptr(), nfree.data_ptr(), B, W, ld, page, P)
         return
     at = min(max(int(nfree), 0), P)
     for b in done.nonzero().flatten().tolist():
@@ -169,20 +172,29 @@ def page_release(done: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, st
 
 
 # ----------------------------------------------------------------------------------------------------------------
-def _pools(what: str, k_cache, v_cache, q, heads: typing.Optional[int] = None) -> typing.Tuple[int, int, int]:
+def _pools(what: str, k_cache, v_cache, q, dev: int, D: int, heads: typing.Optional[int] = None
+           ) -> typing.Tuple[int, int, int]:
     """(pages, kv heads, page) of a layer's caches"""
-    if k_cache.dim() != 4 or v_cache.dim() != 5:
+    ks, vs, dt = k_cache.shape, v_cache.shape, q.dtype
+    if len(ks) != 4:
         raise L.KernelError(f"{what}: caches [P, heads, page, D] and [P, heads, page / 8, D, 8] (page_pools), got "
-                            f"{list(k_cache.shape)}, {list(v_cache.shape)}")
-    P, H, page, D = k_cache.shape
-    if (tuple(v_cache.shape) != (P, H, page // 8, D, 8) or page not in PAGES or P < 1 or D != q.shape[-1]
-            or (heads is not None and H != heads) or P * page > _MAX_SLOTS):
-        raise L.KernelError(f"{what}: caches {list(k_cache.shape)}, {list(v_cache.shape)} for heads {heads} x "
-                            f"{q.shape[-1]}, pages of {PAGES} tokens")
-    for t in (k_cache, v_cache):
-        if t.dtype != q.dtype or t.device != q.device or not t.is_contiguous():
-            raise L.KernelError(f"{what}: caches must be contiguous {q.dtype} on {q.device}")
+                            f"{list(ks)}, {list(vs)}")
+    P, H, page, d = ks
+    if (vs != (P, H, page // 8, D, 8) or page not in PAGES or P < 1 or d != D or (heads is not None and H != heads)
+            or P * page > _MAX_SLOTS):
+        raise L.KernelError(f"{what}: caches {list(ks)}, {list(vs)} for heads {heads} x {D}, pages of {PAGES} tokens")
+    if (k_cache.dtype != dt or v_cache.dtype != dt or k_cache.get_device() != dev or v_cache.get_device() != dev
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
+        raise L.KernelError(f"{what}: caches must be contiguous {dt} on the device of q")
     return P, H, page
+
+
+def _out(what: str, out, q, shape, dev: int):
+    if out is None:
+        return q.new_empty(shape)
+    if out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
+        raise L.KernelError(f"{what}: out must be contiguous {q.dtype} {list(shape)} on the device of q")
+    return out
 
 
 def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -194,34 +206,31 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
     k and v [T, Hk, D] (any token and head strides), ``slots`` int32 [T] (outside the pool: neither key nor value is
     written), ``pos`` int64 [T]. Returns the turned queries [T, Hq, D]. ``freqs`` None and no weights: a plain append.
     One launch, no gradient. Tokens of one call must have different slots."""
-    check_heads("rotary_append", q, k)
-    if q.dim() != 3 or v.shape != k.shape or v.dtype != q.dtype or v.device != q.device:
-        raise L.KernelError(f"rotary_append: q [T, Hq, D], k and v [T, Hk, D] of one type, got {list(q.shape)}, "
-                            f"{list(k.shape)}, {list(v.shape)}")
+    pos, freqs, rot, T = check_args("rotary_append", q, k, pos, freqs, q_weight, k_weight, eps)
+    qs, ks, dev = q.shape, k.shape, q.get_device()
+    if len(qs) != 3 or v.shape != ks or v.dtype != q.dtype or v.get_device() != dev:
+        raise L.KernelError(f"rotary_append: q [T, Hq, D], k and v [T, Hk, D] of one type, got {list(qs)}, {list(ks)}, "
+                            f"{list(v.shape)}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise L.KernelError("rotary_append has no gradient: call it under torch.no_grad()")
-    T, Hq, D = q.shape
-    P, Hk, page = _pools("rotary_append", k_cache, v_cache, q, k.shape[1])
-    _ints("rotary_append", q.device, slots=slots)
+    _, Hq, D = qs
+    P, Hk, page = _pools("rotary_append", k_cache, v_cache, q, dev, D, ks[1])
+    _ints("rotary_append", dev, ("slots", slots))
     if slots.dim() != 1 or slots.numel() != T:
         raise L.KernelError(f"rotary_append: slots {list(slots.shape)} for {T} tokens")
-    pos, freqs, rot = check_turn("rotary_append", q, pos, freqs, (q_weight, k_weight), eps)
-    if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise L.KernelError(f"rotary_append: out must be contiguous {q.dtype} {list(q.shape)}")
-    if q.device.type == "meta" or T == 0:
+    out = _out("rotary_append", out, q, qs, dev)
+    if T == 0 or q.is_meta:
         return out
-    if raw.on_gpu(q):
+    if dev >= 0:
         q, q_ts, q_hs = tokens_view(q)
         k, k_ts, k_hs = tokens_view(k)
         v, v_ts, v_hs = tokens_view(v)
         wq, wk, wt = kernel_weights(q_weight, k_weight)
-        d = L.RotDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, out.data_ptr(), k_cache.data_ptr(),
-                      v_cache.data_ptr(), L.ptr(wq), L.ptr(wk), L.ptr(freqs), pos.data_ptr(), slots.data_ptr(), 0, 0,
-                      0, q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, 0, 0, 0, 0, T, P * page, Hq, Hk, D, rot,
-                      int(interleaved), DTYPES[q.dtype], wt, 0, 0, page, mscale, eps)
-        L.launch(L.lib().obst_rotary_fwd, q, "rotary_append", d)
+        L.launch(L.lib().obst_rotary_fwd, q, "rotary_append", L.ROT_DESC.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            L.ptr(wq), L.ptr(wk), L.ptr(freqs), pos.data_ptr(), slots.data_ptr(), 0, 0, 0, q_ts, q_hs, k_ts, k_hs, v_ts,
+            v_hs, 0, 0, 0, 0, T, P * page, Hq, Hk, D, rot, bool(interleaved), DTYPES[q.dtype], wt, 0, 0, page, mscale,
+            eps))
         return out
     # ---- torch oracle
     ko = rotary_t(k, None if k_weight is None else k_weight.detach(), pos, freqs, interleaved, mscale, eps)
@@ -246,48 +255,45 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     ``max_len`` (default: what the table's width holds) is a bound on lens that the host knows; it sizes the launch, so
     a close one helps a wide table. A page id outside the pool hides its tokens. What the cache holds behind a length
     is never looked at. No gradient."""
-    if q.dim() != 3 or q.shape[0] < 0 or q.numel() == 0 and q.shape[0] > 0:
-        raise L.KernelError(f"paged_attn: q must be [B, heads, D], got {list(q.shape)}")
-    B, Hq, D = q.shape
-    P, Hk, page = _pools("paged_attn", k_cache, v_cache, q)
-    if Hk < 1 or Hq < 1 or Hq % Hk:
+    qs, dev = q.shape, q.get_device()
+    if len(qs) != 3 or qs[1] < 1 or qs[2] < 1:
+        raise L.KernelError(f"paged_attn: q must be [B, heads, D], got {list(qs)}")
+    B, Hq, D = qs
+    P, Hk, page = _pools("paged_attn", k_cache, v_cache, q, dev, D)
+    if Hk < 1 or Hq % Hk:
         raise L.KernelError(f"paged_attn: {Hq} query heads over {Hk} key heads")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise L.KernelError("paged_attn has no gradient: call it under torch.no_grad()")
-    _table("paged_attn", table, B, q.device)
-    _ints("paged_attn", q.device, lens=lens)
+    W, ld = _table("paged_attn", table, B, dev)
+    _ints("paged_attn", dev, ("lens", lens))
     if lens.dim() != 1 or lens.numel() != B:
         raise L.KernelError(f"paged_attn: lens {list(lens.shape)} for {B} requests")
-    W = table.shape[1]
     cap = min(W * page, _MAX_SLOTS // page * page)
     if max_len is not None:
         if max_len < 0:
             raise L.KernelError(f"paged_attn: max_len {max_len}")
         cap = min(cap, max_len)
-    if out is None:
-        out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise L.KernelError(f"paged_attn: out must be contiguous {q.dtype} {list(q.shape)}")
-    if B == 0 or q.device.type == "meta":
+    out = _out("paged_attn", out, q, qs, dev)
+    if B == 0 or q.is_meta:
         return out
-    if raw.on_gpu(q):
+    if dev >= 0:
+        rows = Hk * (-(-Hq // Hk // 16))
         if D not in HEAD_DIMS or q.dtype not in (torch.bfloat16, torch.float16):
             raise L.KernelError(f"paged_attn: heads of {HEAD_DIMS} in bf16 or fp16 on the GPU, got {D} in {q.dtype}")
-        if B > 65535 or Hk * (-(-Hq // Hk // 16)) > 65535:
+        if B > 65535 or rows > 65535:
             raise L.KernelError(f"paged_attn: {B} requests x {Hk} heads (at most 65535 each)")
-        if q.stride(2) != 1 or (q.stride(0) | q.stride(1)) % 8 or q.data_ptr() % 16:
-            q = q.contiguous()
-            if q.data_ptr() % 16:
-                q = q.clone()
-        for t in (k_cache, v_cache):
-            if t.data_ptr() % 16:
-                raise L.KernelError("paged_attn: caches must be 16-byte aligned")
-        nsplit, split = _splits(B * Hk * (-(-Hq // Hk // 16)), cap)
-        part = torch.empty(B * Hq * nsplit * (D + 2), dtype=torch.float32, device=q.device) if nsplit > 1 else None
-        d = L.PagedDesc(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(),
-                        lens.data_ptr(), L.ptr(part), q.stride(0), q.stride(1), B, Hq, Hk, D, P, cap,
-                        max(table.stride(0), W), page.bit_length() - 1, DTYPES[q.dtype], nsplit, split, scale)
-        L.launch(L.lib().obst_paged_attn, q, "paged_attn", d)
+        q_bs, q_hs, q_ds = q.stride()
+        if q_ds != 1 or (q_bs | q_hs) % 8 or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            q_bs, q_hs = Hq * D, D
+        if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+            raise L.KernelError("paged_attn: caches must be 16-byte aligned")
+        nsplit, split = _splits(B * rows, cap)
+        part = q.new_empty(B * Hq * nsplit * (D + 2), dtype=torch.float32) if nsplit > 1 else None
+        L.launch(L.lib().obst_paged_attn, q, "paged_attn", L.PAGED_DESC.pack(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
+            L.ptr(part), q_bs, q_hs, B, Hq, Hk, D, P, cap, ld, page.bit_length() - 1, DTYPES[q.dtype], nsplit, split,
+            scale))
         return out
     # ---- torch oracle
     G = Hq // Hk
@@ -308,8 +314,9 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
 
 
 def _splits(rows: int, cap: int) -> typing.Tuple[int, int]:
-    """(splits, tokens a split) of the length for ``rows`` blocks without one: enough blocks to fill the card"""
-    want = max(1, -(-2048 // rows))
+    """(splits, tokens a split) of the length for ``rows`` blocks without one: enough blocks to fill the card, at most
+    1024 splits (csrc/kernels/paged.hip MAX_SPLITS)"""
+    want = min(1024, max(1, -(-1024 // rows)))
     split = max(256, -(-cap // want))
     split = -(-split // 128) * 128
     return max(1, -(-cap // split)), split

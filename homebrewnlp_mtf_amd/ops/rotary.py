@@ -22,6 +22,7 @@ from . import raw
 from .functional import _acc_grad, _done, _param32
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_TYPES = set(DTYPES)
 MAX_DIM = 512
 
 
@@ -76,75 +77,73 @@ def rotary_freqs(rot_dim: int, theta: float = 10000.0, scaling: typing.Optional[
 
 
 # ----------------------------------------------------------------------------------------------------------------
-# argument checks and layouts shared with the serving form
+# argument checks and layouts shared with the serving form. A decode step calls these once per layer and waits for them:
+# they touch each tensor attribute once
 def tokens_view(t: torch.Tensor) -> typing.Tuple[torch.Tensor, int, int]:
     """[..., H, D] -> (the tensor, token stride, head stride); a copy only where the leading dims are no single stride
     or the last one is not dense"""
-    shape, st = t.shape, t.stride()
-    n = len(shape)
-    ok = st[-1] == 1 or shape[-1] == 1
-    for i in range(n - 3):
-        if shape[i] != 1 and st[i] != st[i + 1] * shape[i + 1]:
-            # a leading dim whose inner one is 1 wide takes its stride from further in
-            ok = ok and all(shape[j] == 1 for j in range(i + 1, n - 2))
-    if not ok:
-        t = t.contiguous()
-        st = t.stride()
-    ts = 0
-    for i in range(n - 3, -1, -1):
-        if shape[i] != 1:
-            ts = st[i]
-            break
-    return t, ts, st[-2]
+    shape = t.shape
+    if t.is_contiguous():
+        return t, shape[-1] * shape[-2], shape[-1]
+    st, n = t.stride(), len(shape)
+    # the leading dims that are wider than 1 must follow from one another
+    lead = [i for i in range(n - 2) if shape[i] != 1]
+    if (st[-1] != 1 and shape[-1] != 1) or any(st[i] != st[j] * shape[j] for i, j in zip(lead, lead[1:])):
+        return t.contiguous(), shape[-1] * shape[-2], shape[-1]
+    return t, st[lead[-1]] if lead else 0, st[-2]
 
 
-def check_heads(what: str, q, k):
-    if q.dim() < 3 or k.dim() != q.dim() or q.shape[:-2] != k.shape[:-2] or q.shape[-1] != k.shape[-1]:
-        raise L.KernelError(f"{what}: q {list(q.shape)} and k {list(k.shape)} must be [..., heads, dim] over the same "
-                            "tokens")
-    if q.shape[-2] < 1 or k.shape[-2] < 1 or not 1 <= q.shape[-1] <= MAX_DIM:
-        raise L.KernelError(f"{what}: at least one head of 1 to {MAX_DIM} dims, got {list(q.shape)}, {list(k.shape)}")
-    if k.dtype != q.dtype or k.device != q.device:
+def check_args(what: str, q, k, pos, freqs, wq, wk, eps: float):
+    """(positions over the tokens, frequencies, both contiguous; rotated dims; tokens)"""
+    qs, ks, dev = q.shape, k.shape, q.get_device()
+    n, D = len(qs), qs[-1] if len(qs) else 0
+    if n < 3 or len(ks) != n or ks[-1] != D or qs[:-2] != ks[:-2]:
+        raise L.KernelError(f"{what}: q {list(qs)} and k {list(ks)} must be [..., heads, dim] over the same tokens")
+    if qs[-2] < 1 or ks[-2] < 1 or not 1 <= D <= MAX_DIM:
+        raise L.KernelError(f"{what}: at least one head of 1 to {MAX_DIM} dims, got {list(qs)}, {list(ks)}")
+    if k.dtype != q.dtype or k.get_device() != dev:
         raise L.KernelError(f"{what}: q and k must share type and device")
-    if q.device.type == "cuda" and q.dtype not in DTYPES:
+    if dev >= 0 and q.dtype not in DTYPES:
         raise L.KernelError(f"{what}: bf16, fp16 or fp32 on the GPU, got {q.dtype}")
-
-
-def check_turn(what: str, q, pos, freqs, weights, eps: float):
-    """(positions [tokens] contiguous, rotated dims)"""
-    lead = q.shape[:-2]
-    if pos.dtype != torch.int64 or pos.device != q.device:
+    if pos.dtype != torch.int64 or pos.get_device() != dev:
         raise L.KernelError(f"{what}: positions must be int64 on the device of q")
+    lead = qs[:-2]
     if pos.shape != lead:
         try:
             pos = pos.expand(lead)
         except RuntimeError:
             raise L.KernelError(f"{what}: positions {list(pos.shape)} for tokens {list(lead)}") from None
+    if not pos.is_contiguous():
+        pos = pos.contiguous()
     rot = 0
     if freqs is not None:
         rot = 2 * freqs.numel()
-        if freqs.dtype != torch.float64 or freqs.dim() != 1 or freqs.device != q.device or rot > q.shape[-1]:
-            raise L.KernelError(f"{what}: freqs must be float64 [pairs] on the device of q with 2 * pairs <= "
-                                f"{q.shape[-1]}, got {freqs.dtype} {list(freqs.shape)} on {freqs.device}")
-        freqs = freqs.contiguous()
-    for w in weights:
-        if w is not None and (w.numel() != q.shape[-1] or w.device != q.device or not w.is_floating_point()):
-            raise L.KernelError(f"{what}: norm weights must be [{q.shape[-1]}] on the device of q")
+        if freqs.dtype != torch.float64 or freqs.dim() != 1 or freqs.get_device() != dev or rot > D:
+            raise L.KernelError(f"{what}: freqs must be float64 [pairs] on the device of q with 2 * pairs <= {D}, got "
+                                f"{freqs.dtype} {list(freqs.shape)} on {freqs.device}")
+        if not freqs.is_contiguous():
+            freqs = freqs.contiguous()
+    for w in (wq, wk):
+        if w is not None and (w.numel() != D or w.get_device() != dev or not w.dtype.is_floating_point):
+            raise L.KernelError(f"{what}: norm weights must be [{D}] on the device of q")
     if not eps > 0:
         raise L.KernelError(f"{what}: eps must be positive, got {eps}")
-    return pos.contiguous(), freqs, rot
+    return pos, freqs, rot, math.prod(lead)
 
 
 def kernel_weights(wq, wk):
     """(wq, wk, type code) as the kernels read them: the fp32 master copy of a model parameter, else the tensor itself;
     of two types, both in fp32"""
-    wq, wk = (None if w is None else (_param32(w) if hasattr(w, "master") else w).detach().contiguous()
-              for w in (wq, wk))
+    if wq is None and wk is None:
+        return None, None, 0
+    if hasattr(wq, "master") or hasattr(wk, "master"):
+        wq, wk = _param32(wq), _param32(wk)
     types = {w.dtype for w in (wq, wk) if w is not None}
-    if len(types) > 1 or (types and not types <= set(DTYPES)):
+    if len(types) > 1 or not types <= _TYPES:
         wq, wk = (None if w is None else w.float() for w in (wq, wk))
         types = {torch.float32}
-    return wq, wk, DTYPES[types.pop()] if types else 0
+    wq, wk = (w if w is None or w.is_contiguous() else w.contiguous() for w in (wq, wk))
+    return wq, wk, DTYPES[types.pop()]
 
 
 # ----------------------------------------------------------------------------------------------------------------
@@ -183,16 +182,12 @@ def rotary_bwd_t(x, w, g, pos, freqs, inter: bool, mscale: float, eps: float):
 
 
 # ----------------------------------------------------------------------------------------------------------------
-def _tokens(q) -> int:
-    return q.numel() // (q.shape[-1] * q.shape[-2])
-
-
-def _forward(q, k, pos, freqs, rot, wq, wk, inter, mscale, eps):
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if q.device.type == "meta" or q.numel() == 0:
+def _forward(q, k, pos, freqs, rot, T, wq, wk, inter, mscale, eps):
+    qs, ks = q.shape, k.shape
+    qo, ko = q.new_empty(qs), k.new_empty(ks)
+    if T == 0 or q.is_meta:
         return qo, ko
-    if not raw.on_gpu(q):
+    if q.get_device() < 0:
         w = [None if x is None else _param32(x).detach() for x in (wq, wk)]
         qo.copy_(rotary_t(q, w[0], pos, freqs, inter, mscale, eps))
         ko.copy_(rotary_t(k, w[1], pos, freqs, inter, mscale, eps))
@@ -200,28 +195,28 @@ def _forward(q, k, pos, freqs, rot, wq, wk, inter, mscale, eps):
     q, q_ts, q_hs = tokens_view(q)
     k, k_ts, k_hs = tokens_view(k)
     wq, wk, wt = kernel_weights(wq, wk)
-    d = L.RotDesc(q.data_ptr(), k.data_ptr(), 0, 0, 0, qo.data_ptr(), ko.data_ptr(), 0, L.ptr(wq), L.ptr(wk),
-                  L.ptr(freqs), pos.data_ptr(), 0, 0, 0, 0, q_ts, q_hs, k_ts, k_hs, 0, 0, 0, 0, 0, 0, _tokens(q), 0,
-                  q.shape[-2], k.shape[-2], q.shape[-1], rot, int(inter), DTYPES[q.dtype], wt, 0, 0, 0, mscale, eps)
-    L.launch(L.lib().obst_rotary_fwd, q, "rotary", d)
+    L.launch(L.lib().obst_rotary_fwd, q, "rotary", L.ROT_DESC.pack(
+        q.data_ptr(), k.data_ptr(), 0, 0, 0, qo.data_ptr(), ko.data_ptr(), 0, L.ptr(wq), L.ptr(wk), L.ptr(freqs),
+        pos.data_ptr(), 0, 0, 0, 0, q_ts, q_hs, k_ts, k_hs, 0, 0, 0, 0, 0, 0, T, 0, qs[-2], ks[-2], qs[-1], rot, inter,
+        DTYPES[q.dtype], wt, 0, 0, 0, mscale, eps))
     return qo, ko
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, pos, freqs, rot, inter, mscale, eps):
+    def forward(ctx, q, k, wq, wk, pos, freqs, rot, T, inter, mscale, eps):
         normed = wq is not None or wk is not None
         ctx.save_for_backward(q if normed else None, k if normed else None, wq, wk, pos, freqs)
-        ctx.cfg = (rot, inter, mscale, eps)
-        return _forward(q, k, pos, freqs, rot, wq, wk, inter, mscale, eps)
+        ctx.cfg = (rot, T, inter, mscale, eps)
+        return _forward(q, k, pos, freqs, rot, T, wq, wk, inter, mscale, eps)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, pos, freqs = ctx.saved_tensors
-        rot, inter, mscale, eps = ctx.cfg
-        dq = torch.empty(gq.shape, dtype=gq.dtype, device=gq.device)
-        dk = torch.empty(gk.shape, dtype=gk.dtype, device=gk.device)
+        rot, T, inter, mscale, eps = ctx.cfg
+        gs, hs = gq.shape, gk.shape
+        dq, dk = gq.new_empty(gs), gk.new_empty(hs)
         ws = (wq, wk)
         # model parameters accumulate into their fp32 main gradient; other weights get theirs back in their own type
         main = any(getattr(w, "main_grad", None) is not None for w in ws if w is not None)
@@ -232,7 +227,7 @@ class _Rotary(torch.autograd.Function):
             if main:
                 dws[i], kept[i] = _acc_grad(w)
             elif raw.on_gpu(w) and wt_direct(ws):
-                dws[i], kept[i] = torch.empty(w.shape, dtype=w.dtype, device=w.device), False
+                dws[i], kept[i] = w.new_empty(w.shape), False
             else:
                 dws[i] = torch.zeros(w.shape, device=w.device, dtype=torch.float64 if w.dtype == torch.float64
                                      else torch.float32)
@@ -255,23 +250,22 @@ class _Rotary(torch.autograd.Function):
             if q is not None:
                 q, q_ts, q_hs = tokens_view(q)
                 k, k_ts, k_hs = tokens_view(k)
-                part = torch.empty(lib.obst_rotary_part(gq.shape[-1]), dtype=torch.float32, device=gq.device)
+                part = gq.new_empty(lib.obst_rotary_part(gs[-1]), dtype=torch.float32)
             vq, vk, wt = kernel_weights(wq, wk)
-            typed = [x for x in into if x is not None]
-            d = L.RotDesc(L.ptr(q), L.ptr(k), 0, gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), 0,
-                          L.ptr(vq), L.ptr(vk), L.ptr(freqs), pos.data_ptr(), 0, L.ptr(part), L.ptr(into[0]),
-                          L.ptr(into[1]), q_ts, q_hs, k_ts, k_hs, 0, 0, gq_ts, gq_hs, gk_ts, gk_hs, _tokens(gq), 0,
-                          gq.shape[-2], gk.shape[-2], gq.shape[-1], rot, int(inter), DTYPES[gq.dtype], wt,
-                          DTYPES[typed[0].dtype] if typed else 0, int(main), 0, mscale, eps)
-            L.launch(lib.obst_rotary_bwd, gq, "rotary_bwd", d)
+            dt = next((DTYPES[x.dtype] for x in into if x is not None), 0)
+            L.launch(lib.obst_rotary_bwd, gq, "rotary_bwd", L.ROT_DESC.pack(
+                L.ptr(q), L.ptr(k), 0, gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), 0, L.ptr(vq),
+                L.ptr(vk), L.ptr(freqs), pos.data_ptr(), 0, L.ptr(part), L.ptr(into[0]), L.ptr(into[1]), q_ts, q_hs,
+                k_ts, k_hs, 0, 0, gq_ts, gq_hs, gk_ts, gk_hs, T, 0, gs[-2], hs[-2], gs[-1], rot, inter,
+                DTYPES[gq.dtype], wt, dt, main, 0, mscale, eps))
         if into[1] is not dws[1]:
             dws[1].add_(into[1])
         out = []
         for w, g, keep in zip(ws, dws, kept):
             if w is not None:
                 _done(w)
-            out.append(None if w is None or keep else g.to(w.dtype))
-        return dq, dk, out[0], out[1], None, None, None, None, None, None
+            out.append(None if w is None or keep else g if g.dtype == w.dtype else g.to(w.dtype))
+        return dq, dk, out[0], out[1], None, None, None, None, None, None, None
 
 
 def wt_direct(ws) -> bool:
@@ -287,9 +281,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, freqs: typing.Op
     turned (module docstring); any token and head strides. ``pos`` int64 over the tokens (or broadcastable to them, any
     value), ``freqs`` float64 from ``rotary_freqs`` (None: no rotation). Returns new contiguous tensors; differentiable
     in q, k and the weights, sums in fp32, weight gradients in a fixed order (the same bits each run)."""
-    check_heads("rotary", q, k)
-    pos, freqs, rot = check_turn("rotary", q, pos, freqs, (q_weight, k_weight), eps)
+    pos, freqs, rot, T = check_args("rotary", q, k, pos, freqs, q_weight, k_weight, eps)
+    cfg = (rot, T, bool(interleaved), float(mscale), float(eps))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
-        return _Rotary.apply(q, k, q_weight, k_weight, pos, freqs, rot, bool(interleaved), float(mscale), float(eps))
-    return _forward(q, k, pos, freqs, rot, q_weight, k_weight, bool(interleaved), float(mscale), float(eps))
+        return _Rotary.apply(q, k, q_weight, k_weight, pos, freqs, *cfg)
+    return _forward(q, k, pos, freqs, rot, T, q_weight, k_weight, *cfg[2:])
