@@ -36,13 +36,18 @@ constexpr int NTH = 256;
 // asked for up to and including it pass the stack. Its i-th new page is the stack's entry nfree - 1 - (pages asked for
 // before it) - i. Sums over the requests before b are all that a group needs, so every block forms them itself from
 // the lengths (a few KB out of the caches) and one launch does it all: the call's latency is what matters here.
+//
+// Bound by the latency of three dependent loads (lengths, stack, the launch itself): 5 us for 64 requests' decode step as for
+// 203 ragged prompts.
 struct Want { long long n, need; bool fits; };
+
+__device__ __forceinline__ unsigned pages_of(unsigned tokens, unsigned page) { return tokens ? (tokens - 1) / page + 1 : 0; }
 
 __device__ __forceinline__ Want want_of(const PlanDesc& d, int b, int& c) {
   c = max(d.cached[b], 0);
   const int n = max(d.nnew[b], 0);
-  const long long old = (c + (long long)d.page - 1) / d.page, all = ((long long)c + n + d.page - 1) / d.page;
-  const bool fits = all <= d.W;
+  const unsigned old = pages_of(c, d.page), all = pages_of((unsigned)c + n, d.page);   // c + n < 2^32
+  const bool fits = all <= (unsigned)d.W;
   return {n, fits ? all - old : 0, fits};
 }
 
@@ -52,13 +57,67 @@ __device__ __forceinline__ long long wave_sum_ll(long long v) {
   return v;
 }
 
-// grid (request groups, token segments): 8 requests a block, 32 lanes each
+// sum over the threads before this one
+__device__ __forceinline__ long long block_before(long long v, long long* red) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long y = __shfl_up(x, o, 64);
+    x += lane >= o ? y : 0;
+  }
+  __syncthreads();
+  if (lane == 63) red[w] = x;
+  __syncthreads();
+  x -= v;
+  for (int i = 0; i < w; ++i) x += red[i];
+  return x;
+}
+
+// grid (request groups + 1, token segments): 8 requests a block, 32 lanes each; the last group's block forms what all
+// requests share
 constexpr int GR = 8, GL = NTH / GR;
 
 __global__ __launch_bounds__(NTH) void page_plan_kernel(const PlanDesc d) {
   __shared__ long long red[3][NTH / 64];
   __shared__ long long s_n[GR], s_need[GR];
   const int tid = threadIdx.x, r0 = blockIdx.x * GR;
+  const int avail = min(max(*d.nfree, 0), d.P);
+  const bool first = blockIdx.y == 0;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (!first) return;
+    // what is left of the stack: the pages asked for up to the last request that got some. Thread t takes its run of
+    // requests
+    const int per = (d.B + NTH - 1) / NTH, j0 = min(d.B, tid * per), j1 = min(d.B, j0 + per);
+    int c;
+    long long n = 0, need = 0, taken = 0;
+    for (int j = j0; j < j1; ++j) n += want_of(d, j, c).n;
+    const long long at0 = block_before(n, red[0]);
+    if (tid == NTH - 1) d.start[d.B] = (int)min(at0 + n, (long long)0x7fffffff);
+    long long at = at0;
+    for (int j = j0; j < j1; ++j) {
+      const Want x = want_of(d, j, c);
+      at += x.n;
+      if (at <= d.T) need += x.need;
+    }
+    long long asked = block_before(need, red[1]);
+    at = at0;
+    for (int j = j0; j < j1; ++j) {
+      const Want x = want_of(d, j, c);
+      at += x.n;
+      if (at > d.T) break;
+      asked += x.need;
+      if (x.need > 0 && asked <= avail) taken = asked;
+    }
+    for (int o = 32; o > 0; o >>= 1) taken = max(taken, (long long)__shfl_xor(taken, o, 64));
+    if ((tid & 63) == 0) red[2][tid >> 6] = taken;
+    __syncthreads();
+    if (tid == 0) {
+      for (int i = 0; i < NTH / 64; ++i) taken = max(taken, red[2][i]);
+      *d.nfree_out = (int)(avail - taken);
+    }
+    return;
+  }
   long long n0 = 0, need0 = 0, total = 0;        // tokens and pages before the block's requests; all tokens
   for (int j = tid; j < d.B; j += NTH) {
     int c;
@@ -80,75 +139,34 @@ __global__ __launch_bounds__(NTH) void page_plan_kernel(const PlanDesc d) {
 #pragma unroll
   for (int i = 0; i < NTH / 64; ++i) { n0 += red[0][i]; need0 += red[1][i]; total += red[2][i]; }
   for (int i = 0; i < g; ++i) { n0 += s_n[i]; need0 += s_need[i]; }
-  const int avail = min(max(*d.nfree, 0), d.P);
-  const bool first = blockIdx.y == 0;
   if (b < d.B) {
     const bool room = w.fits && n0 + w.n <= d.T;
     const bool ok = room && (w.need == 0 || need0 + w.need <= avail);
-    const long long old = (c + (long long)d.page - 1) / d.page;
+    const unsigned old = pages_of(c, d.page);
     if (first && l == 0) {
       d.lens[b] = ok ? (int)(c + w.n) : c;
       d.start[b] = (int)min(n0, (long long)0x7fffffff);
     }
+    // (an entry of the stack is used only where ok: its index is then below avail)
     if (first && ok)
       for (long long i = l; i < w.need; i += GL) d.table[(long long)b * d.ld + old + i] = d.free[avail - 1 - need0 - i];
     for (long long i = (long long)blockIdx.y * GL + l; i < w.n && n0 + i < d.T; i += (long long)gridDim.y * GL) {
-      const long long p = c + i, e = p / d.page;
+      const long long p = c + i;
       int slot = -1;
-      if (ok) {
+      if (ok) {                                    // p < W * page, below 2^32
+        const unsigned e = (unsigned)p / (unsigned)d.page, off = (unsigned)p % (unsigned)d.page;
         const int id = e < old ? d.table[(long long)b * d.ld + e] : d.free[avail - 1 - need0 - (e - old)];
-        if ((unsigned)id < (unsigned)d.P) slot = id * d.page + (int)(p % d.page);
+        if ((unsigned)id < (unsigned)d.P) slot = id * d.page + (int)off;
       }
       d.slots[n0 + i] = slot;
       d.pos[n0 + i] = p;
     }
   }
   // places of the step's buffer behind the last token
-  for (long long t = total + (blockIdx.y * (long long)gridDim.x + blockIdx.x) * NTH + tid; t < d.T;
-       t += (long long)gridDim.x * gridDim.y * NTH) {
+  const long long gx = gridDim.x - 1;
+  for (long long t = total + (blockIdx.y * gx + blockIdx.x) * NTH + tid; t < d.T; t += gx * gridDim.y * NTH) {
     d.slots[t] = -1;
     d.pos[t] = 0;
-  }
-  if (!first || blockIdx.x != gridDim.x - 1) return;
-  // what is left of the stack: the pages asked for up to the last request that got some. Thread t takes its run of
-  // requests; the runs' sums are joined in order
-  __shared__ long long sn[NTH], sneed[NTH], top[NTH / 64];
-  const int per = (d.B + NTH - 1) / NTH, j0 = tid * per, j1 = min(d.B, j0 + per);
-  long long n = 0;
-  for (int j = j0; j < j1; ++j) {
-    int cc;
-    n += want_of(d, j, cc).n;
-  }
-  sn[tid] = n;
-  __syncthreads();
-  long long at = 0;
-  for (int i = 0; i < tid; ++i) at += sn[i];
-  long long need = 0, a2 = at;
-  for (int j = j0; j < j1; ++j) {
-    int cc;
-    const Want x = want_of(d, j, cc);
-    a2 += x.n;
-    if (a2 <= d.T) need += x.need;
-  }
-  sneed[tid] = need;
-  __syncthreads();
-  long long asked = 0, taken = 0;
-  for (int i = 0; i < tid; ++i) asked += sneed[i];
-  for (int j = j0; j < j1; ++j) {
-    int cc;
-    const Want x = want_of(d, j, cc);
-    at += x.n;
-    if (at > d.T) continue;
-    asked += x.need;
-    if (x.need > 0 && asked <= avail) taken = asked;
-  }
-  for (int o = 32; o > 0; o >>= 1) taken = max(taken, (long long)__shfl_xor(taken, o, 64));
-  if ((tid & 63) == 0) top[tid >> 6] = taken;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 0; i < NTH / 64; ++i) taken = max(taken, top[i]);
-    *d.nfree_out = (int)(avail - taken);
-    d.start[d.B] = (int)min(total, (long long)0x7fffffff);
   }
 }
 
@@ -436,7 +454,7 @@ OBST_API int obst_page_plan(const PlanDesc* d, hipStream_t st) {
   const int gx = (d->B + GR - 1) / GR;
   long long gy = d->T / ((long long)d->B * GL * 4);      // a few rounds of a request's tokens per lane
   gy = gy < 1 ? 1 : gy > 64 ? 64 : gy;
-  hipLaunchKernelGGL(page_plan_kernel, dim3(gx, (unsigned)gy), dim3(NTH), 0, st, *d);
+  hipLaunchKernelGGL(page_plan_kernel, dim3(gx + 1, (unsigned)gy), dim3(NTH), 0, st, *d);
   return (int)hipGetLastError();
 }
 
