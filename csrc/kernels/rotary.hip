@@ -61,6 +61,18 @@ __device__ __forceinline__ void store(E* p, const float* f) {
   *reinterpret_cast<Chunk<E, VEC>*>(p) = c;
 }
 
+// A chunk that is read once: past the caches where a head's lanes together take whole 128-byte lines (bf16 x 128 normed
+// backward 165 -> 153 us); where they take parts, the caches hold the rest for the other half's load (fp32 x 96, half a
+// head 1.5 lines: 26 us, 30 past the caches)
+template <bool LINES, typename E, int VEC>
+__device__ __forceinline__ Chunk<E, VEC> load_once(const E* p) {
+  if constexpr (LINES) {
+    typedef __attribute__((ext_vector_type(4))) uint32_t u4;
+    return __builtin_bit_cast(Chunk<E, VEC>, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p)));
+  }
+  return *reinterpret_cast<const Chunk<E, VEC>*>(p);
+}
+
 // the compiler no longer knows what a loaded chunk holds: what it derived from it is not kept
 template <typename E, int VEC>
 __device__ __forceinline__ void forget(Chunk<E, VEC>& c) {
@@ -371,7 +383,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
 // lanes and waves in a fixed order into part[block], rotary_fold_kernel the blocks: no atomics, the same bits each run.
 // With sums to keep, a block works on one tensor (the first nbq on q): sums for both took 16 more registers a lane and
 // spilled.
-template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool NORM>
+template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool NORM, bool LINES>
 __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int lph, int pq, int pk, int nbq) {
   typedef typename Elem<TYPE>::t E;
   __shared__ Staged sh;
@@ -402,11 +414,11 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
       const E* x = isq ? (const E*)d.q + t * d.q_ts + h * d.q_hs : (const E*)d.k + t * d.k_ts + h * d.k_hs;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
-        ga[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(g + ln.ca[it]);
-        gb[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(g + ln.cb[it]);
+        ga[p][it] = load_once<LINES, E, VEC>(g + ln.ca[it]);
+        gb[p][it] = load_once<LINES, E, VEC>(g + ln.cb[it]);
         if (NORM) {
-          xa[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.ca[it]);
-          xb[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.cb[it]);
+          xa[p][it] = load_once<LINES, E, VEC>(x + ln.ca[it]);
+          xb[p][it] = load_once<LINES, E, VEC>(x + ln.cb[it]);
         }
       }
     }
@@ -580,12 +592,12 @@ template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE>
 int backward(const RotDesc& d, int lph, hipStream_t st) {
   const Passes p(d, lph);
   const int grid = Passes::blocks(d.T * ((p.pq + p.pk + U - 1) / U), BWD_BLOCKS);
-  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false>), dim3(grid), dim3(NTH), 0, st, d, lph, p.pq,
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false, false>), dim3(grid), dim3(NTH), 0, st, d, lph, p.pq,
                      p.pk, 0);
   return (int)hipGetLastError();
 }
 
-template <int TYPE, int VEC, int ITEMS, bool INSIDE>
+template <int TYPE, int VEC, int ITEMS, bool INSIDE, bool LINES>
 int backward_normed(const RotDesc& d, int lph, hipStream_t st) {
   const Passes p(d, lph);
   // blocks for q and for k, as many as their units ask for
@@ -596,7 +608,7 @@ int backward_normed(const RotDesc& d, int lph, hipStream_t st) {
     nq = nq < 1 ? 1 : nq > BWD_BLOCKS - 1 ? BWD_BLOCKS - 1 : nq;
     nk = BWD_BLOCKS - nq;
   }
-  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, 1, INSIDE, true>), dim3(nq + nk), dim3(NTH), 0, st, d, lph, p.pq,
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, 1, INSIDE, true, LINES>), dim3(nq + nk), dim3(NTH), 0, st, d, lph, p.pq,
                      p.pk, nq);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
@@ -611,14 +623,16 @@ template <int TYPE, int VEC, bool INSIDE>
 int by_tokens(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
   const bool few = d.T < 1024;
   if (!bwd) return few ? forward<TYPE, VEC, 1, 1, INSIDE>(d, lph, st) : forward<TYPE, VEC, 1, 4, INSIDE>(d, lph, st);
-  if (d.wq || d.wk) return backward_normed<TYPE, VEC, 1, INSIDE>(d, lph, st);
+  if (d.wq || d.wk)
+    return items_of(d, VEC) * 16 % 128 == 0 ? backward_normed<TYPE, VEC, 1, INSIDE, true>(d, lph, st)
+                                            : backward_normed<TYPE, VEC, 1, INSIDE, false>(d, lph, st);
   return few ? backward<TYPE, VEC, 1, 1, INSIDE>(d, lph, st) : backward<TYPE, VEC, 1, 4, INSIDE>(d, lph, st);
 }
 
 template <int TYPE, int ITEMS>
 int by_element(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
   if (!bwd) return forward<TYPE, 1, ITEMS, 1, false>(d, lph, st);
-  return d.wq || d.wk ? backward_normed<TYPE, 1, ITEMS, false>(d, lph, st) : backward<TYPE, 1, ITEMS, 1, false>(d, lph, st);
+  return d.wq || d.wk ? backward_normed<TYPE, 1, ITEMS, false, false>(d, lph, st) : backward<TYPE, 1, ITEMS, 1, false>(d, lph, st);
 }
 
 template <int TYPE>
