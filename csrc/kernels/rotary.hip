@@ -513,22 +513,24 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
   }
 }
 
-// weight gradients from the blocks' partials: 16 columns a block, 64 rows of it side by side, in a fixed order
+// weight gradients from the blocks' partials, in 64 bits (up to 1024 of them): 16 columns a block, 64 rows of it side by
+// side, in a fixed order
 __global__ __launch_bounds__(1024) void rotary_fold_kernel(const RotDesc d, int nbq, int nb) {
-  __shared__ float red[64][17];
+  __shared__ double red[64][17];
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
-  float v = 0.f;
+  double s = 0.0;
   if (e < 2 * d.D) {
 #pragma unroll 4
     for (int r = row + (e < d.D ? 0 : nbq); r < (e < d.D ? nbq : nb); r += 64)
-      v += d.part[(long long)r * d.D + (e < d.D ? e : e - d.D)];
+      s += d.part[(long long)r * d.D + (e < d.D ? e : e - d.D)];
   }
-  red[row][col] = v;
+  red[row][col] = s;
   __syncthreads();
   if (threadIdx.x >= 16 || e >= 2 * d.D) return;
-  v = 0.f;
+  s = 0.0;
 #pragma unroll
-  for (int i = 0; i < 64; ++i) v += red[i][col];
+  for (int i = 0; i < 64; ++i) s += red[i][col];
+  const float v = (float)s;
   void* o = e < d.D ? d.dwq : d.dwk;
   const int i = e < d.D ? e : e - d.D;
   if (!o) return;
