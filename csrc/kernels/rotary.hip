@@ -24,7 +24,7 @@ struct RotDesc {
   void *qo, *ko, *vo;                   // outputs, contiguous [T, H, D]; ko / vo: the caches when slots is set
   const void *wq, *wk;                  // norm weights [D] or null
   const double* freqs;                  // [R / 2]
-  const long long* pos;                 // [T]
+  const long long* pos;                 // [T]; null: nothing turns
   const int* slots;                     // [T] or null
   float* part;                          // backward: weight-gradient partials [blocks][D]
   void *dwq, *dwk;                      // backward: weight gradients
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
         xb[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.cb[it]);
       }
     }
-    const double pos = (double)d.pos[t];
+    const double pos = CACHE && !d.pos ? 0.0 : (double)d.pos[t];
     const long long slot = CACHE ? d.slots[t] : 0;
     const bool live = !CACHE || (slot >= 0 && slot < d.nslots);
     const long long page = CACHE ? slot / d.page : 0;
@@ -649,10 +649,10 @@ int dispatch(const RotDesc& d, bool bwd, hipStream_t st) {
 }
 
 int run(const RotDesc* d, bool bwd, hipStream_t st) {
-  if (!d || d->T < 0 || d->Hq < 1 || d->Hk < 1 || d->D < 1 || d->D > 512 || d->R < 0 || d->R > d->D ||
-      d->R % 2)
+  if (!d || d->T < 0 || d->Hq < (d->slots ? 0 : 1) || d->Hk < 1 || d->D < 1 || d->D > 512 || d->R < 0 || d->R > d->D ||
+      d->R % 2 || (d->T > 0 && !d->pos && (d->R || !d->slots)))
     return -1;
-  if (d->slots && (d->page < 8 || d->page % 8 || d->nslots < 0)) return -2;
+  if (d->slots && (d->page < 8 || d->page % 8 || d->nslots < 0 || !aligned(d->vo))) return -2;
   if (d->T == 0) {                         // no tokens: the weight gradients are zero
     if (!bwd || !(d->wq || d->wk)) return 0;
     hipLaunchKernelGGL(rotary_fold_kernel, dim3((2 * d->D + 15) / 16), dim3(1024), 0, st, *d, 0, 0);

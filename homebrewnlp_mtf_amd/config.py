@@ -115,6 +115,11 @@ _DEFAULTS: typing.Dict[str, typing.Any] = dict(
     hip_graphs_distributed=False,
     kv_cache=True,               # incremental decoding over per-layer KV caches for causal-attention bodies (Sampler)
     decode_hip_graphs=True,      # replay the single-token decode step from a hipGraph (Model._decode_graphed)
+    kv_page_size=0,              # tokens a page of the paged KV cache (16, 32, 64, 128, 256; ops/paged.py); 0: one dense
+                                 # [batch, sequence] cache per layer. Pages hold what the requests need, not the whole context
+    # attention-dot_product-context-rotary: rotary positions of queries and keys (ops/rotary.py); -qk_norm: their norm per head
+    rotary_theta=10000.0, rotary_fraction=1.0, rotary_interleaved=False,
+    rotary_scaling=None,         # {"type": "linear" | "base" | "ramp", "factor": s, ...} (rotary.rotary_freqs)
     log_every=10, metrics_path=None, pad_vocab_to=128,
     tokenizer_path=None,         # tokenizers JSON for vocab_size > 256 (the reference downloads GPT-2's)
     web_host="0.0.0.0", web_port=62220, serve_max_batch=8,
@@ -178,6 +183,11 @@ class ModelParameter:
             self.language_token_per_frame = self.sequence_length
         if self.macro_batching > 1 and self.grad_accumulation > 1 and self.macro_batching % self.grad_accumulation:
             raise ValueError('"macro_batching" needs do be divisible by "grad_accumulation"')
+
+        if self.kv_page_size not in (0, 16, 32, 64, 128, 256):
+            raise ValueError(f"kv_page_size must be 0, 16, 32, 64, 128 or 256, got {self.kv_page_size}")
+        if not 0 < self.rotary_fraction <= 1:
+            raise ValueError(f"rotary_fraction must be in (0, 1], got {self.rotary_fraction}")
 
         self.torch_storage_dtype = _DTYPES[self.storage_dtype]
         self.torch_calculation_dtype = _DTYPES[self.calculation_dtype]

@@ -15,6 +15,7 @@ import typing
 import torch
 
 from ..config import Dim, ModelParameter
+from ..ops import paged
 from . import dims as D
 from .variables import ParamStore, Scope, SharedCache
 
@@ -30,6 +31,41 @@ class Act:
 
     def __repr__(self):
         return f"Act({[f'{d.name}:{d.size}' for d in self.dims]})"
+
+
+class Pages:
+    """The pages of one decode (``kv_page_size``): every request reserves what it needs at the prefill, in one table for
+    all layers. Buffers outlive the request (KVCache.persist) while they are large enough, so the decode step's graph
+    keeps their addresses."""
+
+    def __init__(self, persist: dict, page: int, need: typing.List[int], prompt: torch.Tensor, S: int):
+        dev, B = prompt.device, len(need)
+        total, T = sum(-(-n // page) for n in need), sum(need)
+        old = persist["bufs"].get("pages")
+        if old is None or old["key"] != (B, S, page, dev) or old["count"] < total:
+            old = persist["bufs"]["pages"] = {"key": (B, S, page, dev), "count": max(total, 1), "table": torch.empty(
+                B, -(-S // page), dtype=torch.int32, device=dev)}
+            persist["graph"] = None
+        self.page, self.count, self.table = page, old["count"], old["table"]
+        self.table.fill_(-1)          # a position that was not reserved has no slot
+
+        def i32(v):
+            return torch.tensor(v, dtype=torch.int32, device=dev)
+        plan = paged.page_plan(i32([0] * B), i32(need), self.table, torch.arange(self.count, dtype=torch.int32, device=dev),
+                               i32([self.count]), page, tokens=T)
+        # the prompt's slots in the prefill's [B, S] layout
+        at = torch.arange(S, device=dev)
+        idx = (plan.start[:B, None].long() + at).clamp(max=T - 1)
+        self.pos = at.expand(B, S).reshape(-1)
+        self.prompt_slots = torch.where(at < prompt.view(B, 1), plan.slots[idx], -1).reshape(-1).contiguous()
+        self.slots: typing.Optional[torch.Tensor] = None
+        self.lens: typing.Optional[torch.Tensor] = None
+
+    def step(self, pos: torch.Tensor):
+        """slots and lengths of the decode step's tokens, one a request at ``pos`` (on the device, once a step)"""
+        ids = self.table.gather(1, torch.div(pos, self.page, rounding_mode="floor").unsqueeze(1)).squeeze(1).long()
+        self.slots = (ids * self.page + pos % self.page).int()
+        self.lens = (pos + 1).int()
 
 
 class KVCache:
@@ -51,6 +87,20 @@ class KVCache:
         # state that outlives one request: cache buffers per layer (reused while the shape stays) and the decode
         # step's hipGraph (Model._decode_graphed), which bakes their addresses in
         self.persist = persist if persist is not None else {"bufs": {}, "graph": None}
+        self.pages: typing.Optional[Pages] = None     # paged k / v caches (layers: their pools) instead of dense ones
+
+    def keep_paged(self, i: int, k: torch.Tensor, v: torch.Tensor, scale: float):
+        """the prompts' k / v [B, S, H, D] into the pages of attention layer ``i``"""
+        pg, (B, S, H, Dh) = self.pages, k.shape
+        bufs = self.persist["bufs"]
+        old = bufs.get(("pool", i))
+        if (old is None or old[0].shape != (pg.count, H, pg.page, Dh) or old[0].dtype != k.dtype
+                or old[0].device != k.device):
+            old = bufs[("pool", i)] = paged.page_pools(pg.count, pg.page, H, Dh, k.dtype, k.device)
+            self.persist["graph"] = None
+        k, v = k.reshape(B * S, H, Dh), v.reshape(B * S, H, Dh)
+        paged.append(k, v, *old, pg.prompt_slots)
+        self.layers[i] = (*old, scale)
 
     def keep(self, i: int, k: torch.Tensor, v: torch.Tensor, scale: float):
         bufs = self.persist["bufs"]
@@ -114,6 +164,8 @@ class Builder:
         if self.kv is not None:
             self.kv.idx = 0
             self.kv.cidx = 0
+            if self.kv.pages is not None and self.kv.mode == "decode":
+                self.kv.pages.step(self.kv.pos)
         if self.register:
             self.use_counts = {}
 

@@ -19,6 +19,7 @@ import torch
 from ..config import Dim, anonymize_dim, unanonymize_dim
 from ..ops import aux as X
 from ..ops import functional as F
+from ..ops import paged, rotary
 from ..ops import raw as R
 from ..parallel import state as pstate
 from . import dims as D
@@ -543,18 +544,78 @@ def _attention_fast_ok(args: BlockArgs, ins, outs) -> bool:
     return True
 
 
-def _attention_kv(kv, x: Act, w_in, ws, w_in_dims, base_dims, w_out_dims, act_in, scale: float) -> Act:
-    """causal dot-product attention with a KV cache (serving): prefill keeps k / v of the whole context; a decode
-    step appends the new token's k / v and attends its query over the row's prefix in one kernel"""
-    base = F.linear(x.t, w_in, x.dims, w_in_dims, base_dims, act=act_in)
-    k, q, v = (F.linear(base, w, base_dims, w_out_dims, x.dims).contiguous() for w in ws)
+class _Turn:
+    """what the ``rotary`` / ``qk_norm`` extras do to queries and keys (ops/rotary.py): frequencies and norm weights, None
+    where the extra is absent"""
+
+    def __init__(self, args: BlockArgs):
+        p, b = args.params, args.builder
+        if pstate.tp_size() > 1 and 'qk_norm' in args:
+            raise NotImplementedError("qk_norm: its weights are shared by the heads, their gradients are not summed over TP")
+        ws = [_scoped(args, "qk_norm", normal_var, args, [p.key_dim], 0.02, 1.0) if 'qk_norm' in args else None
+              for _ in range(2)]
+        self.kw = dict(freqs=None, interleaved=bool(p.rotary_interleaved), mscale=1.0, q_weight=ws[0], k_weight=ws[1],
+                       eps=R.EPS)
+        self.builder = b
+        if 'rotary' in args:
+            rot = int(p.key_dim.size * p.rotary_fraction) // 2 * 2
+            dev = "meta" if b.register else b.device
+            scaling = p.rotary_scaling
+            cache = b.__dict__.setdefault("_rotary_cache", {})       # constants of the config, kept on the device
+            key = (rot, float(p.rotary_theta), str(sorted(scaling.items()) if scaling else None), str(dev))
+            if key not in cache:
+                freqs, m = rotary.rotary_freqs(rot, float(p.rotary_theta), scaling)
+                cache[key] = (freqs.to(dev), m)
+            self.kw["freqs"], self.kw["mscale"] = cache[key]
+
+    def positions(self, B: int, S: int) -> torch.Tensor:
+        b = self.builder
+        dev = "meta" if b.register else b.device
+        cache = b.__dict__.setdefault("_rotary_cache", {})
+        if ("pos", B, S, str(dev)) not in cache:
+            cache["pos", B, S, str(dev)] = torch.arange(S, device=dev).expand(B, S).contiguous()
+        return cache["pos", B, S, str(dev)]
+
+    def __call__(self, q, k, pos):
+        return rotary.rotary(q, k, pos, **self.kw)
+
+
+def _qkv(x: Act, w_in, ws, w_in_dims, base_dims, w_out_dims, act_in):
+    """the attention's projections as separate products: (q, k, v)"""
+    tp = pstate.tp_size() > 1
+
+    def lin(t, w, xd, wd, od, act=None):
+        if act and tp and F.linear_plan(tuple(xd), tuple(wd), tuple(od)).row_parallel:
+            return F.activation(F.linear(t, w, xd, wd, od), act)      # the all-reduce precedes the activation
+        return F.linear(t, w, xd, wd, od, act=act)
+    base = lin(x.t, w_in, x.dims, w_in_dims, base_dims, act_in)
+    k, q, v = (lin(base, w, base_dims, w_out_dims, x.dims) for w in ws)
+    return q, k, v
+
+
+def _attention_kv(kv, x: Act, w_in, ws, w_in_dims, base_dims, w_out_dims, act_in, scale: float,
+                  turn: typing.Optional[_Turn] = None) -> Act:
+    """causal dot-product attention with a KV cache (serving): prefill keeps k / v of the whole context (paged caches: of
+    the prompts); a decode step appends the new token's k / v and attends its query over the row's prefix"""
+    q, k, v = (t.contiguous() for t in _qkv(x, w_in, ws, w_in_dims, base_dims, w_out_dims, act_in))
     i = kv.idx
     kv.idx += 1
+    B, S, H, Dh = q.shape
     if kv.mode == "prefill":
-        kv.keep(i, k, v, scale)          # the scale may depend on the context length (attention_scale "sequence")
+        if turn is not None:
+            q, k = turn(q, k, turn.positions(B, S))
+        # the scale may depend on the context length (attention_scale "sequence")
+        (kv.keep if kv.pages is None else kv.keep_paged)(i, k, v, scale)
         return Act(F.attention_core(q, k, v, scale, True), x.dims)
     K, V, scale = kv.layers[i]
-    B, S, H, Dh = K.shape
+    if kv.pages is not None:
+        q, k, v = (t.view(B, H, Dh) for t in (q, k, v))
+        q = paged.rotary_append(q, k, v, K, V, kv.pages.slots, kv.pos, **(turn.kw if turn is not None else {"freqs": None}))
+        o = paged.paged_attn(q, K, V, kv.pages.table, kv.pages.lens, scale)
+        return Act(o.view(B, S, H, Dh), x.dims)
+    if turn is not None:
+        q, k = turn(q, k, kv.pos.view(B, 1))
+    S = K.shape[1]
     o = torch.empty_like(q)
     R.decode_attn(q, k, v, K, V, o, kv.pos, B, S, H, Dh, scale)
     return Act(o, x.dims)
@@ -623,7 +684,8 @@ def _note_mixer(args: BlockArgs, dim: Dim, causal: bool, before) -> None:
 
 
 def attention(args: BlockArgs) -> Act:
-    """ref spatial.py:42-81 (all variants). Fast path: dot_product + context (causal flash attention)."""
+    """ref spatial.py:42-81 (all variants). Fast path: dot_product + context (causal flash attention), there also with
+    ``rotary`` positions and ``qk_norm`` (this framework's own extras)."""
     p = args.params
     p.attention_idx += 1
     x = args.tensor
@@ -637,6 +699,10 @@ def attention(args: BlockArgs) -> Act:
         scale = p.key_dim.size ** -0.5
     causal = D.is_masked(p, x.dims)
 
+    turned = 'rotary' in args or 'qk_norm' in args
+    if turned and not _attention_fast_ok(args, ins, outs):
+        raise ValueError("attention extras rotary / qk_norm need plain dot_product-context attention over the sequence, got "
+                         f"{args.name_extras}")
     if _attention_fast_ok(args, ins, outs):
         a_in = args(ins)
         act_in = next((a for a in ins if a in ACTIVATIONS), None)
@@ -646,10 +712,17 @@ def attention(args: BlockArgs) -> Act:
         old2, new2 = D.linear_shapes(p, a_out, base_dims)
         w_in = _scoped(a_in, "linear", orthogonal_var, a_in, list(old1) + list(new1), list(old1))
         ws = [_scoped(a_out, "linear", orthogonal_var, a_out, list(old2) + list(new2), list(old2)) for _ in range(3)]
+        turn = _Turn(args) if turned else None
         kv = args.builder.kv
         if kv is not None and causal and pstate.tp_size() == 1:
             return _attention_kv(kv, x, w_in, ws, D.deduplicate(old1 + new1), base_dims, D.deduplicate(old2 + new2),
-                                 act_in, scale)
+                                 act_in, scale, turn)
+        if turn is not None:
+            if kv is not None:
+                kv.unsupported = True
+            q, k, v = _qkv(x, w_in, ws, D.deduplicate(old1 + new1), base_dims, D.deduplicate(old2 + new2), act_in)
+            q, k = turn(q, k, turn.positions(x.dims[0].size, x.dims[1].size))
+            return Act(F.attention_core(q, k, v, scale, causal), x.dims)
         res = args.residual if (args.residual is not None and args.residual.dims == x.dims) else None
         geo = (x.dims[0].size, x.dims[1].size, p.head_dim.size, p.key_dim.size)
         try:

@@ -20,9 +20,10 @@ import torch
 from ..config import Dim, ModelParameter
 from ..ops import aux as X
 from ..ops import functional as F
+from ..ops import paged
 from ..ops import raw as R
 from . import dims as D
-from .context import Act, BlockArgs, Builder, KVCache
+from .context import Act, BlockArgs, Builder, KVCache, Pages
 from .frontend import block_part_fn
 from .layers import embed, gather_embed, linear, linear_to_features, named_einsum, dropout
 from .reversible import run_body
@@ -120,12 +121,24 @@ class Model:
                 and not (p.contrastive_across_samples or p.contrastive_across_token_embeddings))
 
     @torch.no_grad()
-    def prefill(self, token_x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+    def prefill(self, token_x: torch.Tensor, positions: torch.Tensor,
+                need: typing.Optional[torch.Tensor] = None) -> torch.Tensor:
         """Start incremental decoding: one forward over the whole context that fills the per-layer KV caches;
-        returns the logits at ``positions`` ([B, 1, patch, vocab])"""
+        returns the logits at ``positions`` ([B, 1, patch, vocab]). With ``kv_page_size`` the caches are pages for the
+        tokens up to ``positions``, with room for ``need`` tokens of each row ([B]; default: the whole context)"""
         if not hasattr(self, "_kv_persist"):
             self._kv_persist = {"bufs": {}, "graph": None}
         kv = KVCache(self._kv_persist)
+        page = int(self.params.kv_page_size)
+        if page:
+            S, dim = token_x.shape[1], self.params.key_dim.size
+            if self.device.type == "cuda" and (dim not in paged.HEAD_DIMS or self.dtype not in (torch.bfloat16,
+                                                                                              torch.float16)):
+                raise ValueError(f"kv_page_size on the GPU needs features_per_head in {paged.HEAD_DIMS} and 16-bit "
+                                 f"activations, got {dim} in {self.dtype}")
+            prompt = (positions.to(self.device).long() + 1).clamp(1, S)
+            need = torch.full_like(prompt, S) if need is None else torch.maximum(need.to(prompt), prompt).clamp(max=S)
+            kv.pages = Pages(self._kv_persist, page, need.tolist(), prompt, S)
         self.builder.kv = kv
         try:
             out = self.logits(token_x, positions=positions)
@@ -158,7 +171,7 @@ class Model:
         k / v), so the eager warm-up runs feed the very step they warm up. The returned logits are the graph's
         static output: valid until the next step."""
         g = kv.persist["graph"]
-        if g is None or g["shape"] != tuple(tokens.shape):
+        if g is None or g["shape"] != (tuple(tokens.shape), kv.pages is not None):
             tok = tokens.to(self.device).clone()
             kv.pos = positions.to(self.device, torch.int64).clone()
             side = torch.cuda.Stream(self.device)
@@ -170,7 +183,7 @@ class Model:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 out = self.logits(tok)
-            g = kv.persist["graph"] = {"shape": tuple(tokens.shape), "graph": graph, "tok": tok, "pos": kv.pos,
+            g = kv.persist["graph"] = {"shape": (tuple(tokens.shape), kv.pages is not None), "graph": graph, "tok": tok, "pos": kv.pos,
                                        "out": out}
         else:
             g["tok"].copy_(tokens, non_blocking=True)

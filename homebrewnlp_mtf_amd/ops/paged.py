@@ -21,7 +21,7 @@ import torch
 
 from . import _lib as L
 from . import raw
-from .rotary import DTYPES, check_args, kernel_weights, rotary_t, tokens_view
+from .rotary import DTYPES, MAX_DIM, check_args, kernel_weights, rotary_t, tokens_view
 
 HEAD_DIMS = (32, 64, 96, 128, 256)
 PAGES = (16, 32, 64, 128, 256)
@@ -186,6 +186,8 @@ def _pools(what: str, k_cache, v_cache, q, dev: int, D: int, heads: typing.Optio
     if (k_cache.dtype != dt or v_cache.dtype != dt or k_cache.get_device() != dev or v_cache.get_device() != dev
             or not k_cache.is_contiguous() or not v_cache.is_contiguous()):
         raise L.KernelError(f"{what}: caches must be contiguous {dt} on the device of q")
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16 and dev >= 0:
+        raise L.KernelError(f"{what}: caches must be 16-byte aligned")
     return P, H, page
 
 
@@ -233,13 +235,46 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
             eps))
         return out
     # ---- torch oracle
-    ko = rotary_t(k, None if k_weight is None else k_weight.detach(), pos, freqs, interleaved, mscale, eps)
-    live = (slots >= 0) & (slots < P * page)
-    s = slots[live].long()
-    k_cache[s // page, :, s % page] = ko[live]
-    v_cache[s // page, :, s % page // 8, :, s % 8] = v[live]
+    _scatter_t(rotary_t(k, None if k_weight is None else k_weight.detach(), pos, freqs, interleaved, mscale, eps), v,
+               k_cache, v_cache, slots)
     out.copy_(rotary_t(q, None if q_weight is None else q_weight.detach(), pos, freqs, interleaved, mscale, eps))
     return out
+
+
+def append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor) -> None:
+    """keys and values [T, Hk, D] as they are into the cache at ``slots`` (as ``rotary_append`` writes them): for prompts
+    whose turned keys their own attention has read"""
+    ks, dev = k.shape, k.get_device()
+    if len(ks) != 3 or v.shape != ks or v.dtype != k.dtype or v.get_device() != dev or ks[1] < 1 or not 1 <= ks[2] <= MAX_DIM:
+        raise L.KernelError(f"append: k and v [T, Hk, D] of one type, D up to {MAX_DIM}, got {list(ks)}, {list(v.shape)}")
+    if dev >= 0 and k.dtype not in DTYPES:
+        raise L.KernelError(f"append: bf16, fp16 or fp32 on the GPU, got {k.dtype}")
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+        raise L.KernelError("append has no gradient: call it under torch.no_grad()")
+    T, Hk, D = ks
+    P, Hk, page = _pools("append", k_cache, v_cache, k, dev, D, Hk)
+    _ints("append", dev, ("slots", slots))
+    if slots.dim() != 1 or slots.numel() != T:
+        raise L.KernelError(f"append: slots {list(slots.shape)} for {T} tokens")
+    if T == 0 or k.is_meta:
+        return
+    if dev >= 0:
+        k, k_ts, k_hs = tokens_view(k)
+        v, v_ts, v_hs = tokens_view(v)
+        L.launch(L.lib().obst_rotary_fwd, k, "append", L.ROT_DESC.pack(
+            0, k.data_ptr(), v.data_ptr(), 0, 0, 0, k_cache.data_ptr(), v_cache.data_ptr(), 0, 0, 0, 0, slots.data_ptr(), 0,
+            0, 0, 0, 0, k_ts, k_hs, v_ts, v_hs, 0, 0, 0, 0, T, P * page, 0, Hk, D, 0, 0, DTYPES[k.dtype], 0, 0, 0, page,
+            1.0, 1.0))
+        return
+    _scatter_t(k, v, k_cache, v_cache, slots)
+
+
+def _scatter_t(k, v, k_cache, v_cache, slots):
+    P, _, page, _ = k_cache.shape
+    live = (slots >= 0) & (slots < P * page)
+    s = slots[live].long()
+    k_cache[s // page, :, s % page] = k[live]
+    v_cache[s // page, :, s % page // 8, :, s % 8] = v[live]
 
 
 # ----------------------------------------------------------------------------------------------------------------
@@ -286,8 +321,6 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
         if q_ds != 1 or (q_bs | q_hs) % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
             q_bs, q_hs = Hq * D, D
-        if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
-            raise L.KernelError("paged_attn: caches must be 16-byte aligned")
         nsplit, split = _splits(B * rows, cap)
         part = q.new_empty(B * Hq * nsplit * (D + 2), dtype=torch.float32) if nsplit > 1 else None
         L.launch(L.lib().obst_paged_attn, q, "paged_attn", L.PAGED_DESC.pack(

@@ -130,7 +130,7 @@ class Sampler:
         B, S = x.shape[0], x.shape[1]
         m = self.model
         try:
-            logits = m.prefill(x, (pos - 1).clamp(max=S - 1))
+            logits = m.prefill(x, (pos - 1).clamp(max=S - 1), need=end)
         except NotImplementedError:
             self.kv_cache = False
             return self.sample(x, pos, temp, end)

@@ -442,3 +442,95 @@ def test_rotary_backward_in_a_graph(cuda):
         gr.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(out, run(q, k, gq, gk)))
+
+
+# ----------------------------------------------------------------------------------------------------------------
+def test_plain_append_gpu(cuda):
+    g = gen(cuda, 60)
+    for D, Hk, page, dtype in ((128, 4, 16, BF), (33, 1, 32, HF), (64, 3, 64, F32)):
+        k, v = (torch.randn(50, Hk, D, device=cuda, generator=g).to(dtype) for _ in range(2))
+        slots = torch.arange(3, 53, dtype=torch.int32, device=cuda)
+        slots[7] = -1
+        kc, vc = paged.page_pools(5, page, Hk, D, dtype, cuda)
+        kc.zero_()
+        vc.zero_()
+        cpu = [t.cpu() for t in (kc, vc)]
+        paged.append(k, v, kc, vc, slots)
+        paged.append(k.cpu(), v.cpu(), *cpu, slots.cpu())
+        assert torch.equal(kc.cpu(), cpu[0]) and torch.equal(vc.cpu(), cpu[1])
+
+
+def _model(cuda, **kw):
+    from homebrewnlp_mtf_amd.config import ModelParameter
+    from homebrewnlp_mtf_amd.models.model import Model
+    from homebrewnlp_mtf_amd.parallel import state as pstate
+    pstate.set_mesh(pstate.Mesh())
+    torch.manual_seed(0)
+    cfg = dict(model_mode="gpt", use_video=False, use_language=True, heads=2, features_per_head=64, depth=2,
+               sequence_length=96, train_batch_size=3, vocab_size=256, calculation_dtype="bfloat16",
+               storage_dtype="bfloat16", block_config=[
+                   {"layer": ["norm-shift-scale", "attention-dot_product-context-rotary-qk_norm"], "skip": True},
+                   {"layer": ["norm-shift-scale", "feed_forward-in:gelu"], "skip": True}],
+               memory_reduction_strategy="none", **kw)
+    p = ModelParameter(cfg)
+    return Model(p, cuda), p
+
+
+def test_model_paged_decoding_gpu(cuda):
+    """paged caches: the replayed decode graph gives the eager steps' tokens exactly, over requests of several sizes (the
+    pool grows, the graph is taken anew); the steps' logits are the full recompute's but for bf16 roundings, as those of
+    dense caches of the same model are"""
+    from homebrewnlp_mtf_amd.run.infer import Sampler
+    m, p = _model(cuda, kv_page_size=16)
+    rows = torch.arange(3, device=cuda)
+    for seed, start, end in ((1, [3, 7, 1], [16, 30, 9]), (2, [60, 2, 90], [96, 40, 96]), (3, [5, 5, 5], [20, 20, 20])):
+        x = torch.randint(0, 256, (3, 96, 1), generator=torch.Generator().manual_seed(seed)).to(cuda)
+        got = []
+        for graphs in (True, False, True):
+            p.decode_hip_graphs = graphs
+            s = Sampler(m, p, cuda)
+            got.append(s.sample(x, start, 0.0, end))
+            assert s.kv_cache
+        assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+        full = m.logits(got[0])[:, :, 0]
+        pos = torch.tensor(start, device=cuda)
+        for page in (16, 0):
+            p.kv_page_size = page
+            step = m.prefill(got[0], pos - 1)
+            for i in range(10):
+                cur = (pos + i - 1).clamp(max=95)
+                if i:
+                    step = m.decode(got[0][rows, cur].unsqueeze(1), cur)
+                ref = full[rows, cur]
+                # two layers of about ten bf16 roundings each, every one off by 2^-8 of what it rounds at most
+                assert bool(((step[:, 0, 0] - ref).norm(dim=-1) <= 20 * 2.0 ** -8 * ref.norm(dim=-1)).all())
+            m.end_decode()
+        p.kv_page_size = 16
+    x = torch.randint(0, 256, (3, 96, 1), device=cuda)
+    bad, _ = _model(cuda)
+    bad.params.kv_page_size = 16
+    bad.dtype = torch.float32
+    with pytest.raises(ValueError):
+        bad.prefill(x, torch.tensor([1, 1, 1], device=cuda))
+
+
+def test_model_rotary_training_gpu(cuda):
+    """one training step's gradients on the GPU point where the CPU oracle's do (bf16 activations through two layers)"""
+    from homebrewnlp_mtf_amd.models.model import Model
+    m, p = _model(cuda, rotary_fraction=0.5)
+    c = Model(p, "cpu")
+    c.store.master.copy_(m.store.master)
+    if c.store.compute.data_ptr() != c.store.master.data_ptr():
+        c.store.compute.copy_(c.store.master)
+    t = torch.randint(0, 256, (3, 97, 1), generator=torch.Generator().manual_seed(3))
+    for mm, dev in ((m, cuda), (c, "cpu")):
+        mm.store.grad.zero_()
+        mm(token_x=t[:, :-1].contiguous().to(dev), token_y=t[:, 1:].contiguous().to(dev))["loss"].backward()
+    names = [n for n in m.store.order if "qk_norm" in n]
+    assert len(names) == 4
+    for n in names:
+        sp = m.store.specs[n]
+        a, b = (mm.store.grad[sp.offset:sp.offset + sp.numel].cpu() for mm in (m, c))
+        assert torch.nn.functional.cosine_similarity(a, b, dim=0) > 0.97, n
+    cos = torch.nn.functional.cosine_similarity(m.store.grad.cpu(), c.store.grad, dim=0)
+    assert cos > 0.97, cos

@@ -286,3 +286,122 @@ def test_step_by_step_matches_dense():
             kk, vv = torch.stack(ks[b]).repeat_interleave(2, 1), torch.stack(vs[b]).repeat_interleave(2, 1)
             s = torch.softmax(torch.einsum("hd,jhd->hj", qo[b].double(), kk) * D ** -0.5, -1)
             assert torch.allclose(o[b].double(), torch.einsum("hj,jhd->hd", s, vv), atol=1e-5)
+
+
+def test_plain_append():
+    g = torch.Generator().manual_seed(9)
+    k, v = torch.randn(4, 2, 32, generator=g), torch.randn(4, 2, 32, generator=g)
+    slots = torch.tensor([5, -1, 31, 32], dtype=torch.int32)
+    pools = [paged.page_pools(2, 16, 2, 32, torch.float32, "cpu") for _ in range(2)]
+    for kc, vc in pools:
+        kc.zero_()
+        vc.zero_()
+    paged.append(k, v, *pools[0], slots)
+    paged.rotary_append(k, k, v, *pools[1], slots, torch.zeros(4, dtype=torch.int64), None)
+    assert torch.equal(pools[0][0], pools[1][0]) and torch.equal(pools[0][1], pools[1][1])
+    for bad in (dict(k=k[:3]), dict(v=v.double()), dict(slots=slots.long()), dict(slots=slots[:3]), dict(k=k[0]),
+                dict(k_cache=pools[0][0].double()), dict(k=k.clone().requires_grad_())):
+        with pytest.raises(L.KernelError):
+            paged.append(**{**dict(k=k, v=v, k_cache=pools[0][0], v_cache=pools[0][1], slots=slots), **bad})
+
+
+# ----------------------------------------------------------------------------------------------------------------
+def _params(**kw):
+    from homebrewnlp_mtf_amd.config import ModelParameter
+    cfg = dict(model_mode="gpt", use_video=False, use_language=True, heads=2, features_per_head=8, depth=2,
+               sequence_length=16, train_batch_size=3, vocab_size=64, intermediate_feed_forward_multiplier=2,
+               memory_reduction_strategy="none", calculation_dtype="float32", learning_rate=0.01,
+               optimizer="adam-learning_rate",
+               block_config=[{"layer": ["norm-shift-scale", "attention-dot_product-context-rotary-qk_norm"], "skip": True},
+                             {"layer": ["norm-shift-scale", "feed_forward-in:gelu"], "skip": True}])
+    cfg.update(kw)
+    return ModelParameter(cfg)
+
+
+ROTARY = dict(rotary_fraction=0.5, rotary_interleaved=True, rotary_scaling={"type": "ramp", "factor": 4.0, "length": 8})
+
+
+@pytest.mark.parametrize("strategy", ["none", "revnet"])
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("extras", ["-rotary-qk_norm", "-rotary", "-qk_norm", ""])
+def test_model_decodes_like_full_recompute(extras, page, strategy, monkeypatch):
+    """rotary / qk_norm attention under dense and paged caches: the tokens of the full recompute, rows of different
+    lengths, one of them done from the start, twice with one model (buffers of another request)"""
+    from homebrewnlp_mtf_amd.models.model import Model
+    from homebrewnlp_mtf_amd.parallel import state as pstate
+    from homebrewnlp_mtf_amd.run.infer import Sampler
+    pstate.set_mesh(pstate.Mesh())
+    torch.manual_seed(0)
+    p = _params(kv_page_size=page, memory_reduction_strategy=strategy, sequence_length=40, **ROTARY, block_config=[
+        {"layer": ["norm-shift-scale", "attention-dot_product-context" + extras], "skip": True},
+        {"layer": ["norm-shift-scale", "feed_forward-in:gelu"], "skip": True}])
+    m = Model(p, "cpu")
+    calls = []
+    real = paged.paged_attn
+    monkeypatch.setattr(paged, "paged_attn", lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    for seed, start, end in ((4, [3, 7, 1], [16, 40, 9]), (5, [30, 2, 40], [40, 8, 12])):
+        x = torch.randint(0, 64, (3, 40, 1), generator=torch.Generator().manual_seed(seed))
+        for temp in (0.0, [0.0, 1.0, 3.0]):
+            cached, full = Sampler(m, p, "cpu"), Sampler(m, p, "cpu")
+            full.kv_cache = False
+            a = cached.sample(x, start, temp, end)
+            assert cached.kv_cache and bool(calls) == bool(page)
+            assert torch.equal(a, full.sample(x, start, temp, end))
+    assert m.builder.kv is None
+
+
+def test_model_rotary_positions_matter_and_train():
+    """the rotation changes the logits, and one step's gradients match differences (fp64 model)"""
+    from homebrewnlp_mtf_amd.models.model import Model
+    from homebrewnlp_mtf_amd.parallel import state as pstate
+    pstate.set_mesh(pstate.Mesh())
+    torch.manual_seed(0)
+    p = _params(**ROTARY)
+    m = Model(p, "cpu", dtype=torch.float64)
+    names = [n for n in m.store.order if "qk_norm" in n]
+    assert len(names) == 4 and all(m.store.specs[n].full_shape == [8] for n in names)
+    g = torch.Generator().manual_seed(1)
+    t = torch.randint(0, 64, (3, 17, 1), generator=g)
+    batch = {"token_x": t[:, :-1].contiguous(), "token_y": t[:, 1:].contiguous()}
+    base = m.logits(batch["token_x"])
+    m.params.rotary_theta = m.builder.params.rotary_theta = 50.0
+    assert not torch.allclose(base, m.logits(batch["token_x"]))
+    with pytest.raises(ValueError):
+        Model(_params(block_config=[{"layer": ["attention-dot_product-embedded-absolute-rotary"]}]), "cpu")
+    for bad in (dict(kv_page_size=24), dict(rotary_fraction=0.0), dict(rotary_fraction=1.5)):
+        with pytest.raises(ValueError):
+            _params(**bad)
+
+
+def test_trainer_steps_with_rotary_attention():
+    """gradients of the qk_norm weights through a whole training step against differences of the loss"""
+    from homebrewnlp_mtf_amd.parallel import state as pstate
+    from homebrewnlp_mtf_amd.run.trainer import Trainer
+    pstate.set_mesh(pstate.Mesh())
+    torch.manual_seed(0)
+    tr = Trainer(_params(**ROTARY), "cpu")
+    st = tr.store if hasattr(tr, "store") else tr.model.store
+    g = torch.Generator().manual_seed(2)
+    t = torch.randint(0, 64, (3, 17, 1), generator=g)
+    batch = {"token_x": t[:, :-1].contiguous(), "token_y": t[:, 1:].contiguous()}
+
+    def loss():
+        return tr.model(**batch)["loss"]
+    name = next(n for n in st.order if "qk_norm" in n)
+    out = loss()
+    st.zero_grad() if hasattr(st, "zero_grad") else st.grad.zero_()
+    out.backward()
+    sp = st.specs[name]
+    grad = st.grad[sp.offset:sp.offset + sp.numel].clone()
+    assert float(grad.abs().max()) > 0
+    for i in (0, 5):
+        vals = []
+        for d in (1e-2, -1e-2):
+            for buf in {st.master.data_ptr(): st.master, st.compute.data_ptr(): st.compute}.values():
+                buf[sp.offset + i] += d
+            with torch.no_grad():
+                vals.append(float(loss()))
+            for buf in {st.master.data_ptr(): st.master, st.compute.data_ptr(): st.compute}.values():
+                buf[sp.offset + i] -= d
+        # central difference: third derivatives times 1e-4 / 6, and two fp32 losses (~4, half a step 2.4e-7) over 2e-2
+        assert abs((vals[0] - vals[1]) / 2e-2 - float(grad[i])) < 1e-4 + 0.02 * abs(float(grad[i]))
