@@ -471,7 +471,7 @@ OBST_API int obst_page_release(const void* done, void* lens, const void* table, 
 }
 
 OBST_API int obst_paged_attn(const PagedDesc* d, hipStream_t st) {
-  if (!d || d->B < 1 || d->B > 65535 || d->Hk < 1 || d->Hq < 1 || d->Hq % d->Hk || d->P < 1 || d->cap < 0 ||
+  if (!d || d->B < 1 || d->B > 65535 || d->Hk < 1 || d->Hq < 1 || d->Hq % d->Hk || d->P < 1 || d->cap < 0 || d->cap > 1 << 30 ||
       d->nsplit < 1 || d->nsplit > MAX_SPLITS || d->split < 32 || d->split % 32 || (d->nsplit > 1 && !d->part))
     return -1;
   if (d->shift < 4 || d->shift > 8 || (long long)d->ld << d->shift < d->cap) return -3;

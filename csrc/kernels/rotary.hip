@@ -51,7 +51,7 @@ __device__ __forceinline__ void from_f(float f, bf16_t& o) { o = f2bf(f); }
 __device__ __forceinline__ void from_f(float f, __half& o) { o = __float2half(f); }
 
 template <typename E, int VEC>
-struct alignas(sizeof(E) * VEC) Chunk { E e[VEC]; };
+struct alignas(sizeof(E) * VEC < 16 ? sizeof(E) * VEC : 16) Chunk { E e[VEC]; };
 
 template <typename E, int VEC>
 __device__ __forceinline__ void store(E* p, const float* f) {

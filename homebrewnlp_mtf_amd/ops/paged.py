@@ -26,6 +26,7 @@ from .rotary import DTYPES, MAX_DIM, check_args, kernel_weights, rotary_t, token
 HEAD_DIMS = (32, 64, 96, 128, 256)
 PAGES = (16, 32, 64, 128, 256)
 _MAX_SLOTS = 2 ** 31 - 1
+_MAX_LEN = 2 ** 30
 
 
 def page_pools(pages: int, page: int, kv_heads: int, dim: int, dtype: torch.dtype,
@@ -71,7 +72,7 @@ def _table(what: str, table, B: int, dev: int) -> typing.Tuple[int, int]:
             or (shape[1] > 1 and st[1] != 1) or (B > 1 and not shape[1] <= st[0] < 2 ** 31)):
         raise L.KernelError(f"{what}: the table must be int32 [{B}, pages] with dense rows beside the other tensors, got "
                             f"{table.dtype} {list(shape)} strides {list(st)} on {table.device}")
-    return shape[1], max(st[0], shape[1])
+    return shape[1], st[0] if B > 1 else shape[1]
 
 
 def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stack: torch.Tensor, nfree: torch.Tensor,
@@ -303,11 +304,13 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     _ints("paged_attn", dev, ("lens", lens))
     if lens.dim() != 1 or lens.numel() != B:
         raise L.KernelError(f"paged_attn: lens {list(lens.shape)} for {B} requests")
-    cap = min(W * page, _MAX_SLOTS // page * page)
+    cap = W * page
     if max_len is not None:
         if max_len < 0:
             raise L.KernelError(f"paged_attn: max_len {max_len}")
         cap = min(cap, max_len)
+    if cap > _MAX_LEN:
+        raise L.KernelError(f"paged_attn: {cap} tokens a request (at most {_MAX_LEN}; max_len bounds a wide table)")
     out = _out("paged_attn", out, q, qs, dev)
     if B == 0 or q.is_meta:
         return out

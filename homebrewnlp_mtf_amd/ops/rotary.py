@@ -229,8 +229,8 @@ class _Rotary(torch.autograd.Function):
             elif raw.on_gpu(w) and wt_direct(ws):
                 dws[i], kept[i] = w.new_empty(w.shape), False
             else:
-                dws[i] = torch.zeros(w.shape, device=w.device, dtype=torch.float64 if w.dtype == torch.float64
-                                     else torch.float32)
+                wide = w.dtype == torch.float64 and not raw.on_gpu(w)
+                dws[i] = torch.zeros(w.shape, device=w.device, dtype=torch.float64 if wide else torch.float32)
                 kept[i] = False
         into = list(dws)
         if main and wq is not None and wk is not None and dws[0].data_ptr() == dws[1].data_ptr():

@@ -445,6 +445,29 @@ def test_rotary_backward_in_a_graph(cuda):
 
 
 # ----------------------------------------------------------------------------------------------------------------
+def test_odd_weights_and_single_rows(cuda):
+    """norm weights of two types and in 64 bits; a table of one row with a stride of no meaning"""
+    g = gen(cuda, 61)
+    q, k = torch.randn(6, 2, 64, device=cuda, generator=g).to(BF), torch.randn(6, 1, 64, device=cuda, generator=g).to(BF)
+    freqs, pos = rotary.rotary_freqs(64, device=cuda)[0], torch.arange(6, device=cuda)
+    one = torch.ones(6, 2, 64, device=cuda)
+    for a, b in ((torch.float64, torch.float64), (F32, BF), (BF, torch.float64)):
+        wq, wk = ((torch.rand(64, device=cuda, generator=g) + 0.5).to(t).requires_grad_() for t in (a, b))
+        o = rotary.rotary(q, k, pos, freqs, q_weight=wq, k_weight=wk)
+        close_rows(o[0].detach(), rotary64(q, wq.detach(), pos, freqs, False, 1.0, 1e-5), BF)
+        dq, dk = torch.autograd.grad(o[0].float().sum() + o[1].float().sum(), (wq, wk))
+        assert dq.dtype == a and dk.dtype == b
+        # weights in 64 bits are read in 32: one more rounding of each term
+        _, dw, mag = rotary_grad64(q, wq.detach(), one, pos, freqs, False, 1.0, 1e-5)
+        assert bool(((dq.double() - dw).abs() <= half_step(a) * dw.abs() + (64 + 117) * U32 * mag).all())
+    kc, vc, table, ln = make_cache([40], 16, 1, 64, BF, cuda, seed=8)
+    row = torch.empty(1, 2 ** 33, dtype=torch.int32, device="meta").stride()[0]
+    odd = torch.as_strided(table, (1, 3), (row, 1))
+    qq = q[:1]
+    ref, err = attn64(qq, kc, vc, table, ln, 0.125)
+    assert near(paged.paged_attn(qq, kc, vc, odd, ln, 0.125), ref, half_step(BF) * ref.abs() + err)
+
+
 def test_plain_append_gpu(cuda):
     g = gen(cuda, 60)
     for D, Hk, page, dtype in ((128, 4, 16, BF), (33, 1, 32, HF), (64, 3, 64, F32)):

@@ -255,6 +255,12 @@ def test_attn_refusals():
                 dict(k_cache=kc.transpose(1, 2)), dict(q=q.clone().requires_grad_())):
         with pytest.raises(L.KernelError):
             paged.paged_attn(**{**ok, **bad})
+    wide = torch.zeros(1, 2 ** 22 + 1, dtype=torch.int32)                     # pages of 256: more than 2^30 tokens
+    big = dict(q=q[:1], k_cache=torch.zeros(1, 2, 256, 32, dtype=torch.bfloat16), table=wide, lens=ln[:1], scale=1.0,
+               v_cache=torch.zeros(1, 2, 32, 32, 8, dtype=torch.bfloat16))
+    with pytest.raises(L.KernelError):
+        paged.paged_attn(**big)
+    paged.paged_attn(**big, max_len=300)
     assert paged.paged_attn(**{**ok, "q": q[:0], "table": table[:0], "lens": ln[:0]}).shape == (0, 4, 32)
 
 
