@@ -15,7 +15,6 @@ import math
 import typing
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import raw
@@ -182,7 +181,7 @@ def rotary_bwd_t(x, w, g, pos, freqs, inter: bool, mscale: float, eps: float):
 
 
 # ----------------------------------------------------------------------------------------------------------------
-def _forward(q, k, pos, freqs, rot, T, wq, wk, inter, mscale, eps):
+def _forward(q, k, pos, freqs, wq, wk, rot, T, inter, mscale, eps):
     qs, ks = q.shape, k.shape
     qo, ko = q.new_empty(qs), k.new_empty(ks)
     if T == 0 or q.is_meta:
@@ -204,19 +203,24 @@ def _forward(q, k, pos, freqs, rot, T, wq, wk, inter, mscale, eps):
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, pos, freqs, rot, T, inter, mscale, eps):
-        normed = wq is not None or wk is not None
-        ctx.save_for_backward(q if normed else None, k if normed else None, wq, wk, pos, freqs)
-        ctx.cfg = (rot, T, inter, mscale, eps)
-        return _forward(q, k, pos, freqs, rot, T, wq, wk, inter, mscale, eps)
+    def forward(ctx, q, k, wq, wk, pos, freqs, cfg):
+        ctx.cfg = cfg
+        if wq is None and wk is None:
+            ctx.save_for_backward(pos, freqs)
+        else:
+            ctx.save_for_backward(pos, freqs, q, k, wq, wk)
+        return _forward(q, k, pos, freqs, wq, wk, *cfg)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk, pos, freqs = ctx.saved_tensors
-        rot, T, inter, mscale, eps = ctx.cfg
-        gs, hs = gq.shape, gk.shape
-        dq, dk = gq.new_empty(gs), gk.new_empty(hs)
+        if torch.is_grad_enabled():
+            raise L.KernelError("rotary has no second derivative (create_graph)")
+        pos, freqs, *normed = ctx.saved_tensors
+        dq, dk = gq.new_empty(gq.shape), gk.new_empty(gk.shape)
+        if not normed:
+            _backward(None, None, gq, gk, dq, dk, None, None, None, None, False, pos, freqs, *ctx.cfg)
+            return dq, dk, None, None, None, None, None
+        q, k, wq, wk = normed
         ws = (wq, wk)
         # model parameters accumulate into their fp32 main gradient; other weights get theirs back in their own type
         main = any(getattr(w, "main_grad", None) is not None for w in ws if w is not None)
@@ -235,29 +239,7 @@ class _Rotary(torch.autograd.Function):
         into = list(dws)
         if main and wq is not None and wk is not None and dws[0].data_ptr() == dws[1].data_ptr():
             into[1] = torch.zeros(wk.shape, dtype=torch.float32, device=wk.device)   # one parameter for both
-        if not raw.on_gpu(gq):
-            for i, (x, w, g, o) in enumerate(((q, wq, gq, dq), (k, wk, gk, dk))):
-                dx, dw = rotary_bwd_t(x, None if w is None else _param32(w).detach(), g, pos, freqs, inter, mscale, eps)
-                o.copy_(dx)
-                if dw is not None:
-                    into[i].add_(dw.reshape(into[i].shape))
-        else:
-            gq, gq_ts, gq_hs = tokens_view(gq)
-            gk, gk_ts, gk_hs = tokens_view(gk)
-            q_ts = q_hs = k_ts = k_hs = 0
-            part = None
-            lib = L.lib()
-            if q is not None:
-                q, q_ts, q_hs = tokens_view(q)
-                k, k_ts, k_hs = tokens_view(k)
-                part = gq.new_empty(lib.obst_rotary_part(gs[-1]), dtype=torch.float32)
-            vq, vk, wt = kernel_weights(wq, wk)
-            dt = next((DTYPES[x.dtype] for x in into if x is not None), 0)
-            L.launch(lib.obst_rotary_bwd, gq, "rotary_bwd", L.ROT_DESC.pack(
-                L.ptr(q), L.ptr(k), 0, gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), 0, L.ptr(vq),
-                L.ptr(vk), L.ptr(freqs), pos.data_ptr(), 0, L.ptr(part), L.ptr(into[0]), L.ptr(into[1]), q_ts, q_hs,
-                k_ts, k_hs, 0, 0, gq_ts, gq_hs, gk_ts, gk_hs, T, 0, gs[-2], hs[-2], gs[-1], rot, inter,
-                DTYPES[gq.dtype], wt, dt, main, 0, mscale, eps))
+        _backward(q, k, gq, gk, dq, dk, wq, wk, into[0], into[1], main, pos, freqs, *ctx.cfg)
         if into[1] is not dws[1]:
             dws[1].add_(into[1])
         out = []
@@ -265,7 +247,34 @@ class _Rotary(torch.autograd.Function):
             if w is not None:
                 _done(w)
             out.append(None if w is None or keep else g if g.dtype == w.dtype else g.to(w.dtype))
-        return dq, dk, out[0], out[1], None, None, None, None, None, None, None
+        return dq, dk, out[0], out[1], None, None, None
+
+
+def _backward(q, k, gq, gk, dq, dk, wq, wk, dwq, dwk, add: bool, pos, freqs, rot, T, inter, mscale, eps):
+    """dq, dk and the weights' gradients (into dwq, dwk; added to what they hold in fp32 where ``add``)"""
+    if gq.get_device() < 0:
+        for x, w, g, o, dw in ((q, wq, gq, dq, dwq), (k, wk, gk, dk, dwk)):
+            dx, d = rotary_bwd_t(x, None if w is None else _param32(w).detach(), g, pos, freqs, inter, mscale, eps)
+            o.copy_(dx)
+            if d is not None:
+                dw.add_(d.reshape(dw.shape))
+        return
+    gs, lib = gq.shape, L.lib()
+    gq, gq_ts, gq_hs = tokens_view(gq)
+    gk, gk_ts, gk_hs = tokens_view(gk)
+    q_ts = q_hs = k_ts = k_hs = wt = dt = 0
+    part = None
+    if q is not None:
+        q, q_ts, q_hs = tokens_view(q)
+        k, k_ts, k_hs = tokens_view(k)
+        part = gq.new_empty(lib.obst_rotary_part(gs[-1]), dtype=torch.float32)
+        wq, wk, wt = kernel_weights(wq, wk)
+        dt = DTYPES[(dwk if dwq is None else dwq).dtype]
+    L.launch(lib.obst_rotary_bwd, gq, "rotary_bwd", L.ROT_DESC.pack(
+        L.ptr(q), L.ptr(k), 0, gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), 0, L.ptr(wq), L.ptr(wk),
+        L.ptr(freqs), pos.data_ptr(), 0, L.ptr(part), L.ptr(dwq), L.ptr(dwk), q_ts, q_hs, k_ts,
+        k_hs, 0, 0, gq_ts, gq_hs, gk_ts, gk_hs, T, 0, gs[-2], gk.shape[-2], gs[-1], rot, inter, DTYPES[gq.dtype], wt, dt,
+        add, 0, mscale, eps))
 
 
 def wt_direct(ws) -> bool:
@@ -285,5 +294,5 @@ def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, freqs: typing.Op
     cfg = (rot, T, bool(interleaved), float(mscale), float(eps))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
-        return _Rotary.apply(q, k, q_weight, k_weight, pos, freqs, *cfg)
-    return _forward(q, k, pos, freqs, rot, T, q_weight, k_weight, *cfg[2:])
+        return _Rotary.apply(q, k, q_weight, k_weight, pos, freqs, cfg)
+    return _forward(q, k, pos, freqs, q_weight, k_weight, *cfg)

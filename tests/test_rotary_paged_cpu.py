@@ -110,6 +110,9 @@ def test_rotary_refusals():
             rotary.rotary(**{**ok, **bad})
     e = rotary.rotary(q[:0], k[:0], pos[:0], f)
     assert e[0].shape == (0, 2, 8)
+    qq = q.clone().requires_grad_()
+    with pytest.raises(L.KernelError):
+        torch.autograd.grad(rotary.rotary(qq, k, pos, f)[0].sum(), qq, create_graph=True)
     # no tokens: zero gradients
     z = q[:0].clone().requires_grad_()
     w = torch.ones(8, requires_grad=True)
