@@ -15,7 +15,7 @@
 // VEC = 1 takes what 16-byte accesses cannot (odd head widths, strides or addresses).
 //
 // Bound by memory: every element is read once and written once. At 32768 tokens of 2 x 16 heads x 128 in bf16, normed:
-// forward 89 us (537 MB, 6.0 TB/s), backward 164 us (805 MB, 4.9 TB/s) and 4 us for the weight sums.
+// forward 88 us (537 MB, 6.1 TB/s), backward 141 us (805 MB, 5.7 TB/s) and 4 us for the weight sums.
 #include <hip/hip_fp16.h>
 #include "common.h"
 
@@ -50,25 +50,28 @@ __device__ __forceinline__ void from_f(float f, float& o) { o = f; }
 __device__ __forceinline__ void from_f(float f, bf16_t& o) { o = f2bf(f); }
 __device__ __forceinline__ void from_f(float f, __half& o) { o = __float2half(f); }
 
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+
 template <typename E, int VEC>
 struct alignas(sizeof(E) * VEC < 16 ? sizeof(E) * VEC : 16) Chunk { E e[VEC]; };
 
-template <typename E, int VEC>
+template <bool LINES, typename E, int VEC>
 __device__ __forceinline__ void store(E* p, const float* f) {
   Chunk<E, VEC> c;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) from_f(f[i], c.e[i]);
-  *reinterpret_cast<Chunk<E, VEC>*>(p) = c;
+  if constexpr (LINES) __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, c), reinterpret_cast<u32x4_t*>(p));
+  else *reinterpret_cast<Chunk<E, VEC>*>(p) = c;
 }
 
-// A chunk that is read once: past the caches where a head's lanes together take whole 128-byte lines (bf16 x 128 normed
-// backward 165 -> 153 us); where they take parts, the caches hold the rest for the other half's load (fp32 x 96, half a
-// head 1.5 lines: 26 us, 30 past the caches)
+// LINES, in the normed backward: chunks go past the caches where a head's lanes together take whole 128-byte lines (bf16 x
+// 128: 165 -> 146 us for the loads, 141 with the stores). Where they take parts of lines, the caches hold the rest for the other
+// half's access (fp32 x 96, half a head 1.5 lines: 26 us, 30 past the caches). The forward, at 6 TB/s, gains nothing from
+// loads and loses 10 % with stores past the caches.
 template <bool LINES, typename E, int VEC>
 __device__ __forceinline__ Chunk<E, VEC> load_once(const E* p) {
   if constexpr (LINES) {
-    typedef __attribute__((ext_vector_type(4))) uint32_t u4;
-    return __builtin_bit_cast(Chunk<E, VEC>, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p)));
+    return __builtin_bit_cast(Chunk<E, VEC>, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p)));
   }
   return *reinterpret_cast<const Chunk<E, VEC>*>(p);
 }
@@ -371,8 +374,8 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
         read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
         read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
         turn<VEC, INSIDE>(a[it], b[it], c, s);
-        if (ln.ha[it]) store<E, VEC>(o + ln.ca[it], a[it]);
-        if (ln.hb[it]) store<E, VEC>(o + ln.cb[it], b[it]);
+        if (ln.ha[it]) store<false, E, VEC>(o + ln.ca[it], a[it]);
+        if (ln.hb[it]) store<false, E, VEC>(o + ln.cb[it], b[it]);
       }
     }
   }
@@ -484,8 +487,8 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
       E* o = isq ? (E*)d.qo + (t * d.Hq + h) * d.D : (E*)d.ko + (t * d.Hk + h) * d.D;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
-        if (ln.ha[it]) store<E, VEC>(o + ln.ca[it], a[it]);
-        if (ln.hb[it]) store<E, VEC>(o + ln.cb[it], b[it]);
+        if (ln.ha[it]) store<LINES, E, VEC>(o + ln.ca[it], a[it]);
+        if (ln.hb[it]) store<LINES, E, VEC>(o + ln.cb[it], b[it]);
       }
     }
   }
@@ -562,8 +565,8 @@ int pow2_at_least(int n) {
   return p;
 }
 
-// the backward's block count also sizes its partials
-constexpr int FWD_BLOCKS = 2048, BWD_BLOCKS = 1024;
+// four blocks a CU; the backward's count also sizes its partials
+constexpr int FWD_BLOCKS = 1024, BWD_BLOCKS = 1024;
 
 struct Passes {
   int hpw, pq, pk;
@@ -620,7 +623,7 @@ int backward_normed(const RotDesc& d, int lph, hipStream_t st) {
 
 // Passes a unit. Four share one token's angles and keep four rows of loads in flight; under 1024 tokens one each spreads
 // them over more waves. The normed backward takes one: a second pass' loads and the sums leave it three waves a SIMD
-// (199 us where one pass takes 164, at 32768 tokens, 2 x 16 heads x 128 in bf16).
+// (199 us where one pass took 164 at the time, 32768 tokens of 2 x 16 heads x 128 in bf16).
 template <int TYPE, int VEC, bool INSIDE>
 int by_tokens(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
   const bool few = d.T < 1024;
