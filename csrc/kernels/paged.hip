@@ -251,9 +251,10 @@ constexpr float NEG = -3.0e38f;                   // a running maximum before an
 template <int TYPE, int D>
 __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   typedef typename Mat<TYPE>::v vec;
-  constexpr int NK = D / 32, NV = D / 16;
-  __shared__ float sm[4][16], sl[4][16];
-  __shared__ float sacc[4][16][D + 4];
+  constexpr int NK = D / 32, NV = D / 16, NW = NTH / 64;
+  __shared__ float sm[NW][16], sl[NW][16];
+  extern __shared__ float sacc[];                 // [NW][query heads of the block][D + 4]: one head's 2 KB leave room for
+                                                  // four blocks a CU, space for 16 heads for three
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
   const int G = d.Hq / d.Hk, ng = (G + 15) / 16;
   const int hk = blockIdx.y / ng, gi = blockIdx.y % ng, b = blockIdx.z, sp = blockIdx.x;
@@ -287,7 +288,7 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
     iv = tb[min(t0 + rv, d.cap - 1) >> d.shift];
   };
   if (d.cap > 0) ids(k0 + 32 * w);
-  for (int t0 = k0 + 32 * w; t0 < k1; t0 += 128) {
+  for (int t0 = k0 + 32 * w; t0 < k1; t0 += 32 * NW) {
     const bool bad_v = (unsigned)iv >= (unsigned)d.P;
     const long long ja = (unsigned)ia < (unsigned)d.P ? ia : 0, jb = (unsigned)ib < (unsigned)d.P ? ib : 0, jv = bad_v ? 0 : iv;
     const uint16_t* pa = K + ja * pst + hoff + ((t0 + ra) & in_page) * D + 8 * g;
@@ -302,7 +303,7 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) v[j] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(pv + 128 * j));
-    ids(t0 + 128);
+    ids(t0 + 32 * NW);
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
       s0 = Mat<TYPE>::mul(a[j], q[j], s0);
@@ -358,19 +359,20 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   if (g == 0) { sm[w][n] = m; sl[w][n] = l; }
   if (n < gc) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[w][n][16 * j + 4 * g]) = acc[j];
+    for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[(w * gc + n) * (D + 4) + 16 * j + 4 * g]) = acc[j];
   }
   __syncthreads();
   const bool whole = len <= d.split;
   for (int e = threadIdx.x; e < gc * D; e += NTH) {
     const int h = e / D, i = e % D;
-    const float M = fmaxf(fmaxf(sm[0][h], sm[1][h]), fmaxf(sm[2][h], sm[3][h]));
-    float L = 0.f, o = 0.f;
+    float M = sm[0][h], L = 0.f, o = 0.f;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 1; x < NW; ++x) M = fmaxf(M, sm[x][h]);
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
       const float f = __builtin_amdgcn_exp2f(sm[x][h] - M);
       L += f * sl[x][h];
-      o += f * sacc[x][h][i];
+      o += f * sacc[(x * gc + h) * (D + 4) + i];
     }
     if (whole) {
       ((uint16_t*)d.o)[((long long)b * d.Hq + h0 + h) * D + i] = Mat<TYPE>::bits(L != 0.f ? o / L : 0.f);
@@ -434,16 +436,21 @@ __global__ __launch_bounds__(NTH) void paged_join_kernel(const PagedDesc d) {
   for (int i = 0; i < 4; ++i) out[i] = Mat<TYPE>::bits(L != 0.f ? o[i] / L : 0.f);
 }
 
+template <int TYPE, int D>
+void launch_attn(const PagedDesc& d, hipStream_t st) {
+  const int G = d.Hq / d.Hk, ng = (G + 15) / 16, gc = G < 16 ? G : 16;
+  hipLaunchKernelGGL((paged_attn_kernel<TYPE, D>), dim3(d.nsplit, d.Hk * ng, d.B), dim3(NTH),
+                     NTH / 64 * gc * (D + 4) * sizeof(float), st, d);
+}
+
 template <int TYPE>
 int attn(const PagedDesc& d, hipStream_t st) {
-  const int ng = (d.Hq / d.Hk + 15) / 16;
-  const dim3 grid(d.nsplit, d.Hk * ng, d.B), blk(NTH);
   switch (d.D) {
-    case 32: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 32>), grid, blk, 0, st, d); break;
-    case 64: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 64>), grid, blk, 0, st, d); break;
-    case 96: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 96>), grid, blk, 0, st, d); break;
-    case 128: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 128>), grid, blk, 0, st, d); break;
-    case 256: hipLaunchKernelGGL((paged_attn_kernel<TYPE, 256>), grid, blk, 0, st, d); break;
+    case 32: launch_attn<TYPE, 32>(d, st); break;
+    case 64: launch_attn<TYPE, 64>(d, st); break;
+    case 96: launch_attn<TYPE, 96>(d, st); break;
+    case 128: launch_attn<TYPE, 128>(d, st); break;
+    case 256: launch_attn<TYPE, 256>(d, st); break;
     default: return -2;
   }
   int rc = (int)hipGetLastError();

@@ -268,6 +268,7 @@ ATTN = [  # Hq, Hk, D, page, lens
     (17, 1, 32, 256, [1000]),
     (8, 4, 256, 64, [65, 320, 1]),
     (1, 1, 32, 16, [0, 0]),
+    (32, 2, 256, 32, [70, 0, 300]),          # the most shared memory a block takes: 16 heads of 256
     (4, 1, 128, 128, [20000]),               # many splits
 ]
 
