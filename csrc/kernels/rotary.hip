@@ -228,48 +228,43 @@ __device__ __forceinline__ float sum_lanes(float v, int lph) {
   return v;
 }
 
-// values into their columns of eight tokens: V cache [P][Hk][page / 8][D][8]. A wave takes one token and VCH pieces
-// of 64 * EV elements of its heads. Eight tokens of the step that fill one column block, slots 8 j .. 8 j + 7, are
-// written together by the first of them, 16 bytes (32) at a time; the others of the eight have nothing left to do.
-// Tokens outside such a run (a decode step's, a run's ragged ends) write their elements one by one.
+// Values into their columns of eight tokens: V cache [P][Hk][page / 8][D][8]. A wave takes a window of wt neighbouring
+// tokens (8, or 1 where there are few) and VCH pieces of 64 * EV elements of their heads. Eight tokens of the step that
+// fill one column block, slots 8 j .. 8 j + 7, are written together, 16 bytes at a time, by the window that holds the first
+// of them. Tokens outside such a run (a decode step's, a run's ragged ends) write their elements one by one.
+// (A window a token, with the other seven of a run idle, left all of a prompt's work to every eighth block, which is
+// one of the eight dies: 127 us where windows of eight take 46, 5.9 TB/s, at 16384 tokens of 16 heads x 128.)
 constexpr int VCH = 4;
 
 template <typename E, int EV>
-__device__ void append_values(const RotDesc& d, long long unit, int nvg) {
-  const int lane = threadIdx.x & 63;
-  const long long t = unit / nvg;
-  const long long slot = d.slots[t];
-  if (slot < 0 || slot >= d.nslots) return;
-  const int off = (int)(slot % 8);
-  const long long t0 = t - off;
-  bool mine = true;
-  if (lane < 8) mine = t0 + lane >= 0 && t0 + lane < d.T && d.slots[max(0LL, min(t0 + lane, d.T - 1))] == slot - off + lane;
-  const bool run = __all(mine);
-  if (run && off != 0) return;
+__device__ __forceinline__ void append_run(const RotDesc& d, long long t, long long slot, int e0) {
   const long long page = slot / d.page;
-  const int o8 = (int)(slot % d.page) / 8;
+  const int o8 = (int)(slot % d.page) / 8, n = d.Hk * d.D;
   const E* v = (const E*)d.v + t * d.v_ts;
-  const int n = d.Hk * d.D, e0 = (int)(unit % nvg) * VCH * 64 * EV + lane * EV;
-  if (run) {
 #pragma unroll
-    for (int i = 0; i < VCH; ++i) {
-      const int e = e0 + i * 64 * EV;
-      if (e >= n) return;
-      const int h = e / d.D, c = e % d.D;
-      Chunk<E, EV> x[8];
+  for (int i = 0; i < VCH; ++i) {
+    const int e = e0 + i * 64 * EV;
+    if (e >= n) return;
+    const int h = e / d.D, c = e % d.D;
+    Chunk<E, EV> x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const Chunk<E, EV>*>(v + j * d.v_ts + h * d.v_hs + c);
-      E* o = (E*)d.vo + (((page * d.Hk + h) * (d.page / 8) + o8) * d.D + c) * 8;
+    for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const Chunk<E, EV>*>(v + j * d.v_ts + h * d.v_hs + c);
+    E* o = (E*)d.vo + (((page * d.Hk + h) * (d.page / 8) + o8) * d.D + c) * 8;
 #pragma unroll
-      for (int k = 0; k < EV; ++k) {
-        Chunk<E, 8> y;
+    for (int k = 0; k < EV; ++k) {
+      Chunk<E, 8> y;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y.e[j] = x[j].e[k];
-        *reinterpret_cast<Chunk<E, 8>*>(o + 8 * k) = y;
-      }
+      for (int j = 0; j < 8; ++j) y.e[j] = x[j].e[k];
+      *reinterpret_cast<Chunk<E, 8>*>(o + 8 * k) = y;
     }
-    return;
   }
+}
+
+template <typename E, int EV>
+__device__ __forceinline__ void append_one(const RotDesc& d, long long t, long long slot, int e0) {
+  const long long page = slot / d.page;
+  const int off = (int)(slot % 8), o8 = (int)(slot % d.page) / 8, n = d.Hk * d.D;
+  const E* v = (const E*)d.v + t * d.v_ts;
   Chunk<E, EV> x[VCH];
 #pragma unroll
   for (int i = 0; i < VCH; ++i) {
@@ -286,16 +281,36 @@ __device__ void append_values(const RotDesc& d, long long unit, int nvg) {
   }
 }
 
+template <typename E, int EV>
+__device__ __forceinline__ void append_values(const RotDesc& d, long long unit, int nvg, int wt) {
+  const int lane = threadIdx.x & 63, e0 = (int)(unit % nvg) * VCH * 64 * EV + lane * EV;
+  const long long t0 = unit / nvg * wt;
+  // lane i holds the slot of token t0 - 7 + i, -2 where there is none
+  const long long at = t0 - 7 + lane;
+  const int raw = d.slots[min(max(at, 0LL), d.T - 1)];
+  const int slot = at >= 0 && at < d.T && raw >= 0 && raw < d.nslots ? raw : -2;
+  // bit i: the token of lane i follows its neighbour's slot; it is the first of a whole run
+  const unsigned long long next = __ballot(slot >= 0 && slot == __shfl_up(slot, 1, 64) + 1 && lane > 0);
+  const unsigned long long first = __ballot(slot >= 0 && slot % 8 == 0 && lane < 15 && (next >> (lane + 1) & 0x7f) == 0x7f);
+  for (int i = 7; i < 7 + wt; ++i) {
+    const int s = __builtin_amdgcn_readlane(slot, i);
+    if (s < 0) continue;
+    if (first >> i & 1) append_run<E, EV>(d, t0 - 7 + i, s, e0);
+    else if ((first >> (i - 7) & 0xff) == 0) append_one<E, EV>(d, t0 - 7 + i, s, e0);   // in no run
+  }
+}
+
 // ---- forward. A wave's unit is U passes of one token; a pass is 64 / lph heads, all of q or all of k. CACHE: k goes
 // into the pages, and the blocks behind the first `rot` write the values.
 template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool CACHE, int EV>
-__global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int lph, int pq, int pk, int rot, int nvg) {
+__global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int lph, int pq, int pk, int rot, int nvg, int wt) {
   typedef typename Elem<TYPE>::t E;
   __shared__ Staged sh;
   if (CACHE && (int)blockIdx.x >= rot) {
-    const long long units = d.T * nvg, nw = (long long)(gridDim.x - rot) * (NTH / 64);
-    for (long long u = (long long)(blockIdx.x - rot) * (NTH / 64) + (threadIdx.x >> 6); u < units; u += nw)
-      append_values<E, EV>(d, u, nvg);
+    const long long units = (d.T + wt - 1) / wt * nvg, nw = (long long)(gridDim.x - rot) * (NTH / 64);
+    for (long long u = (long long)(blockIdx.x - rot) * (NTH / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+         u < units; u += nw)
+      append_values<E, EV>(d, u, nvg, wt);
     return;
   }
   const int lane = threadIdx.x & 63, hl = lane / lph, il = lane % lph, hpw = 64 / lph;
@@ -583,13 +598,14 @@ int forward(const RotDesc& d, int lph, hipStream_t st) {
   const int grid = Passes::blocks(d.T * ((p.pq + p.pk + U - 1) / U), FWD_BLOCKS);
   if (!d.slots) {
     hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false, 1>), dim3(grid), dim3(NTH), 0, st, d, lph,
-                       p.pq, p.pk, grid, 0);
+                       p.pq, p.pk, grid, 0, 0);
     return (int)hipGetLastError();
   }
   constexpr int EV = VEC == 1 ? 1 : 2;                     // VEC > 1: D and the strides are even
-  const int nvg = (d.Hk * d.D + VCH * 64 * EV - 1) / (VCH * 64 * EV), vgrid = Passes::blocks(d.T * nvg, FWD_BLOCKS);
+  const int nvg = (d.Hk * d.D + VCH * 64 * EV - 1) / (VCH * 64 * EV), wt = d.T < 1024 ? 1 : 8;
+  const int vgrid = Passes::blocks((d.T + wt - 1) / wt * nvg, FWD_BLOCKS);
   hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, true, EV>), dim3(grid + vgrid), dim3(NTH), 0, st, d,
-                     lph, p.pq, p.pk, grid, nvg);
+                     lph, p.pq, p.pk, grid, nvg, wt);
   return (int)hipGetLastError();
 }
 

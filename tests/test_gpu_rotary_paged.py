@@ -217,7 +217,7 @@ def test_release(cuda):
     (2, 2, 128, 128, 16, False, True), (8, 1, 64, 32, 32, True, False), (3, 3, 96, 96, 64, False, True),
     (20, 4, 256, 256, 128, True, True), (2, 1, 32, 0, 256, False, False), (1, 1, 33, 8, 16, False, True),
     (32, 8, 128, 64, 64, True, False), (4, 2, 512, 512, 16, False, True)])
-@pytest.mark.parametrize("T", [1, 37, 300])
+@pytest.mark.parametrize("T", [1, 37, 300, 1500])
 def test_append(cuda, T, Hq, Hk, D, rot, page, inter, norm, dtype):
     g = gen(cuda, T + D)
     rnd = lambda *s: torch.randn(*s, device=cuda, generator=g).to(dtype)  # noqa: E731
