@@ -183,26 +183,28 @@ __device__ __forceinline__ void stage(const RotDesc& d, Staged& s) {
   __syncthreads();
 }
 
-// cos and sin of a token's angles, a pair a lane, through shared memory for all of the wave's heads (each lane forming
-// those of its own pairs, eight times over in a wave of eight heads, took half of the forward's instructions). The angle is
-// reduced in 64 bits to a quarter turn r in [-1/2, 1/2] and its quadrant; there the Taylor polynomials of sin and
-// cos(pi r / 2) to the 9th and 10th power are off by less than 2^-28
+// cos and sin of pos * f turns, times m and (sin) sign. The angle is reduced in 64 bits to a quarter turn r in [-1/2, 1/2] and
+// its quadrant; there the Taylor polynomials of sin and cos(pi r / 2) to the 9th and 10th power are off by less than 2^-28
+__device__ __forceinline__ void turn_of(double pos, double f, float m, float sign, float& c, float& s) {
+  double t = pos * f;
+  t = 4.0 * (t - rint(t));
+  const double k = rint(t);
+  const float r = (float)(t - k), r2 = r * r;
+  const int q = (int)k;
+  const float sn = r * (1.5707963267948966f + r2 * (-0.6459640975062462f + r2 * (0.07969262624616704f +
+                   r2 * (-0.004681754135318688f + r2 * 0.00016044118478735982f))));
+  const float cs = 1.f + r2 * (-1.2337005501361697f + r2 * (0.2536695079010480f + r2 * (-0.02086348076335296f +
+                   r2 * (0.0009192602748394266f + r2 * -2.5202042373060605e-05f))));
+  const float u = q & 1 ? cs : sn, v = q & 1 ? sn : cs;
+  c = m * (q + 1 & 2 ? -v : v);
+  s = m * sign * (q & 2 ? -u : u);
+}
+
+// those of a token, a pair a lane, through shared memory for all of the wave's heads (each lane forming those of its own
+// pairs, eight times over in a wave of eight heads, took half of the forward's instructions)
 __device__ __forceinline__ void turn_angles(const RotDesc& d, Staged& sh, int w, double pos, float sign) {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the wave's reads of its last token's are done
-  for (int i = threadIdx.x & 63; i < d.R / 2; i += 64) {
-    double t = pos * sh.f[i];
-    t = 4.0 * (t - rint(t));
-    const double k = rint(t);
-    const float r = (float)(t - k), r2 = r * r;
-    const int q = (int)k;
-    const float sn = r * (1.5707963267948966f + r2 * (-0.6459640975062462f + r2 * (0.07969262624616704f +
-                     r2 * (-0.004681754135318688f + r2 * 0.00016044118478735982f))));
-    const float cs = 1.f + r2 * (-1.2337005501361697f + r2 * (0.2536695079010480f + r2 * (-0.02086348076335296f +
-                     r2 * (0.0009192602748394266f + r2 * -2.5202042373060605e-05f))));
-    const float u = q & 1 ? cs : sn, v = q & 1 ? sn : cs;
-    sh.c[w][i] = d.mscale * (q + 1 & 2 ? -v : v);
-    sh.s[w][i] = d.mscale * sign * (q & 2 ? -u : u);
-  }
+  for (int i = threadIdx.x & 63; i < d.R / 2; i += 64) turn_of(pos, sh.f[i], d.mscale, sign, sh.c[w][i], sh.s[w][i]);
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
@@ -226,6 +228,37 @@ __device__ __forceinline__ float sum_lanes(float v, int lph) {
   if (lph > 16) v += __shfl_xor(v, 16, 64);
   if (lph > 32) v += __shfl_xor(v, 32, 64);
   return v;
+}
+
+// those of one lane's pairs, for rows of several tokens in a wave
+template <int VEC, bool INSIDE>
+__device__ __forceinline__ void own_angles(const double* f, int fa, int fb, double pos, float m, float sign, float* c,
+                                           float* s) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const int p = INSIDE && i >= VEC / 2 ? fb : fa, j = INSIDE && i >= VEC / 2 ? i - VEC / 2 : i;
+    turn_of(pos, f[p < NOTURN ? p + j : 0], m, sign, c[i], s[i]);
+    c[i] = p < NOTURN ? c[i] : 1.f;
+    s[i] = p < NOTURN ? s[i] : 0.f;
+  }
+}
+
+// Which row a lane has in a pass. Passes run over the heads of q, then of k: of one token, or (ROWS) over all (token, head)
+// pairs of the call, where a token's heads leave most of a wave's lanes without one.
+struct Row {
+  long long t;
+  int h;
+  bool on;
+};
+
+template <bool ROWS>
+__device__ __forceinline__ Row row_of(const RotDesc& d, long long t, int p, int hl, int hpw, int H) {
+  if (!ROWS) {
+    const int h = p * hpw + hl;
+    return {t, min(h, H - 1), h < H};
+  }
+  const unsigned n = (unsigned)d.T * H, r = (unsigned)p * hpw + hl, c = min(r, n - 1);    // T H < 2^31
+  return {c / H, (int)(c % H), r < n};
 }
 
 // Values into their columns of eight tokens: V cache [P][Hk][page / 8][D][8]. A wave takes a window of wt neighbouring
@@ -300,9 +333,9 @@ __device__ __forceinline__ void append_values(const RotDesc& d, long long unit, 
   }
 }
 
-// ---- forward. A wave's unit is U passes of one token; a pass is 64 / lph heads, all of q or all of k. CACHE: k goes
-// into the pages, and the blocks behind the first `rot` write the values.
-template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool CACHE, int EV>
+// ---- forward. A wave's unit is U passes, of one token or (ROWS) of the call; a pass is 64 / lph heads, all of q or all of k.
+// CACHE: k goes into the pages, and the blocks behind the first `rot` write the values.
+template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool ROWS, bool CACHE, int EV>
 __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int lph, int pq, int pk, int rot, int nvg, int wt) {
   typedef typename Elem<TYPE>::t E;
   __shared__ Staged sh;
@@ -319,34 +352,36 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
   const Lane<VEC, ITEMS, INSIDE> ln(d, il, lph);
   stage(d, sh);
   const float inv_d = 1.f / d.D;
-  const long long units = d.T * npg, nw = (long long)rot * (NTH / 64);
+  const long long units = ROWS ? npg : d.T * npg, nw = (long long)rot * (NTH / 64);
   for (long long u = (long long)blockIdx.x * (NTH / 64) + wave; u < units; u += nw) {
-    const long long t = u / npg;
-    const int p0 = (int)(u % npg) * U;
+    const long long t = ROWS ? 0 : u / npg;
+    const int p0 = (int)(ROWS ? u : u % npg) * U;
     Chunk<E, VEC> xa[U][ITEMS], xb[U][ITEMS];
+    Row row[U];
 #pragma unroll
     for (int p = 0; p < U; ++p) {
       if (p0 + p >= np) break;
       const bool isq = p0 + p < pq;
-      const int H = isq ? d.Hq : d.Hk, h = min((p0 + p - (isq ? 0 : pq)) * hpw + hl, H - 1);
-      const E* x = isq ? (const E*)d.q + t * d.q_ts + h * d.q_hs : (const E*)d.k + t * d.k_ts + h * d.k_hs;
+      row[p] = row_of<ROWS>(d, t, p0 + p - (isq ? 0 : pq), hl, hpw, isq ? d.Hq : d.Hk);
+      const long long rt = row[p].t;
+      const int h = row[p].h;
+      const E* x = isq ? (const E*)d.q + rt * d.q_ts + h * d.q_hs : (const E*)d.k + rt * d.k_ts + h * d.k_hs;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
         xa[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.ca[it]);
         xb[p][it] = *reinterpret_cast<const Chunk<E, VEC>*>(x + ln.cb[it]);
       }
     }
-    const double pos = CACHE && !d.pos ? 0.0 : (double)d.pos[t];
-    const long long slot = CACHE ? d.slots[t] : 0;
-    const bool live = !CACHE || (slot >= 0 && slot < d.nslots);
-    const long long page = CACHE ? slot / d.page : 0;
-    const int off = CACHE ? (int)(slot % d.page) : 0;
-    turn_angles(d, sh, wave, pos, 1.f);
+    const bool still = CACHE && !d.pos;                // nothing turns
+    if (!ROWS) turn_angles(d, sh, wave, still ? 0.0 : (double)d.pos[t], 1.f);
 #pragma unroll
     for (int p = 0; p < U; ++p) {
       if (p0 + p >= np) break;
       const bool isq = p0 + p < pq;
-      const int H = isq ? d.Hq : d.Hk, h = (p0 + p - (isq ? 0 : pq)) * hpw + hl;
+      const long long rt = row[p].t;
+      const int h = row[p].h;
+      const long long slot = CACHE && !isq ? d.slots[rt] : 0;
+      const double pos = ROWS && !still ? (double)d.pos[rt] : 0.0;
       float a[ITEMS][VEC], b[ITEMS][VEC];
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it)
@@ -377,17 +412,21 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
             b[it][i] *= r * w[ln.cb[it] + i];
           }
       }
-      if (h >= H || (!isq && !live)) continue;
+      if (!row[p].on || slot < 0 || (CACHE && slot >= d.nslots)) continue;
       E* o;
-      if (isq) o = (E*)d.qo + (t * d.Hq + h) * d.D;
-      else if (CACHE) o = (E*)d.ko + ((page * d.Hk + h) * d.page + off) * d.D;
-      else o = (E*)d.ko + (t * d.Hk + h) * d.D;
+      if (isq) o = (E*)d.qo + (rt * d.Hq + h) * d.D;
+      else if (CACHE) o = (E*)d.ko + ((slot / d.page * d.Hk + h) * d.page + slot % d.page) * d.D;
+      else o = (E*)d.ko + (rt * d.Hk + h) * d.D;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
         float c[VEC], s[VEC];
         const int z = here();
-        read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
-        read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
+        if (ROWS) {
+          own_angles<VEC, INSIDE>(sh.f + z, ln.fa[it], ln.fb[it], pos, d.mscale, 1.f, c, s);
+        } else {
+          read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
+          read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
+        }
         turn<VEC, INSIDE>(a[it], b[it], c, s);
         if (ln.ha[it]) store<false, E, VEC>(o + ln.ca[it], a[it]);
         if (ln.hb[it]) store<false, E, VEC>(o + ln.cb[it], b[it]);
@@ -401,7 +440,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
 // lanes and waves in a fixed order into part[block], rotary_fold_kernel the blocks: no atomics, the same bits each run.
 // With sums to keep, a block works on one tensor (the first nbq on q): sums for both took 16 more registers a lane and
 // spilled.
-template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool NORM, bool LINES>
+template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool ROWS, bool NORM, bool LINES>
 __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int lph, int pq, int pk, int nbq) {
   typedef typename Elem<TYPE>::t E;
   __shared__ Staged sh;
@@ -418,18 +457,21 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
       for (int i = 0; i < VEC; ++i) da[it][i] = db[it][i] = 0.f;
   const float inv_d = 1.f / d.D;
   const int b0 = NORM && !block_q ? nbq : 0, nb = !NORM ? gridDim.x : block_q ? nbq : gridDim.x - nbq;
-  const long long units = d.T * npg, nw = (long long)nb * (NTH / 64);
+  const long long units = ROWS ? npg : d.T * npg, nw = (long long)nb * (NTH / 64);
   for (long long u = (long long)(blockIdx.x - b0) * (NTH / 64) + wave; u < units; u += nw) {
-    const long long t = u / npg;
-    const int p0 = (int)(u % npg) * U;
+    const long long t = ROWS ? 0 : u / npg;
+    const int p0 = (int)(ROWS ? u : u % npg) * U;
+    Row row[U];
     Chunk<E, VEC> ga[U][ITEMS], gb[U][ITEMS], xa[U][ITEMS], xb[U][ITEMS];
 #pragma unroll
     for (int p = 0; p < U; ++p) {
       if (p0 + p >= np) break;
       const bool isq = NORM ? block_q : p0 + p < pq;
-      const int H = isq ? d.Hq : d.Hk, h = min((pb + p0 + p - (isq ? 0 : pq)) * hpw + hl, H - 1);
-      const E* g = isq ? (const E*)d.gq + t * d.gq_ts + h * d.gq_hs : (const E*)d.gk + t * d.gk_ts + h * d.gk_hs;
-      const E* x = isq ? (const E*)d.q + t * d.q_ts + h * d.q_hs : (const E*)d.k + t * d.k_ts + h * d.k_hs;
+      row[p] = row_of<ROWS>(d, t, pb + p0 + p - (isq ? 0 : pq), hl, hpw, isq ? d.Hq : d.Hk);
+      const long long rt = row[p].t;
+      const int h = row[p].h;
+      const E* g = isq ? (const E*)d.gq + rt * d.gq_ts + h * d.gq_hs : (const E*)d.gk + rt * d.gk_ts + h * d.gk_hs;
+      const E* x = isq ? (const E*)d.q + rt * d.q_ts + h * d.q_hs : (const E*)d.k + rt * d.k_ts + h * d.k_hs;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
         ga[p][it] = load_once<LINES, E, VEC>(g + ln.ca[it]);
@@ -440,13 +482,14 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
         }
       }
     }
-    const double pos = (double)d.pos[t];
-    turn_angles(d, sh, wave, pos, -1.f);
+    if (!ROWS) turn_angles(d, sh, wave, (double)d.pos[t], -1.f);
 #pragma unroll
     for (int p = 0; p < U; ++p) {
       if (p0 + p >= np) break;
       const bool isq = NORM ? block_q : p0 + p < pq;
-      const int H = isq ? d.Hq : d.Hk, h = (pb + p0 + p - (isq ? 0 : pq)) * hpw + hl;
+      const long long rt = row[p].t;
+      const int h = row[p].h;
+      const double pos = ROWS ? (double)d.pos[rt] : 0.0;
       float a[ITEMS][VEC], b[ITEMS][VEC];
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
@@ -457,8 +500,12 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
         }
         float c[VEC], s[VEC];
         const int z = here();
-        read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
-        read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
+        if (ROWS) {
+          own_angles<VEC, INSIDE>(sh.f + z, ln.fa[it], ln.fb[it], pos, d.mscale, -1.f, c, s);
+        } else {
+          read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
+          read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
+        }
         turn<VEC, INSIDE>(a[it], b[it], c, s);
       }
       if (NORM && (isq ? d.wq != nullptr : d.wk != nullptr)) {
@@ -482,7 +529,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
         ss = sum_lanes(ss, lph);
         e = sum_lanes(e, lph);
         // lanes past the last head repeat it for their loads: nothing of theirs may reach the weight sums
-        const float r = rsqrtf(ss * inv_d + d.eps), rw = h < H ? r : 0.f, k = e * inv_d * r * r * r;
+        const float r = rsqrtf(ss * inv_d + d.eps), rw = row[p].on ? r : 0.f, k = e * inv_d * r * r * r;
         w = sh.w[isq ? 0 : 1] + here();
 #pragma unroll
         for (int it = 0; it < ITEMS; ++it) {
@@ -498,8 +545,8 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
           }
         }
       }
-      if (h >= H) continue;
-      E* o = isq ? (E*)d.qo + (t * d.Hq + h) * d.D : (E*)d.ko + (t * d.Hk + h) * d.D;
+      if (!row[p].on) continue;
+      E* o = isq ? (E*)d.qo + (rt * d.Hq + h) * d.D : (E*)d.ko + (rt * d.Hk + h) * d.D;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
         if (ln.ha[it]) store<LINES, E, VEC>(o + ln.ca[it], a[it]);
@@ -583,53 +630,57 @@ int pow2_at_least(int n) {
 // four blocks a CU; the backward's count also sizes its partials
 constexpr int FWD_BLOCKS = 1024, BWD_BLOCKS = 1024;
 
+// passes of a token, or (ROWS) of the call
+template <bool ROWS>
 struct Passes {
-  int hpw, pq, pk;
-  Passes(const RotDesc& d, int lph) : hpw(64 / lph), pq((d.Hq + hpw - 1) / hpw), pk((d.Hk + hpw - 1) / hpw) {}
+  int pq, pk;
+  Passes(const RotDesc& d, int lph) : pq(of(d, d.Hq, 64 / lph)), pk(of(d, d.Hk, 64 / lph)) {}
+  static int of(const RotDesc& d, int H, int hpw) { return (int)(((ROWS ? d.T * H : H) + hpw - 1) / hpw); }
+  long long units(const RotDesc& d, int U) const { return (ROWS ? 1 : d.T) * ((pq + pk + U - 1) / U); }
   static int blocks(long long units, int most) {
     const long long b = (units + 3) / 4;
     return (int)(b < most ? b : most);
   }
 };
 
-template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE>
+template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool ROWS>
 int forward(const RotDesc& d, int lph, hipStream_t st) {
-  const Passes p(d, lph);
-  const int grid = Passes::blocks(d.T * ((p.pq + p.pk + U - 1) / U), FWD_BLOCKS);
+  const Passes<ROWS> p(d, lph);
+  const int grid = p.blocks(p.units(d, U), FWD_BLOCKS);
   if (!d.slots) {
-    hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false, 1>), dim3(grid), dim3(NTH), 0, st, d, lph,
+    hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, false, 1>), dim3(grid), dim3(NTH), 0, st, d, lph,
                        p.pq, p.pk, grid, 0, 0);
     return (int)hipGetLastError();
   }
   constexpr int EV = VEC == 1 ? 1 : 2;                     // VEC > 1: D and the strides are even
   const int nvg = (d.Hk * d.D + VCH * 64 * EV - 1) / (VCH * 64 * EV), wt = d.T < 1024 ? 1 : 8;
-  const int vgrid = Passes::blocks((d.T + wt - 1) / wt * nvg, FWD_BLOCKS);
-  hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, true, EV>), dim3(grid + vgrid), dim3(NTH), 0, st, d,
+  const int vgrid = p.blocks((d.T + wt - 1) / wt * nvg, FWD_BLOCKS);
+  hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, true, EV>), dim3(grid + vgrid), dim3(NTH), 0, st, d,
                      lph, p.pq, p.pk, grid, nvg, wt);
   return (int)hipGetLastError();
 }
 
-template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE>
+template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool ROWS>
 int backward(const RotDesc& d, int lph, hipStream_t st) {
-  const Passes p(d, lph);
-  const int grid = Passes::blocks(d.T * ((p.pq + p.pk + U - 1) / U), BWD_BLOCKS);
-  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, false, false>), dim3(grid), dim3(NTH), 0, st, d, lph, p.pq,
+  const Passes<ROWS> p(d, lph);
+  const int grid = p.blocks(p.units(d, U), BWD_BLOCKS);
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, false, false>), dim3(grid), dim3(NTH), 0, st, d, lph, p.pq,
                      p.pk, 0);
   return (int)hipGetLastError();
 }
 
-template <int TYPE, int VEC, int ITEMS, bool INSIDE, bool LINES>
+template <int TYPE, int VEC, int ITEMS, bool INSIDE, bool ROWS, bool LINES>
 int backward_normed(const RotDesc& d, int lph, hipStream_t st) {
-  const Passes p(d, lph);
+  const Passes<ROWS> p(d, lph);
   // blocks for q and for k, as many as their units ask for
-  const long long bq = (d.T * p.pq + 3) / 4, bk = (d.T * p.pk + 3) / 4;
+  const long long n = ROWS ? 1 : d.T, bq = (n * p.pq + 3) / 4, bk = (n * p.pk + 3) / 4;
   int nq = (int)bq, nk = (int)bk;
   if (bq + bk > BWD_BLOCKS) {
-    nq = BWD_BLOCKS * p.pq / (p.pq + p.pk);
+    nq = (int)((long long)BWD_BLOCKS * p.pq / (p.pq + p.pk));
     nq = nq < 1 ? 1 : nq > BWD_BLOCKS - 1 ? BWD_BLOCKS - 1 : nq;
     nk = BWD_BLOCKS - nq;
   }
-  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, 1, INSIDE, true, LINES>), dim3(nq + nk), dim3(NTH), 0, st, d, lph, p.pq,
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, 1, INSIDE, ROWS, true, LINES>), dim3(nq + nk), dim3(NTH), 0, st, d, lph, p.pq,
                      p.pk, nq);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
@@ -637,23 +688,25 @@ int backward_normed(const RotDesc& d, int lph, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// Passes a unit. Four share one token's angles and keep four rows of loads in flight; under 1024 tokens one each spreads
-// them over more waves. The normed backward takes one: a second pass' loads and the sums leave it three waves a SIMD
+// Passes a unit. Four share one token's angles and keep four rows of loads in flight (two where the rows are several tokens':
+// registers); under 1024 tokens one each spreads them over more waves. The normed backward takes one: a second pass' loads and the sums leave it three waves a SIMD
 // (199 us where one pass took 164 at the time, 32768 tokens of 2 x 16 heads x 128 in bf16).
-template <int TYPE, int VEC, bool INSIDE>
+template <int TYPE, int VEC, bool INSIDE, bool ROWS>
 int by_tokens(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
+  constexpr int MANY = ROWS ? 2 : 4;
   const bool few = d.T < 1024;
-  if (!bwd) return few ? forward<TYPE, VEC, 1, 1, INSIDE>(d, lph, st) : forward<TYPE, VEC, 1, 4, INSIDE>(d, lph, st);
+  if (!bwd)
+    return few ? forward<TYPE, VEC, 1, 1, INSIDE, ROWS>(d, lph, st) : forward<TYPE, VEC, 1, MANY, INSIDE, ROWS>(d, lph, st);
   if (d.wq || d.wk)
-    return items_of(d, VEC) * 16 % 128 == 0 ? backward_normed<TYPE, VEC, 1, INSIDE, true>(d, lph, st)
-                                            : backward_normed<TYPE, VEC, 1, INSIDE, false>(d, lph, st);
-  return few ? backward<TYPE, VEC, 1, 1, INSIDE>(d, lph, st) : backward<TYPE, VEC, 1, 4, INSIDE>(d, lph, st);
+    return items_of(d, VEC) * 16 % 128 == 0 ? backward_normed<TYPE, VEC, 1, INSIDE, ROWS, true>(d, lph, st)
+                                            : backward_normed<TYPE, VEC, 1, INSIDE, ROWS, false>(d, lph, st);
+  return few ? backward<TYPE, VEC, 1, 1, INSIDE, ROWS>(d, lph, st) : backward<TYPE, VEC, 1, MANY, INSIDE, ROWS>(d, lph, st);
 }
 
 template <int TYPE, int ITEMS>
 int by_element(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
-  if (!bwd) return forward<TYPE, 1, ITEMS, 1, false>(d, lph, st);
-  return d.wq || d.wk ? backward_normed<TYPE, 1, ITEMS, false, false>(d, lph, st) : backward<TYPE, 1, ITEMS, 1, false>(d, lph, st);
+  if (!bwd) return forward<TYPE, 1, ITEMS, 1, false, false>(d, lph, st);
+  return d.wq || d.wk ? backward_normed<TYPE, 1, ITEMS, false, false, false>(d, lph, st) : backward<TYPE, 1, ITEMS, 1, false, false>(d, lph, st);
 }
 
 template <int TYPE>
@@ -661,7 +714,13 @@ int dispatch(const RotDesc& d, bool bwd, hipStream_t st) {
   constexpr int V = Elem<TYPE>::VEC;
   if (vec_ok(d, V, bwd)) {
     const int lph = pow2_at_least(items_of(d, V));
-    return d.inter ? by_tokens<TYPE, V, true>(d, bwd, lph, st) : by_tokens<TYPE, V, false>(d, bwd, lph, st);
+    // Rows of several tokens in a wave where one token's heads fill at most half of it. 65536 tokens normed in bf16, forward +
+    // backward, rows against tokens: 1 + 1 heads x 32 17 + 19 against 52 + 99 us, 8 + 8 x 32 34 + 56 against 53 + 101; at 12 +
+    // 12 x 64 (three quarters of a wave), 32768 tokens, 48 + 76 against 40 + 68
+    const int most = d.Hq > d.Hk ? d.Hq : d.Hk;
+    if (most * lph <= 32 && d.T * most < 1LL << 31)
+      return d.inter ? by_tokens<TYPE, V, true, true>(d, bwd, lph, st) : by_tokens<TYPE, V, false, true>(d, bwd, lph, st);
+    return d.inter ? by_tokens<TYPE, V, true, false>(d, bwd, lph, st) : by_tokens<TYPE, V, false, false>(d, bwd, lph, st);
   }
   const int n = items_of(d, 1);
   return n <= 64 ? by_element<TYPE, 1>(d, bwd, pow2_at_least(n), st) : by_element<TYPE, 4>(d, bwd, 64, st);
