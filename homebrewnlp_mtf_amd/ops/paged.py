@@ -324,7 +324,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
         if q_ds != 1 or (q_bs | q_hs) % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
             q_bs, q_hs = Hq * D, D
-        nsplit, split = _splits(B * rows, cap)
+        nsplit, split = _splits(B, B * rows, cap)
         part = q.new_empty(B * Hq * nsplit * (D + 2), dtype=torch.float32) if nsplit > 1 else None
         L.launch(L.lib().obst_paged_attn, q, "paged_attn", L.PAGED_DESC.pack(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
@@ -349,12 +349,16 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     return out
 
 
-def _splits(rows: int, cap: int) -> typing.Tuple[int, int]:
-    """(splits, tokens a split) of the length for ``rows`` blocks without one. Two blocks a CU fill the card: 4 rows of 131072
-    tokens took 44 us + 5 to join in 512 blocks, 47 + 6.5 in 1024, 50 + 9.5 in 2048. At most 2048 tokens a split, so
-    that one long request among short ones is spread as well, and at least 256; at most 1024 splits (csrc/kernels/paged.hip
-    MAX_SPLITS)"""
-    want = max(1, -(-512 // rows))
-    split = max(min(max(256, -(-cap // want)), 2048), -(-cap // 1024))
+def _splits(B: int, rows: int, cap: int) -> typing.Tuple[int, int]:
+    """(splits, tokens a split) of the length for ``rows`` blocks of ``B`` requests without one.
+
+    Up to 8 requests: two blocks a CU, at least 256 tokens each (one request's 4 rows of 131072 tokens take 44 us + 5 to join in
+    512 blocks, 47 + 6.5 in 1024, 50 + 9.5 in 2048). More requests differ in length and leave about half of the splits
+    empty: four blocks a CU, at least 384 tokens each (40 requests of 1 to 4000 tokens, 2 key heads: 24 us, 31 in two; 200 of
+    1 to 2000, 1 head: 28, 35). At most 2048 tokens a split, so that one long request among short ones is spread as well; at most
+    1024 splits (csrc/kernels/paged.hip MAX_SPLITS)."""
+    blocks, least = (512, 256) if B <= 8 else (1024, 384)
+    want = max(1, -(-blocks // rows))
+    split = max(min(max(least, -(-cap // want)), 2048), -(-cap // 1024))
     split = -(-split // 128) * 128
     return max(1, -(-cap // split)), split

@@ -414,3 +414,11 @@ def test_trainer_steps_with_rotary_attention():
                 buf[sp.offset + i] -= d
         # central difference: third derivatives times 1e-4 / 6, and two fp32 losses (~4, half a step 2.4e-7) over 2e-2
         assert abs((vals[0] - vals[1]) / 2e-2 - float(grad[i])) < 1e-4 + 0.02 * abs(float(grad[i]))
+
+
+def test_splits_cover_every_length():
+    for B in (1, 3, 8, 9, 200, 60000):
+        for heads in (1, 4, 20, 64):
+            for cap in (0, 1, 16, 255, 256, 257, 2048, 4097, 131072, 2 ** 21 + 1, 2 ** 30):
+                n, split = paged._splits(B, B * heads, cap)
+                assert 1 <= n <= 1024 and split % 128 == 0 and (n - 1) * split < max(cap, 1) <= n * split
