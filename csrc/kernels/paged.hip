@@ -37,7 +37,7 @@ constexpr int NTH = 256;
 // before it) - i. Sums over the requests before b are all that a group needs, so every block forms them itself from
 // the lengths (a few KB out of the caches) and one launch does it all: the call's latency is what matters here.
 //
-// Bound by the latency of three dependent loads (lengths, stack, the launch itself): 5 us for 64 requests' decode step as for
+// Bound by the latency of its dependent loads (lengths, then stack): 5 us for a decode step of 64 requests, 7 for
 // 203 ragged prompts.
 struct Want { long long n, need; bool fits; };
 

@@ -36,7 +36,6 @@ struct RotDesc {
 
 namespace {
 constexpr int NTH = 256;
-constexpr int NOTURN = 256;       // most pairs of a head
 
 template <int T> struct Elem;
 template <> struct Elem<0> { typedef float t; static constexpr int VEC = 4; };
@@ -110,19 +109,24 @@ __device__ __forceinline__ void item_chunks(int i, int D, int R, int inter, int&
   b = j < n && j + n < nt ? R + (j + n) * VEC : -1;
 }
 
-// the pairs of a lane's two chunks: (a[i], b[i]), or inside each chunk
+// the pairs of a lane's two chunks: (a[i], b[i]), or inside each chunk. Chunks that do not turn (ta, tb) stay as they are,
+// whatever their neighbours hold
 template <int VEC, bool INSIDE>
-__device__ __forceinline__ void turn(float* a, float* b, const float* c, const float* s) {
+__device__ __forceinline__ void turn(float* a, float* b, const float* c, const float* s, bool ta, bool tb) {
   if (INSIDE) {
 #pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) {
-      const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], w = b[2 * i + 1];
-      a[2 * i] = x * c[i] - y * s[i];
-      a[2 * i + 1] = y * c[i] + x * s[i];
-      b[2 * i] = z * c[VEC / 2 + i] - w * s[VEC / 2 + i];
-      b[2 * i + 1] = w * c[VEC / 2 + i] + z * s[VEC / 2 + i];
+    for (int j = 0; j < 2; ++j) {
+      float* v = j ? b : a;
+      if (j ? tb : ta) {
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+          const float x = v[2 * i], y = v[2 * i + 1], cc = c[j * (VEC / 2) + i], ss = s[j * (VEC / 2) + i];
+          v[2 * i] = x * cc - y * ss;
+          v[2 * i + 1] = y * cc + x * ss;
+        }
+      }
     }
-  } else {
+  } else if (ta) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const float x = a[i], y = b[i];
@@ -136,8 +140,8 @@ __device__ __forceinline__ void turn(float* a, float* b, const float* c, const f
 template <int VEC, int ITEMS, bool INSIDE>
 struct Lane {
   int ca[ITEMS], cb[ITEMS];              // first elements, 0 where there is no such chunk
-  bool ha[ITEMS], hb[ITEMS];
-  int fa[ITEMS], fb[ITEMS];              // first pair (INSIDE: of each chunk); NOTURN: these do not turn
+  bool ha[ITEMS], hb[ITEMS], ta[ITEMS], tb[ITEMS];
+  int fa[ITEMS], fb[ITEMS];              // first pair (INSIDE: of each chunk), 0 where the chunk does not turn
 
   __device__ __forceinline__ Lane(const RotDesc& d, int il, int lph) {
 #pragma unroll
@@ -148,18 +152,20 @@ struct Lane {
       hb[it] = b >= 0;
       ca[it] = max(a, 0);
       cb[it] = max(b, 0);
-      fa[it] = a < 0 || a >= d.R ? NOTURN : INSIDE ? a / 2 : VEC == 1 ? il + it * lph : a;
-      fb[it] = b < 0 || b >= d.R ? NOTURN : b / 2;
+      ta[it] = ha[it] && a < d.R;
+      tb[it] = hb[it] && b < d.R;
+      fa[it] = !ta[it] ? 0 : INSIDE ? a / 2 : VEC == 1 ? il + it * lph : a;
+      fb[it] = tb[it] ? b / 2 : 0;
     }
   }
 };
 
 // Shared memory of a block: norm weights (fp32), frequencies (turns per position), and each wave's cos and sin of the
-// pairs of its token, times mscale; behind them a pair that does not turn
+// pairs of its token, times mscale
 struct Staged {
   float w[2][512];
   double f[256];
-  float c[NTH / 64][NOTURN + 8], s[NTH / 64][NOTURN + 8];
+  float c[NTH / 64][256], s[NTH / 64][256];
 };
 
 // an offset of 0 that the compiler cannot see through: reads of Staged at it stay where they are written. Hoisted out of
@@ -176,10 +182,6 @@ __device__ __forceinline__ void stage(const RotDesc& d, Staged& s) {
     if (d.wk) s.w[1][i] = load_w(d.wk, d.wtype, i);
   }
   if ((int)threadIdx.x < d.R / 2) s.f[threadIdx.x] = d.freqs[threadIdx.x] * 0.15915494309189535;
-  if (threadIdx.x < 32) {
-    s.c[threadIdx.x >> 3][NOTURN + (threadIdx.x & 7)] = 1.f;
-    s.s[threadIdx.x >> 3][NOTURN + (threadIdx.x & 7)] = 0.f;
-  }
   __syncthreads();
 }
 
@@ -236,10 +238,7 @@ __device__ __forceinline__ void own_angles(const double* f, int fa, int fb, doub
                                            float* s) {
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const int p = INSIDE && i >= VEC / 2 ? fb : fa, j = INSIDE && i >= VEC / 2 ? i - VEC / 2 : i;
-    turn_of(pos, f[p < NOTURN ? p + j : 0], m, sign, c[i], s[i]);
-    c[i] = p < NOTURN ? c[i] : 1.f;
-    s[i] = p < NOTURN ? s[i] : 0.f;
+    turn_of(pos, f[INSIDE && i >= VEC / 2 ? fb + i - VEC / 2 : fa + i], m, sign, c[i], s[i]);
   }
 }
 
@@ -270,11 +269,11 @@ __device__ __forceinline__ Row row_of(const RotDesc& d, long long t, int p, int 
 constexpr int VCH = 4;
 
 template <typename E, int EV>
-__device__ __forceinline__ void append_run(const RotDesc& d, long long t, long long slot, int e0) {
+__device__ __forceinline__ void append_run(const RotDesc& d, long long t, int slot, int e0) {
   const long long page = slot / d.page;
-  const int o8 = (int)(slot % d.page) / 8, n = d.Hk * d.D;
+  const int o8 = slot % d.page / 8, n = d.Hk * d.D;
   const E* v = (const E*)d.v + t * d.v_ts;
-#pragma unroll
+#pragma unroll 2
   for (int i = 0; i < VCH; ++i) {
     const int e = e0 + i * 64 * EV;
     if (e >= n) return;
@@ -294,9 +293,9 @@ __device__ __forceinline__ void append_run(const RotDesc& d, long long t, long l
 }
 
 template <typename E, int EV>
-__device__ __forceinline__ void append_one(const RotDesc& d, long long t, long long slot, int e0) {
+__device__ __forceinline__ void append_one(const RotDesc& d, long long t, int slot, int e0) {
   const long long page = slot / d.page;
-  const int off = (int)(slot % 8), o8 = (int)(slot % d.page) / 8, n = d.Hk * d.D;
+  const int off = slot % 8, o8 = slot % d.page / 8, n = d.Hk * d.D;
   const E* v = (const E*)d.v + t * d.v_ts;
   Chunk<E, EV> x[VCH];
 #pragma unroll
@@ -380,7 +379,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
       const bool isq = p0 + p < pq;
       const long long rt = row[p].t;
       const int h = row[p].h;
-      const long long slot = CACHE && !isq ? d.slots[rt] : 0;
+      const int slot = CACHE && !isq ? d.slots[rt] : 0;
       const double pos = ROWS && !still ? (double)d.pos[rt] : 0.0;
       float a[ITEMS][VEC], b[ITEMS][VEC];
 #pragma unroll
@@ -415,7 +414,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
       if (!row[p].on || slot < 0 || (CACHE && slot >= d.nslots)) continue;
       E* o;
       if (isq) o = (E*)d.qo + (rt * d.Hq + h) * d.D;
-      else if (CACHE) o = (E*)d.ko + ((slot / d.page * d.Hk + h) * d.page + slot % d.page) * d.D;
+      else if (CACHE) o = (E*)d.ko + (((long long)(slot / d.page) * d.Hk + h) * d.page + slot % d.page) * d.D;
       else o = (E*)d.ko + (rt * d.Hk + h) * d.D;
 #pragma unroll
       for (int it = 0; it < ITEMS; ++it) {
@@ -427,7 +426,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int
           read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
           read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
         }
-        turn<VEC, INSIDE>(a[it], b[it], c, s);
+        turn<VEC, INSIDE>(a[it], b[it], c, s, ln.ta[it], ln.tb[it]);
         if (ln.ha[it]) store<false, E, VEC>(o + ln.ca[it], a[it]);
         if (ln.hb[it]) store<false, E, VEC>(o + ln.cb[it], b[it]);
       }
@@ -506,7 +505,7 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
           read_angles<VEC, INSIDE>(sh.c[wave] + z, ln.fa[it], ln.fb[it], c);
           read_angles<VEC, INSIDE>(sh.s[wave] + z, ln.fa[it], ln.fb[it], s);
         }
-        turn<VEC, INSIDE>(a[it], b[it], c, s);
+        turn<VEC, INSIDE>(a[it], b[it], c, s, ln.ta[it], ln.tb[it]);
       }
       if (NORM && (isq ? d.wq != nullptr : d.wk != nullptr)) {
         // with p = sum x^2 and e = sum g w x:  u = x r,  dx = r g w - (e r^3 / D) x,  dw += g x r

@@ -558,3 +558,32 @@ def test_model_rotary_training_gpu(cuda):
         assert torch.nn.functional.cosine_similarity(a, b, dim=0) > 0.97, n
     cos = torch.nn.functional.cosine_similarity(m.store.grad.cpu(), c.store.grad, dim=0)
     assert cos > 0.97, cos
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("dtype,D,rot", [(BF, 128, 64), (HF, 96, 48), (F32, 64, 32), (BF, 128, 0), (BF, 33, 8), (BF, 24, 16),
+                                         (BF, 80, 16)])
+def test_dims_that_do_not_turn_are_untouched(cuda, dtype, D, rot, inter):
+    """infinities and NaN beside the rotated dims, in either direction, and in keys that are appended as they are"""
+    g = gen(cuda, 70)
+    q, k = (torch.randn(5, h, D, device=cuda, generator=g).to(dtype) for h in (3, 1))
+    q[:, :, rot::2] = float("inf")
+    k[1, :, -1] = float("nan")
+    k[2, :, rot] = float("-inf")
+    freqs = rotary.rotary_freqs(rot, device=cuda)[0] if rot else None
+    f64 = freqs if rot else torch.zeros(0, dtype=torch.float64, device=cuda)
+    pos = torch.arange(5, device=cuda) * 1000
+    q.requires_grad_()
+    qo, ko = rotary.rotary(q, k, pos, freqs, interleaved=inter, mscale=1.3)
+    for x, y in ((q.detach(), qo.detach()), (k, ko)):
+        assert torch.equal(torch.nan_to_num(y[..., rot:]), torch.nan_to_num(x[..., rot:]))
+        assert torch.equal(torch.isnan(y), torch.isnan(x))
+        if rot:
+            close_rows(y[..., :rot].contiguous(), rotary64(x, None, pos, f64, inter, 1.3, 1e-5)[..., :rot], dtype)
+    dq, = torch.autograd.grad(qo, q, q.detach())
+    assert torch.equal(dq[..., rot:], q.detach()[..., rot:]) and bool(torch.isfinite(dq[..., :rot]).all())
+    slots = torch.arange(5, dtype=torch.int32, device=cuda) + 2
+    kc, vc = paged.page_pools(1, 16, 1, D, dtype, cuda)
+    paged.append(k, k, kc, vc, slots)
+    assert torch.equal(torch.nan_to_num(kc[0, :, 2:7].transpose(0, 1)), torch.nan_to_num(k))
+    assert torch.equal(torch.isnan(kc[0, :, 2:7].transpose(0, 1)), torch.isnan(k))
