@@ -41,7 +41,9 @@ constexpr int NTH = 256;
 // 203 ragged prompts.
 struct Want { long long n, need; bool fits; };
 
-__device__ __forceinline__ unsigned pages_of(unsigned tokens, unsigned page) { return tokens ? (tokens - 1) / page + 1 : 0; }
+__device__ __forceinline__ unsigned pages_of(unsigned tokens, unsigned page) {
+  return tokens ? (tokens - 1) / page + 1 : 0;
+}
 
 __device__ __forceinline__ Want want_of(const PlanDesc& d, int b, int& c) {
   c = max(d.cached[b], 0);
@@ -238,13 +240,14 @@ template <> struct Mat<2> {
 // still a small part of the loads' (16 x 16-cycle products to 16 KB a tile and wave).
 //
 // Softmax in one pass with the running maximum; P enters the product as two summands of the cache's type (its value
-// and what that rounding left), so the weights keep at least 16 bits. Waves, then splits, are joined by their maxima and sums.
+// and what that rounding left), so the weights keep at least 16 bits. Waves, then splits, are joined by their maxima
+// and sums.
 //
 // Keys past the length, and pages whose id is not one, have weight 0 and a value of 0 whatever the cache holds there.
 //
-// Bound by the read of the cache. V goes past the caches: a load takes whole lines of it. K's loads take half a line of each
-// key row, the next load the other half out of the cache; past it they cost 7 % more. At 64 x ~6100 tokens, 8 key heads x
-// 128, 4 query heads each (1.6 GB): 258 us, 6.2 TB/s, where a bare read of such data reaches 7.1.
+// Bound by the read of the cache. V goes past the caches: a load takes whole lines of it. K's loads take half a line
+// of each key row, the next load the other half out of the cache; past it they cost 7 % more. At 64 x ~6100 tokens, 8
+// key heads x 128, 4 query heads each (1.6 GB): 258 us, 6.2 TB/s, where a bare read of such data reaches 7.1.
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG = -3.0e38f;                   // a running maximum before any key
 
@@ -253,8 +256,8 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   typedef typename Mat<TYPE>::v vec;
   constexpr int NK = D / 32, NV = D / 16, NW = NTH / 64;
   __shared__ float sm[NW][16], sl[NW][16];
-  extern __shared__ float sacc[];                 // [NW][query heads of the block][D + 4]: one head's 2 KB leave room for
-                                                  // four blocks a CU, space for 16 heads for three
+  // [NW][query heads of the block][D + 4]: one head's 2 KB leave room for four blocks a CU, 16 heads' for three
+  extern __shared__ float sacc[];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
   const int G = d.Hq / d.Hk, ng = (G + 15) / 16;
   const int hk = blockIdx.y / ng, gi = blockIdx.y % ng, b = blockIdx.z, sp = blockIdx.x;
@@ -290,7 +293,8 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   if (d.cap > 0) ids(k0 + 32 * w);
   for (int t0 = k0 + 32 * w; t0 < k1; t0 += 32 * NW) {
     const bool bad_v = (unsigned)iv >= (unsigned)d.P;
-    const long long ja = (unsigned)ia < (unsigned)d.P ? ia : 0, jb = (unsigned)ib < (unsigned)d.P ? ib : 0, jv = bad_v ? 0 : iv;
+    const long long ja = (unsigned)ia < (unsigned)d.P ? ia : 0, jb = (unsigned)ib < (unsigned)d.P ? ib : 0;
+    const long long jv = bad_v ? 0 : iv;
     const uint16_t* pa = K + ja * pst + hoff + ((t0 + ra) & in_page) * D + 8 * g;
     const uint16_t* pb = K + jb * pst + hoff + ((t0 + ra + 4) & in_page) * D + 8 * g;
     const uint16_t* pv = V + jv * pst + hoff + ((t0 + rv) & in_page) * D + 8 * n;
@@ -388,7 +392,51 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   }
 }
 
-// the splits of one query head: block (Hq, B). The weights of the splits first, each by a thread; then D / 4 threads a
+// Splits of one request joined, up to NS of them: a wave a query head, its lanes over the dims, every row and weight
+// loaded at once -- no exchange, one round trip after the length's (64 requests x 32 heads, 4 splits: 4.2 us; the
+// kernel for many, three round trips: 5.4)
+template <int TYPE, int D, int NS>
+__global__ __launch_bounds__(NTH) void paged_join_few_kernel(const PagedDesc d) {
+  const long long u = (long long)blockIdx.x * (NTH / 64) + (threadIdx.x >> 6);
+  if (u >= (long long)d.B * d.Hq) return;
+  const int lane = threadIdx.x & 63;
+  const int len = min(max(d.lens[u / d.Hq], 0), d.cap);
+  if (len <= d.split) return;
+  const int ns = (len + d.split - 1) / d.split;
+  const float* ml = d.part + (long long)d.B * d.Hq * d.nsplit * D + u * d.nsplit * 2;
+  const float* pt = d.part + u * d.nsplit * D;
+  constexpr int R = (D + 63) / 64;                   // dims lane, lane + 64, ...
+  float m[NS], l[NS], x[NS][R];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const int j = min(s, ns - 1);                    // past the last split: its row again, with weight 0
+    m[s] = ml[2 * j];
+    l[s] = ml[2 * j + 1];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[s][r] = pt[j * D + min(lane + 64 * r, D - 1)];
+  }
+  float M = m[0];
+#pragma unroll
+  for (int s = 1; s < NS; ++s) M = fmaxf(M, m[s]);
+  float L = 0.f, o[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) o[r] = 0.f;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const float f = __builtin_amdgcn_exp2f(m[s] - M);
+    if (s < ns) {
+      L += f * l[s];
+#pragma unroll
+      for (int r = 0; r < R; ++r) o[r] += f * x[s][r];
+    }
+  }
+  uint16_t* out = (uint16_t*)d.o + u * D;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (lane + 64 * r < D) out[lane + 64 * r] = Mat<TYPE>::bits(L != 0.f ? o[r] / L : 0.f);
+}
+
+// Many splits of one query head: block (Hq, B). The weights of the splits first, each by a thread; then D / 4 threads a
 // split row, 1024 / D rows side by side, joined in a fixed order
 constexpr int MAX_SPLITS = 1024;
 
@@ -437,26 +485,30 @@ __global__ __launch_bounds__(NTH) void paged_join_kernel(const PagedDesc d) {
 }
 
 template <int TYPE, int D>
-void launch_attn(const PagedDesc& d, hipStream_t st) {
+int attn_of(const PagedDesc& d, hipStream_t st) {
   const int G = d.Hq / d.Hk, ng = (G + 15) / 16, gc = G < 16 ? G : 16;
   hipLaunchKernelGGL((paged_attn_kernel<TYPE, D>), dim3(d.nsplit, d.Hk * ng, d.B), dim3(NTH),
                      NTH / 64 * gc * (D + 4) * sizeof(float), st, d);
+  const int rc = (int)hipGetLastError();
+  if (rc || d.nsplit == 1) return rc;
+  const long long rows = (long long)d.B * d.Hq;
+  const dim3 few((unsigned)((rows + NTH / 64 - 1) / (NTH / 64)));
+  if (d.nsplit <= 4) hipLaunchKernelGGL((paged_join_few_kernel<TYPE, D, 4>), few, dim3(NTH), 0, st, d);
+  else if (d.nsplit <= 12) hipLaunchKernelGGL((paged_join_few_kernel<TYPE, D, 12>), few, dim3(NTH), 0, st, d);
+  else hipLaunchKernelGGL(paged_join_kernel<TYPE>, dim3(d.Hq, d.B), dim3(NTH), 0, st, d);
+  return (int)hipGetLastError();
 }
 
 template <int TYPE>
 int attn(const PagedDesc& d, hipStream_t st) {
   switch (d.D) {
-    case 32: launch_attn<TYPE, 32>(d, st); break;
-    case 64: launch_attn<TYPE, 64>(d, st); break;
-    case 96: launch_attn<TYPE, 96>(d, st); break;
-    case 128: launch_attn<TYPE, 128>(d, st); break;
-    case 256: launch_attn<TYPE, 256>(d, st); break;
-    default: return -2;
+    case 32: return attn_of<TYPE, 32>(d, st);
+    case 64: return attn_of<TYPE, 64>(d, st);
+    case 96: return attn_of<TYPE, 96>(d, st);
+    case 128: return attn_of<TYPE, 128>(d, st);
+    case 256: return attn_of<TYPE, 256>(d, st);
   }
-  int rc = (int)hipGetLastError();
-  if (rc || d.nsplit == 1) return rc;
-  hipLaunchKernelGGL(paged_join_kernel<TYPE>, dim3(d.Hq, d.B), dim3(NTH), 0, st, d);
-  return (int)hipGetLastError();
+  return -2;
 }
 }  // namespace
 
@@ -478,7 +530,8 @@ OBST_API int obst_page_release(const void* done, void* lens, const void* table, 
 }
 
 OBST_API int obst_paged_attn(const PagedDesc* d, hipStream_t st) {
-  if (!d || d->B < 1 || d->B > 65535 || d->Hk < 1 || d->Hq < 1 || d->Hq % d->Hk || d->P < 1 || d->cap < 0 || d->cap > 1 << 30 ||
+  if (!d || d->B < 1 || d->B > 65535 || d->Hk < 1 || d->Hq < 1 || d->Hq % d->Hk || d->P < 1 || d->cap < 0 ||
+      d->cap > 1 << 30 ||
       d->nsplit < 1 || d->nsplit > MAX_SPLITS || d->split < 32 || d->split % 32 || (d->nsplit > 1 && !d->part))
     return -1;
   if (d->shift < 4 || d->shift > 8 || (long long)d->ld << d->shift < d->cap) return -3;

@@ -63,10 +63,10 @@ __device__ __forceinline__ void store(E* p, const float* f) {
   else *reinterpret_cast<Chunk<E, VEC>*>(p) = c;
 }
 
-// LINES, in the normed backward: chunks go past the caches where a head's lanes together take whole 128-byte lines (bf16 x
-// 128: 165 -> 146 us for the loads, 141 with the stores). Where they take parts of lines, the caches hold the rest for the other
-// half's access (fp32 x 96, half a head 1.5 lines: 26 us, 30 past the caches). The forward, at 6 TB/s, gains nothing from
-// loads and loses 10 % with stores past the caches.
+// LINES, in the normed backward: chunks go past the caches where a head's lanes together take whole 128-byte lines
+// (bf16 x 128: 165 -> 146 us for the loads, 141 with the stores). Where they take parts of lines, the caches hold the
+// rest for the other half's access (fp32 x 96, half a head 1.5 lines: 26 us, 30 past the caches). The forward, at 6
+// TB/s, gains nothing from loads and loses 10 % with stores past the caches.
 template <bool LINES, typename E, int VEC>
 __device__ __forceinline__ Chunk<E, VEC> load_once(const E* p) {
   if constexpr (LINES) {
@@ -86,7 +86,8 @@ __device__ __forceinline__ void forget(Chunk<E, VEC>& c) {
 }
 
 __device__ __forceinline__ float load_w(const void* w, int type, int i) {
-  return type == 0 ? ((const float*)w)[i] : type == 1 ? bf2f(((const bf16_t*)w)[i]) : __half2float(((const __half*)w)[i]);
+  if (type == 0) return ((const float*)w)[i];
+  return type == 1 ? bf2f(((const bf16_t*)w)[i]) : __half2float(((const __half*)w)[i]);
 }
 
 // first elements of the two chunks of item `i` of a head; -1: no such chunk
@@ -109,8 +110,8 @@ __device__ __forceinline__ void item_chunks(int i, int D, int R, int inter, int&
   b = j < n && j + n < nt ? R + (j + n) * VEC : -1;
 }
 
-// the pairs of a lane's two chunks: (a[i], b[i]), or inside each chunk. Chunks that do not turn (ta, tb) stay as they are,
-// whatever their neighbours hold
+// the pairs of a lane's two chunks: (a[i], b[i]), or inside each chunk. Chunks that do not turn (ta, tb) stay as they
+// are, whatever their neighbours hold
 template <int VEC, bool INSIDE>
 __device__ __forceinline__ void turn(float* a, float* b, const float* c, const float* s, bool ta, bool tb) {
   if (INSIDE) {
@@ -168,8 +169,8 @@ struct Staged {
   float c[NTH / 64][256], s[NTH / 64][256];
 };
 
-// an offset of 0 that the compiler cannot see through: reads of Staged at it stay where they are written. Hoisted out of
-// the loops, as it would have them, they hold 32 to 48 registers a lane and spill
+// an offset of 0 that the compiler cannot see through: reads of Staged at it stay where they are written. Hoisted out
+// of the loops, as it would have them, they hold 32 to 48 registers a lane and spill
 __device__ __forceinline__ int here() {
   int z = 0;
   asm volatile("" : "+s"(z));
@@ -185,8 +186,9 @@ __device__ __forceinline__ void stage(const RotDesc& d, Staged& s) {
   __syncthreads();
 }
 
-// cos and sin of pos * f turns, times m and (sin) sign. The angle is reduced in 64 bits to a quarter turn r in [-1/2, 1/2] and
-// its quadrant; there the Taylor polynomials of sin and cos(pi r / 2) to the 9th and 10th power are off by less than 2^-28
+// cos and sin of pos * f turns, times m and (sin) sign. The angle is reduced in 64 bits to a quarter turn r in [-1/2,
+// 1/2] and its quadrant; there the Taylor polynomials of sin and cos(pi r / 2) to the 9th and 10th power are off by
+// less than 2^-28
 __device__ __forceinline__ void turn_of(double pos, double f, float m, float sign, float& c, float& s) {
   double t = pos * f;
   t = 4.0 * (t - rint(t));
@@ -202,8 +204,8 @@ __device__ __forceinline__ void turn_of(double pos, double f, float m, float sig
   s = m * sign * (q & 2 ? -u : u);
 }
 
-// those of a token, a pair a lane, through shared memory for all of the wave's heads (each lane forming those of its own
-// pairs, eight times over in a wave of eight heads, took half of the forward's instructions)
+// those of a token, a pair a lane, through shared memory for all of the wave's heads (each lane forming those of its
+// own pairs, eight times over in a wave of eight heads, took half of the forward's instructions)
 __device__ __forceinline__ void turn_angles(const RotDesc& d, Staged& sh, int w, double pos, float sign) {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // the wave's reads of its last token's are done
   for (int i = threadIdx.x & 63; i < d.R / 2; i += 64) turn_of(pos, sh.f[i], d.mscale, sign, sh.c[w][i], sh.s[w][i]);
@@ -242,8 +244,8 @@ __device__ __forceinline__ void own_angles(const double* f, int fa, int fb, doub
   }
 }
 
-// Which row a lane has in a pass. Passes run over the heads of q, then of k: of one token, or (ROWS) over all (token, head)
-// pairs of the call, where a token's heads leave most of a wave's lanes without one.
+// Which row a lane has in a pass. Passes run over the heads of q, then of k: of one token, or (ROWS) over all (token,
+// head) pairs of the call, where a token's heads leave most of a wave's lanes without one.
 struct Row {
   long long t;
   int h;
@@ -260,12 +262,13 @@ __device__ __forceinline__ Row row_of(const RotDesc& d, long long t, int p, int 
   return {c / H, (int)(c % H), r < n};
 }
 
-// Values into their columns of eight tokens: V cache [P][Hk][page / 8][D][8]. A wave takes a window of wt neighbouring
-// tokens (8, or 1 where there are few) and VCH pieces of 64 * EV elements of their heads. Eight tokens of the step that
-// fill one column block, slots 8 j .. 8 j + 7, are written together, 16 bytes at a time, by the window that holds the first
-// of them. Tokens outside such a run (a decode step's, a run's ragged ends) write their elements one by one.
-// (A window a token, with the other seven of a run idle, left all of a prompt's work to every eighth block, which is
-// one of the eight dies: 127 us where windows of eight take 46, 5.9 TB/s, at 16384 tokens of 16 heads x 128.)
+// Values into their columns of eight tokens: V cache [P][Hk][page / 8][D][8]. A wave takes a window of wt
+// neighbouring tokens (8, or 1 where there are few) and VCH pieces of 64 * EV elements of their heads. Eight tokens
+// of the step that fill one column block, slots 8 j .. 8 j + 7, are written together, 16 bytes at a time, by the
+// window that holds the first of them. Tokens outside such a run (a decode step's, a run's ragged ends) write their
+// elements one by one. (A window a token, with the other seven of a run idle, left all of a prompt's work to every
+// eighth block, which is one of the eight dies: 127 us where windows of eight take 46, 5.9 TB/s, at 16384 tokens of
+// 16 heads x 128.)
 constexpr int VCH = 4;
 
 template <typename E, int EV>
@@ -323,7 +326,8 @@ __device__ __forceinline__ void append_values(const RotDesc& d, long long unit, 
   const int slot = at >= 0 && at < d.T && raw >= 0 && raw < d.nslots ? raw : -2;
   // bit i: the token of lane i follows its neighbour's slot; it is the first of a whole run
   const unsigned long long next = __ballot(slot >= 0 && slot == __shfl_up(slot, 1, 64) + 1 && lane > 0);
-  const unsigned long long first = __ballot(slot >= 0 && slot % 8 == 0 && lane < 15 && (next >> (lane + 1) & 0x7f) == 0x7f);
+  const unsigned long long first =
+      __ballot(slot >= 0 && slot % 8 == 0 && lane < 15 && (next >> (lane + 1) & 0x7f) == 0x7f);
   for (int i = 7; i < 7 + wt; ++i) {
     const int s = __builtin_amdgcn_readlane(slot, i);
     if (s < 0) continue;
@@ -332,10 +336,11 @@ __device__ __forceinline__ void append_values(const RotDesc& d, long long unit, 
   }
 }
 
-// ---- forward. A wave's unit is U passes, of one token or (ROWS) of the call; a pass is 64 / lph heads, all of q or all of k.
-// CACHE: k goes into the pages, and the blocks behind the first `rot` write the values.
+// ---- forward. A wave's unit is U passes, of one token or (ROWS) of the call; a pass is 64 / lph heads, all of q or
+// all of k. CACHE: k goes into the pages, and the blocks behind the first `rot` write the values.
 template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool ROWS, bool CACHE, int EV>
-__global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int lph, int pq, int pk, int rot, int nvg, int wt) {
+__global__ __launch_bounds__(NTH, 4) void rotary_fwd_kernel(const RotDesc d, int lph, int pq, int pk, int rot,
+                                                            int nvg, int wt) {
   typedef typename Elem<TYPE>::t E;
   __shared__ Staged sh;
   if (CACHE && (int)blockIdx.x >= rot) {
@@ -577,8 +582,8 @@ __global__ __launch_bounds__(NTH, 4) void rotary_bwd_kernel(const RotDesc d, int
   }
 }
 
-// weight gradients from the blocks' partials, in 64 bits (up to 1024 of them): 16 columns a block, 64 rows of it side by
-// side, in a fixed order
+// weight gradients from the blocks' partials, in 64 bits (up to 1024 of them): 16 columns a block, 64 rows of it side
+// by side, in a fixed order
 __global__ __launch_bounds__(1024) void rotary_fold_kernel(const RotDesc d, int nbq, int nb) {
   __shared__ double red[64][17];
   const int col = threadIdx.x & 15, row = threadIdx.x >> 4, e = blockIdx.x * 16 + col;
@@ -647,15 +652,15 @@ int forward(const RotDesc& d, int lph, hipStream_t st) {
   const Passes<ROWS> p(d, lph);
   const int grid = p.blocks(p.units(d, U), FWD_BLOCKS);
   if (!d.slots) {
-    hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, false, 1>), dim3(grid), dim3(NTH), 0, st, d, lph,
-                       p.pq, p.pk, grid, 0, 0);
+    hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, false, 1>), dim3(grid), dim3(NTH), 0, st,
+                       d, lph, p.pq, p.pk, grid, 0, 0);
     return (int)hipGetLastError();
   }
   constexpr int EV = VEC == 1 ? 1 : 2;                     // VEC > 1: D and the strides are even
   const int nvg = (d.Hk * d.D + VCH * 64 * EV - 1) / (VCH * 64 * EV), wt = d.T < 1024 ? 1 : 8;
   const int vgrid = p.blocks((d.T + wt - 1) / wt * nvg, FWD_BLOCKS);
-  hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, true, EV>), dim3(grid + vgrid), dim3(NTH), 0, st, d,
-                     lph, p.pq, p.pk, grid, nvg, wt);
+  hipLaunchKernelGGL((rotary_fwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, true, EV>), dim3(grid + vgrid), dim3(NTH), 0,
+                     st, d, lph, p.pq, p.pk, grid, nvg, wt);
   return (int)hipGetLastError();
 }
 
@@ -663,8 +668,8 @@ template <int TYPE, int VEC, int ITEMS, int U, bool INSIDE, bool ROWS>
 int backward(const RotDesc& d, int lph, hipStream_t st) {
   const Passes<ROWS> p(d, lph);
   const int grid = p.blocks(p.units(d, U), BWD_BLOCKS);
-  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, false, false>), dim3(grid), dim3(NTH), 0, st, d, lph, p.pq,
-                     p.pk, 0);
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, U, INSIDE, ROWS, false, false>), dim3(grid), dim3(NTH), 0, st,
+                     d, lph, p.pq, p.pk, 0);
   return (int)hipGetLastError();
 }
 
@@ -679,33 +684,37 @@ int backward_normed(const RotDesc& d, int lph, hipStream_t st) {
     nq = nq < 1 ? 1 : nq > BWD_BLOCKS - 1 ? BWD_BLOCKS - 1 : nq;
     nk = BWD_BLOCKS - nq;
   }
-  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, 1, INSIDE, ROWS, true, LINES>), dim3(nq + nk), dim3(NTH), 0, st, d, lph, p.pq,
-                     p.pk, nq);
+  hipLaunchKernelGGL((rotary_bwd_kernel<TYPE, VEC, ITEMS, 1, INSIDE, ROWS, true, LINES>), dim3(nq + nk), dim3(NTH), 0, st,
+                     d, lph, p.pq, p.pk, nq);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
   hipLaunchKernelGGL(rotary_fold_kernel, dim3((2 * d.D + 15) / 16), dim3(1024), 0, st, d, nq, nq + nk);
   return (int)hipGetLastError();
 }
 
-// Passes a unit. Four share one token's angles and keep four rows of loads in flight (two where the rows are several tokens':
-// registers); under 1024 tokens one each spreads them over more waves. The normed backward takes one: a second pass' loads and the sums leave it three waves a SIMD
-// (199 us where one pass took 164 at the time, 32768 tokens of 2 x 16 heads x 128 in bf16).
+// Passes a unit. Four share one token's angles and keep four rows of loads in flight (two where the rows are several
+// tokens': registers); under 1024 tokens one each spreads them over more waves. The normed backward takes one: a
+// second pass' loads and the sums leave it three waves a SIMD (199 us where one pass took 164 at the time, 32768
+// tokens of 2 x 16 heads x 128 in bf16).
 template <int TYPE, int VEC, bool INSIDE, bool ROWS>
 int by_tokens(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
   constexpr int MANY = ROWS ? 2 : 4;
   const bool few = d.T < 1024;
   if (!bwd)
-    return few ? forward<TYPE, VEC, 1, 1, INSIDE, ROWS>(d, lph, st) : forward<TYPE, VEC, 1, MANY, INSIDE, ROWS>(d, lph, st);
+    return few ? forward<TYPE, VEC, 1, 1, INSIDE, ROWS>(d, lph, st)
+               : forward<TYPE, VEC, 1, MANY, INSIDE, ROWS>(d, lph, st);
   if (d.wq || d.wk)
     return items_of(d, VEC) * 16 % 128 == 0 ? backward_normed<TYPE, VEC, 1, INSIDE, ROWS, true>(d, lph, st)
                                             : backward_normed<TYPE, VEC, 1, INSIDE, ROWS, false>(d, lph, st);
-  return few ? backward<TYPE, VEC, 1, 1, INSIDE, ROWS>(d, lph, st) : backward<TYPE, VEC, 1, MANY, INSIDE, ROWS>(d, lph, st);
+  return few ? backward<TYPE, VEC, 1, 1, INSIDE, ROWS>(d, lph, st)
+             : backward<TYPE, VEC, 1, MANY, INSIDE, ROWS>(d, lph, st);
 }
 
 template <int TYPE, int ITEMS>
 int by_element(const RotDesc& d, bool bwd, int lph, hipStream_t st) {
   if (!bwd) return forward<TYPE, 1, ITEMS, 1, false, false>(d, lph, st);
-  return d.wq || d.wk ? backward_normed<TYPE, 1, ITEMS, false, false, false>(d, lph, st) : backward<TYPE, 1, ITEMS, 1, false, false>(d, lph, st);
+  return d.wq || d.wk ? backward_normed<TYPE, 1, ITEMS, false, false, false>(d, lph, st)
+                      : backward<TYPE, 1, ITEMS, 1, false, false>(d, lph, st);
 }
 
 template <int TYPE>
@@ -713,13 +722,15 @@ int dispatch(const RotDesc& d, bool bwd, hipStream_t st) {
   constexpr int V = Elem<TYPE>::VEC;
   if (vec_ok(d, V, bwd)) {
     const int lph = pow2_at_least(items_of(d, V));
-    // Rows of several tokens in a wave where one token's heads fill at most half of it. 65536 tokens normed in bf16, forward +
-    // backward, rows against tokens: 1 + 1 heads x 32 17 + 19 against 52 + 99 us, 8 + 8 x 32 34 + 56 against 53 + 101; at 12 +
-    // 12 x 64 (three quarters of a wave), 32768 tokens, 48 + 76 against 40 + 68
+    // Rows of several tokens in a wave where one token's heads fill at most half of it. 65536 tokens normed in bf16,
+    // forward + backward, rows against tokens: 1 + 1 heads x 32 17 + 19 against 52 + 99 us, 8 + 8 x 32 34 + 56
+    // against 53 + 101; at 12 + 12 x 64 (three quarters of a wave), 32768 tokens, 48 + 76 against 40 + 68
     const int most = d.Hq > d.Hk ? d.Hq : d.Hk;
     if (most * lph <= 32 && d.T * most < 1LL << 31)
-      return d.inter ? by_tokens<TYPE, V, true, true>(d, bwd, lph, st) : by_tokens<TYPE, V, false, true>(d, bwd, lph, st);
-    return d.inter ? by_tokens<TYPE, V, true, false>(d, bwd, lph, st) : by_tokens<TYPE, V, false, false>(d, bwd, lph, st);
+      return d.inter ? by_tokens<TYPE, V, true, true>(d, bwd, lph, st)
+                     : by_tokens<TYPE, V, false, true>(d, bwd, lph, st);
+    return d.inter ? by_tokens<TYPE, V, true, false>(d, bwd, lph, st)
+                   : by_tokens<TYPE, V, false, false>(d, bwd, lph, st);
   }
   const int n = items_of(d, 1);
   return n <= 64 ? by_element<TYPE, 1>(d, bwd, pow2_at_least(n), st) : by_element<TYPE, 4>(d, bwd, 64, st);

@@ -183,8 +183,8 @@ class Model:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 out = self.logits(tok)
-            g = kv.persist["graph"] = {"shape": (tuple(tokens.shape), kv.pages is not None), "graph": graph, "tok": tok, "pos": kv.pos,
-                                       "out": out}
+            g = kv.persist["graph"] = {"shape": (tuple(tokens.shape), kv.pages is not None), "graph": graph,
+                                       "tok": tok, "pos": kv.pos, "out": out}
         else:
             g["tok"].copy_(tokens, non_blocking=True)
             g["pos"].copy_(positions, non_blocking=True)

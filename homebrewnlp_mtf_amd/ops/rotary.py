@@ -21,7 +21,6 @@ from . import raw
 from .functional import _acc_grad, _done, _param32
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_TYPES = set(DTYPES)
 MAX_DIM = 512
 
 
@@ -133,16 +132,20 @@ def check_args(what: str, q, k, pos, freqs, wq, wk, eps: float):
 def kernel_weights(wq, wk):
     """(wq, wk, type code) as the kernels read them: the fp32 master copy of a model parameter, else the tensor itself;
     of two types, both in fp32"""
-    if wq is None and wk is None:
+    w = wk if wq is None else wq
+    if w is None:
         return None, None, 0
     if hasattr(wq, "master") or hasattr(wk, "master"):
         wq, wk = _param32(wq), _param32(wk)
-    types = {w.dtype for w in (wq, wk) if w is not None}
-    if len(types) > 1 or not types <= _TYPES:
-        wq, wk = (None if w is None else w.float() for w in (wq, wk))
-        types = {torch.float32}
-    wq, wk = (w if w is None or w.is_contiguous() else w.contiguous() for w in (wq, wk))
-    return wq, wk, DTYPES[types.pop()]
+        w = wk if wq is None else wq
+    if w.dtype not in DTYPES or (wk is not None and wk.dtype != w.dtype):
+        wq, wk = (None if x is None else x.float() for x in (wq, wk))
+        w = wk if wq is None else wq
+    if wq is not None and not wq.is_contiguous():
+        wq = wq.contiguous()
+    if wk is not None and not wk.is_contiguous():
+        wk = wk.contiguous()
+    return wq, wk, DTYPES[w.dtype]
 
 
 # ----------------------------------------------------------------------------------------------------------------

@@ -358,6 +358,31 @@ def test_attn_offsets_past_32_bits(cuda):
     assert near(o, ref, half_step(BF) * ref.abs() + err)
 
 
+def test_paged_refusals_gpu(cuda):
+    """what only the kernels cannot do (the rest is refused on the CPU too): types, head widths, places, alignment"""
+    kc, vc, table, ln = make_cache([5, 9], 16, 2, 32, BF, cuda)
+    q = torch.zeros(2, 4, 32, dtype=BF, device=cuda)
+    ok = dict(q=q, k_cache=kc, v_cache=vc, table=table, lens=ln, scale=1.0)
+    paged.paged_attn(**ok)
+    odd = torch.empty(kc.numel() + 1, dtype=BF, device=cuda)[1:].view(kc.shape)
+    k48, v48 = paged.page_pools(3, 16, 2, 48, BF, cuda)
+    for bad in (dict(q=q.float(), k_cache=kc.float(), v_cache=vc.float()), dict(k_cache=odd), dict(table=table.cpu()),
+                dict(lens=ln.cpu()), dict(k_cache=kc.cpu()), dict(out=torch.empty(2, 4, 32, dtype=BF)),
+                dict(q=torch.zeros(2, 4, 48, dtype=BF, device=cuda), k_cache=k48, v_cache=v48),
+                dict(q=q[:1].expand(70000, 4, 32), table=table[:1].repeat(70000, 1), lens=ln[:1].repeat(70000))):
+        with pytest.raises(L.KernelError):
+            paged.paged_attn(**{**ok, **bad})
+    one = torch.zeros(2, dtype=torch.int32, device=cuda)
+    with pytest.raises(L.KernelError):
+        paged.rotary_append(q, q[:, :2], q[:, :2], odd, vc, one, one.long(), None)
+    with pytest.raises(L.KernelError):
+        paged.append(q[:, :2].double(), q[:, :2].double(), kc.double(), vc.double(), one)
+    with pytest.raises(L.KernelError):
+        paged.page_plan(one, one.cpu(), table, one, one[:1], 16, tokens=2)
+    with pytest.raises(L.KernelError):
+        paged.page_release(torch.ones(2, dtype=torch.bool), one, table, one, one[:1], 16)
+
+
 # ----------------------------------------------------------------------------------------------------------------
 def test_step_graph_and_streams(cuda):
     """decode steps -- plan, append, attend, lengths carried on -- as two captured graphs and eagerly on another stream:
