@@ -11,6 +11,7 @@ serving form that writes keys and values into a paged cache.
 """
 from __future__ import annotations
 
+import functools
 import math
 import typing
 
@@ -224,33 +225,42 @@ class _Rotary(torch.autograd.Function):
             _backward(None, None, gq, gk, dq, dk, None, None, None, None, False, pos, freqs, *ctx.cfg)
             return dq, dk, None, None, None, None, None
         q, k, wq, wk = normed
-        ws = (wq, wk)
-        # model parameters accumulate into their fp32 main gradient; other weights get theirs back in their own type
-        main = any(getattr(w, "main_grad", None) is not None for w in ws if w is not None)
-        dws, kept = [None, None], [True, True]
-        for i, w in enumerate(ws):
+        # model parameters accumulate into their fp32 main gradient; other weights get theirs back, in their own type where
+        # the kernel writes it, else from fp32 (on the CPU fp64 for fp64)
+        main = getattr(wq, "main_grad", None) is not None or getattr(wk, "main_grad", None) is not None
+        one = wq is None or wk is None or wq.dtype == wk.dtype
+        gpu = gq.get_device() >= 0
+
+        def buffer(w):
             if w is None:
-                continue
+                return None, True
             if main:
-                dws[i], kept[i] = _acc_grad(w)
-            elif raw.on_gpu(w) and wt_direct(ws):
-                dws[i], kept[i] = w.new_empty(w.shape), False
-            else:
-                wide = w.dtype == torch.float64 and not raw.on_gpu(w)
-                dws[i] = torch.zeros(w.shape, device=w.device, dtype=torch.float64 if wide else torch.float32)
-                kept[i] = False
-        into = list(dws)
-        if main and wq is not None and wk is not None and dws[0].data_ptr() == dws[1].data_ptr():
-            into[1] = torch.zeros(wk.shape, dtype=torch.float32, device=wk.device)   # one parameter for both
-        _backward(q, k, gq, gk, dq, dk, wq, wk, into[0], into[1], main, pos, freqs, *ctx.cfg)
-        if into[1] is not dws[1]:
-            dws[1].add_(into[1])
-        out = []
-        for w, g, keep in zip(ws, dws, kept):
+                return _acc_grad(w)
+            if gpu and one and w.dtype in DTYPES:
+                return w.new_empty(w.shape), False
+            return w.new_zeros(w.shape, dtype=w.dtype if w.dtype == torch.float64 and not gpu else torch.float32), False
+        dwq, main_q = buffer(wq)
+        dwk, main_k = buffer(wk)
+        into = dwk
+        if main and dwq is not None and dwk is not None and dwq.data_ptr() == dwk.data_ptr():
+            into = torch.zeros_like(dwk)                                   # one parameter for both
+        _backward(q, k, gq, gk, dq, dk, wq, wk, dwq, into, main, pos, freqs, *ctx.cfg)
+        if into is not dwk:
+            dwk.add_(into)
+        for w in (wq, wk):
             if w is not None:
                 _done(w)
-            out.append(None if w is None or keep else g if g.dtype == w.dtype else g.to(w.dtype))
-        return dq, dk, out[0], out[1], None, None, None
+        if not main_q and dwq.dtype != wq.dtype:
+            dwq = dwq.to(wq.dtype)
+        if not main_k and dwk.dtype != wk.dtype:
+            dwk = dwk.to(wk.dtype)
+        return dq, dk, None if main_q else dwq, None if main_k else dwk, None, None, None
+
+
+@functools.lru_cache(None)
+def _part(D: int) -> int:
+    """floats of the weight sums' workspace"""
+    return L.lib().obst_rotary_part(D)
 
 
 def _backward(q, k, gq, gk, dq, dk, wq, wk, dwq, dwk, add: bool, pos, freqs, rot, T, inter, mscale, eps):
@@ -262,7 +272,7 @@ def _backward(q, k, gq, gk, dq, dk, wq, wk, dwq, dwk, add: bool, pos, freqs, rot
             if d is not None:
                 dw.add_(d.reshape(dw.shape))
         return
-    gs, lib = gq.shape, L.lib()
+    gs = gq.shape
     gq, gq_ts, gq_hs = tokens_view(gq)
     gk, gk_ts, gk_hs = tokens_view(gk)
     q_ts = q_hs = k_ts = k_hs = wt = dt = 0
@@ -270,19 +280,14 @@ def _backward(q, k, gq, gk, dq, dk, wq, wk, dwq, dwk, add: bool, pos, freqs, rot
     if q is not None:
         q, q_ts, q_hs = tokens_view(q)
         k, k_ts, k_hs = tokens_view(k)
-        part = gq.new_empty(lib.obst_rotary_part(gs[-1]), dtype=torch.float32)
+        part = gq.new_empty(_part(gs[-1]), dtype=torch.float32)
         wq, wk, wt = kernel_weights(wq, wk)
         dt = DTYPES[(dwk if dwq is None else dwq).dtype]
-    L.launch(lib.obst_rotary_bwd, gq, "rotary_bwd", L.ROT_DESC.pack(
+    L.launch(L.lib().obst_rotary_bwd, gq, "rotary_bwd", L.ROT_DESC.pack(
         L.ptr(q), L.ptr(k), 0, gq.data_ptr(), gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), 0, L.ptr(wq), L.ptr(wk),
         L.ptr(freqs), pos.data_ptr(), 0, L.ptr(part), L.ptr(dwq), L.ptr(dwk), q_ts, q_hs, k_ts,
         k_hs, 0, 0, gq_ts, gq_hs, gk_ts, gk_hs, T, 0, gs[-2], gk.shape[-2], gs[-1], rot, inter, DTYPES[gq.dtype], wt, dt,
         add, 0, mscale, eps))
-
-
-def wt_direct(ws) -> bool:
-    """both weights of one kernel type: the kernel writes their gradients in it"""
-    return len({w.dtype for w in ws if w is not None}) == 1 and all(w is None or w.dtype in DTYPES for w in ws)
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, freqs: typing.Optional[torch.Tensor],
