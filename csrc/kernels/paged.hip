@@ -24,6 +24,7 @@ struct PagedDesc {
   float* part;                         // partial outputs [B][Hq][nsplit][D], then maxima and sums [B][Hq][nsplit][2]
   long long q_bs, q_hs;                // strides of q's batch and head, in elements
   int B, Hq, Hk, D, P, cap, ld, shift, dtype, nsplit, split;   // cap: lengths count up to it; page = 1 << shift
+  int most;                            // > 0: splits grow from `split` until all tokens together make at most so many
   float scale;
 };
 
@@ -243,6 +244,11 @@ template <> struct Mat<2> {
 // and what that rounding left), so the weights keep at least 16 bits. Waves, then splits, are joined by their maxima
 // and sums.
 //
+// Blocks are ordered by key head, request, split, and the requests turn by one with each split. With the split first,
+// the blocks that have work in a table much wider than its requests' lengths all met one XCD (16 requests of 1 to 2000
+// tokens, 64 splits: 175 us, 24 now); without the turn the splits of one long request among short ones met the same CUs
+// (120000 tokens among 63 short: 239 us, 135 now).
+//
 // Keys past the length, and pages whose id is not one, have weight 0 and a value of 0 whatever the cache holds there.
 //
 // Bound by the read of the cache. V goes past the caches: a load takes whole lines of it. K's loads take half a line
@@ -250,6 +256,21 @@ template <> struct Mat<2> {
 // key heads x 128, 4 query heads each (1.6 GB): 258 us, 6.2 TB/s, where a bare read of such data reaches 7.1.
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG = -3.0e38f;                   // a running maximum before any key
+
+// tokens a split of this call. `most` > 0 (only for few requests): it follows from the lengths that the requests have,
+// which the host does not know, so that a table much wider than they are costs nothing. No request then has more than
+// `most` splits: ceil(a / ceil(n / most)) <= most for its share a of all n
+constexpr int MAX_SUM = 16;
+
+__device__ __forceinline__ int split_of(const PagedDesc& d) {
+  if (d.most == 0) return d.split;
+  const int lane = threadIdx.x & 63;
+  int n = lane < d.B ? (min(max(d.lens[lane], 0), d.cap) + 127) >> 7 : 0;   // units of 128 tokens, below 2^28
+#pragma unroll
+  for (int o = MAX_SUM / 2; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+  n = __builtin_amdgcn_readfirstlane(n);
+  return max(d.split, min((n + d.most - 1) / d.most, 1 << 23) * 128);
+}
 
 template <int TYPE, int D>
 __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
@@ -259,12 +280,12 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   // [NW][query heads of the block][D + 4]: one head's 2 KB leave room for four blocks a CU, 16 heads' for three
   extern __shared__ float sacc[];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-  const int G = d.Hq / d.Hk, ng = (G + 15) / 16;
-  const int hk = blockIdx.y / ng, gi = blockIdx.y % ng, b = blockIdx.z, sp = blockIdx.x;
+  const int sp = blockIdx.z, b = (blockIdx.y + blockIdx.z) % gridDim.y;
+  const int len = min(max(d.lens[b], 0), d.cap), split = split_of(d);
+  if (sp > 0 && (long long)sp * split >= len) return;
+  const int k0 = sp * split, k1 = min(len, k0 + split);
+  const int G = d.Hq / d.Hk, gi = blockIdx.x / d.Hk, hk = blockIdx.x % d.Hk;
   const int h0 = hk * G + gi * 16, gc = min(16, G - gi * 16);
-  const int len = min(max(d.lens[b], 0), d.cap);
-  const int k0 = sp * d.split, k1 = min(len, k0 + d.split);
-  if (k0 >= k1 && sp > 0) return;
 
   const uint16_t* qp = (const uint16_t*)d.q + b * d.q_bs + (long long)(h0 + min(n, gc - 1)) * d.q_hs + 8 * g;
   vec q[NK];
@@ -366,7 +387,7 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
     for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[(w * gc + n) * (D + 4) + 16 * j + 4 * g]) = acc[j];
   }
   __syncthreads();
-  const bool whole = len <= d.split;
+  const bool whole = len <= split;
   for (int e = threadIdx.x; e < gc * D; e += NTH) {
     const int h = e / D, i = e % D;
     float M = sm[0][h], L = 0.f, o = 0.f;
@@ -400,9 +421,9 @@ __global__ __launch_bounds__(NTH) void paged_join_few_kernel(const PagedDesc d) 
   const long long u = (long long)blockIdx.x * (NTH / 64) + (threadIdx.x >> 6);
   if (u >= (long long)d.B * d.Hq) return;
   const int lane = threadIdx.x & 63;
-  const int len = min(max(d.lens[u / d.Hq], 0), d.cap);
-  if (len <= d.split) return;
-  const int ns = (len + d.split - 1) / d.split;
+  const int len = min(max(d.lens[u / d.Hq], 0), d.cap), split = split_of(d);
+  if (len <= split) return;
+  const int ns = (len + split - 1) / split;
   const float* ml = d.part + (long long)d.B * d.Hq * d.nsplit * D + u * d.nsplit * 2;
   const float* pt = d.part + u * d.nsplit * D;
   constexpr int R = (D + 63) / 64;                   // dims lane, lane + 64, ...
@@ -445,9 +466,9 @@ __global__ __launch_bounds__(NTH) void paged_join_kernel(const PagedDesc d) {
   __shared__ float wt[MAX_SPLITS], red[2][NTH / 64];
   __shared__ f32x4_t so[NTH];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int len = min(max(d.lens[b], 0), d.cap);
-  if (len <= d.split) return;
-  const int ns = (len + d.split - 1) / d.split;
+  const int len = min(max(d.lens[b], 0), d.cap), split = split_of(d);
+  if (len <= split) return;
+  const int ns = (len + split - 1) / split;
   const long long at = ((long long)b * d.Hq + h) * d.nsplit;
   const float* ml = d.part + (long long)d.B * d.Hq * d.nsplit * d.D + at * 2;
   float M = NEG;
@@ -487,7 +508,7 @@ __global__ __launch_bounds__(NTH) void paged_join_kernel(const PagedDesc d) {
 template <int TYPE, int D>
 int attn_of(const PagedDesc& d, hipStream_t st) {
   const int G = d.Hq / d.Hk, ng = (G + 15) / 16, gc = G < 16 ? G : 16;
-  hipLaunchKernelGGL((paged_attn_kernel<TYPE, D>), dim3(d.nsplit, d.Hk * ng, d.B), dim3(NTH),
+  hipLaunchKernelGGL((paged_attn_kernel<TYPE, D>), dim3(d.Hk * ng, d.B, d.nsplit), dim3(NTH),
                      NTH / 64 * gc * (D + 4) * sizeof(float), st, d);
   const int rc = (int)hipGetLastError();
   if (rc || d.nsplit == 1) return rc;
@@ -535,7 +556,8 @@ OBST_API int obst_paged_attn(const PagedDesc* d, hipStream_t st) {
       d->nsplit < 1 || d->nsplit > MAX_SPLITS || d->split < 32 || d->split % 32 || (d->nsplit > 1 && !d->part))
     return -1;
   if (d->shift < 4 || d->shift > 8 || (long long)d->ld << d->shift < d->cap) return -3;
-  if (d->cap > (long long)d->nsplit * d->split) return -4;
+  if (d->most < 0 || (d->most > 0 && (d->B > MAX_SUM || d->split % 128))) return -6;
+  if (d->cap > (long long)d->nsplit * d->split && (d->most == 0 || d->nsplit < d->most)) return -4;
   if (d->dtype == 1) return attn<1>(*d, st);
   if (d->dtype == 2) return attn<2>(*d, st);
   return -5;

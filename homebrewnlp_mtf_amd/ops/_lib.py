@@ -88,7 +88,7 @@ class OptDesc(ctypes.Structure):
 # fill, this 0.4): field order and types of the C structs in csrc/kernels/rotary.hip and paged.hip, natural alignment
 ROT_DESC = struct.Struct("@16P12q10i2f")      # RotDesc
 PLAN_DESC = struct.Struct("@10P6i")           # PlanDesc
-PAGED_DESC = struct.Struct("@7P2q11if")     # PagedDesc
+PAGED_DESC = struct.Struct("@7P2q12if")     # PagedDesc
 
 
 _SIGS = {

@@ -288,8 +288,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
 
         out[b, h] = softmax_j(scale * q[b, h] . k_j) @ v,  j < min(lens[b], max_len);  0 for a request without tokens
 
-    ``max_len`` (default: what the table's width holds) is a bound on lens that the host knows; it sizes the launch, so
-    a close one helps a wide table. A page id outside the pool hides its tokens. What the cache holds behind a length
+    ``max_len`` (default: what the table's width holds) is a bound on lens that the host knows; a close one spares a wide
+    table some empty blocks and workspace. A page id outside the pool hides its tokens. What the cache holds behind a length
     is never looked at. No gradient."""
     qs, dev = q.shape, q.get_device()
     if len(qs) != 3 or qs[1] < 1 or qs[2] < 1:
@@ -324,12 +324,12 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
         if q_ds != 1 or (q_bs | q_hs) % 8 or q.data_ptr() % 16:
             q = q.clone(memory_format=torch.contiguous_format)
             q_bs, q_hs = Hq * D, D
-        nsplit, split = _splits(B, B * rows, cap)
+        nsplit, split, most = _splits(B, rows, cap)
         part = q.new_empty(B * Hq * nsplit * (D + 2), dtype=torch.float32) if nsplit > 1 else None
         L.launch(L.lib().obst_paged_attn, q, "paged_attn", L.PAGED_DESC.pack(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), table.data_ptr(), lens.data_ptr(),
             L.ptr(part), q_bs, q_hs, B, Hq, Hk, D, P, cap, ld, page.bit_length() - 1, DTYPES[q.dtype], nsplit, split,
-            scale))
+            most, scale))
         return out
     # ---- torch oracle
     G = Hq // Hk
@@ -349,16 +349,22 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     return out
 
 
-def _splits(B: int, rows: int, cap: int) -> typing.Tuple[int, int]:
-    """(splits, tokens a split) of the length for ``rows`` blocks of ``B`` requests without one.
+def _splits(B: int, rows: int, cap: int) -> typing.Tuple[int, int, int]:
+    """(splits of the length, tokens a split, ``most``) for B requests of ``rows`` blocks each without a split.
 
-    Up to 8 requests: two blocks a CU, at least 256 tokens each (one request's 4 rows of 131072 tokens take 44 us + 5 to join in
-    512 blocks, 47 + 6.5 in 1024, 50 + 9.5 in 2048). More requests differ in length and leave about half of the splits
-    empty: four blocks a CU, at least 384 tokens each (40 requests of 1 to 4000 tokens, 2 key heads: 24 us, 31 in two; 200 of
-    1 to 2000, 1 head: 28, 35). At most 2048 tokens a split, so that one long request among short ones is spread as well; at most
-    1024 splits (csrc/kernels/paged.hip MAX_SPLITS)."""
-    blocks, least = (512, 256) if B <= 8 else (1024, 384)
-    want = max(1, -(-blocks // rows))
-    split = max(min(max(least, -(-cap // want)), 2048), -(-cap // 1024))
+    Up to 16 requests (``most`` > 0): the kernel sizes the splits from the lengths it finds, at least 256 tokens each and
+    two blocks a CU from all of them, so no request has more than ``most`` splits and the table's width hardly matters
+    (8 requests of 1 to 2000 tokens, 8 key heads: 12.8 us in a table of 2000, 13.9 in one of 131072; one of 131072, 4 key
+    heads: 47 us, 49 in four blocks a CU). More requests would start too many empty blocks that way (32 of 1 to 2000 in a
+    table of 131072: 42 us, 33 by the width), so the width decides: four blocks a CU, 384 to 2048 tokens a split (64 of
+    6144, 8 key heads: 248 us, 273 in splits of 512; 200 of 1 to 2000, 1 key head: 28 us, 35 in two blocks a CU), and
+    longer splits where that makes more than 65536 blocks (1000 of 1 to 500 in a table of 131072: 209 us, 397 in splits
+    of 2048; 256, one of them of 120000: 209, 170). At most 1024 splits (csrc/kernels/paged.hip MAX_SPLITS)."""
+    if B <= 16:
+        most, split = max(1, 512 // rows), max(256, -(-cap // 1024))
+    else:
+        most, split = 0, max(384, min(-(-cap * rows * B // 1024), 2048), -(-cap // max(1, 65536 // (B * rows))),
+                             -(-cap // 1024))
     split = -(-split // 128) * 128
-    return max(1, -(-cap // split)), split
+    n = max(1, -(-cap // split))
+    return min(n, most) if most else n, split, most

@@ -287,6 +287,26 @@ def test_attn(cuda, Hq, Hk, D, page, lens, dtype):
             assert n or bool((o[b] == 0).all())
 
 
+@pytest.mark.parametrize("Hq,Hk,lens,W", [
+    (8, 2, [3000], 2000),                                    # one request in a table of 32000 tokens
+    (8, 8, [1, 9000, 0, 17, 300, 128, 129, 2], 4096),        # a long one among short ones: splits sized by the kernel
+    (4, 1, [700] * 15 + [20000], 4096),
+    (4, 1, [700] * 16 + [20000], 4096),                      # one request more: sized by the width
+    (64, 64, [1500, 5], 1024),
+    (600, 600, [400, 0, 1000], 512),                         # more heads than blocks asked for: no split
+])
+def test_attn_wide_tables(cuda, Hq, Hk, lens, W):
+    """a table much wider than its requests, and lengths that differ much"""
+    D, page = 64, 16
+    kc, vc, table, ln = make_cache(lens, page, Hk, D, BF, cuda, seed=Hq, W=W)
+    q = torch.randn(len(lens), Hq, D, device=cuda, generator=gen(cuda, 3)).to(BF)
+    ref, err = attn64(q, kc, vc, table, ln, D ** -0.5)
+    tol = half_step(BF) * ref.abs() + err
+    a = paged.paged_attn(q, kc, vc, table, ln, D ** -0.5)
+    assert near(a, ref, tol) and near(paged.paged_attn(q, kc, vc, table, ln, D ** -0.5, max_len=max(lens)), ref, tol)
+    assert torch.equal(a, paged.paged_attn(q, kc, vc, table, ln, D ** -0.5))
+
+
 def test_attn_hidden_ids_bounds_strides(cuda):
     lens = [70, 33, 16, 200, 500]
     kc, vc, table, ln = make_cache(lens, 16, 2, 64, BF, cuda, seed=5)

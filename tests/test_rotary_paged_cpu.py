@@ -417,8 +417,17 @@ def test_trainer_steps_with_rotary_attention():
 
 
 def test_splits_cover_every_length():
-    for B in (1, 3, 8, 9, 200, 60000):
-        for heads in (1, 4, 20, 64):
+    rng = random.Random(3)
+    for B in (1, 3, 8, 16, 17, 200, 60000):
+        for rows in (1, 4, 20, 64, 1000):
             for cap in (0, 1, 16, 255, 256, 257, 2048, 4097, 131072, 2 ** 21 + 1, 2 ** 30):
-                n, split = paged._splits(B, B * heads, cap)
-                assert 1 <= n <= 1024 and split % 128 == 0 and (n - 1) * split < max(cap, 1) <= n * split
+                n, split, most = paged._splits(B, rows, cap)
+                assert 1 <= n <= 1024 and split % 128 == 0
+                if not most:
+                    assert (n - 1) * split < max(cap, 1) <= n * split
+                    continue
+                # the kernel's own size for these lengths: no request needs more than n
+                for lens in ([cap] * B, [cap] + [0] * (B - 1), [rng.randint(0, cap) for _ in range(B)]):
+                    units = sum(-(-x // 128) for x in lens)
+                    s = max(split, min(-(-units // most), 2 ** 23) * 128)
+                    assert s < 2 ** 31 and all(-(-x // s) <= n for x in lens)
