@@ -33,8 +33,8 @@ constexpr int NTH = 256;
 
 // ---- block tables and slot maps
 // Requests are served in order. Request b holds c tokens in ceil(c / page) pages and wants n more. It is refused -- no
-// slots, its length stays -- where its pages pass the table's width, its tokens pass the step's buffer, or the pages
-// asked for up to and including it pass the stack. Its i-th new page is the stack's entry nfree - 1 - (pages asked for
+// slots, its length stays -- where its pages pass the table's width, its length 31 bits, its tokens the step's buffer,
+// or the pages asked for up to and including it the stack. Its i-th new page is the stack's entry nfree - 1 - (pages asked for
 // before it) - i. Sums over the requests before b are all that a group needs, so every block forms them itself from
 // the lengths (a few KB out of the caches) and one launch does it all: the call's latency is what matters here.
 //
@@ -50,7 +50,7 @@ __device__ __forceinline__ Want want_of(const PlanDesc& d, int b, int& c) {
   c = max(d.cached[b], 0);
   const int n = max(d.nnew[b], 0);
   const unsigned old = pages_of(c, d.page), all = pages_of((unsigned)c + n, d.page);   // c + n < 2^32
-  const bool fits = all <= (unsigned)d.W;
+  const bool fits = all <= (unsigned)d.W && (unsigned)c + n <= 0x7fffffffu;
   return {n, fits ? all - old : 0, fits};
 }
 
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(NTH) void page_plan_kernel(const PlanDesc d) {
 __global__ __launch_bounds__(1024) void page_release_kernel(const unsigned char* __restrict__ done, int* lens,
                                                            const int* __restrict__ table, int* stack, int* nfree, int B,
                                                            int W, int ld, int page, int P) {
-  __shared__ int cnt[1024];
+  __shared__ long long cnt[1024];                 // pages of 1024 rows as wide as memory holds pass 31 bits
   __shared__ int base;
   const int tid = threadIdx.x, lane = tid & 63;
   if (tid == 0) base = min(max(*nfree, 0), P);
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(1024) void page_release_kernel(const unsigned char*
     cnt[tid] = n;
     __syncthreads();
     for (int o = 1; o < 1024; o <<= 1) {          // inclusive prefix sums
-      const int v = tid >= o ? cnt[tid - o] : 0;
+      const long long v = tid >= o ? cnt[tid - o] : 0;
       __syncthreads();
       cnt[tid] += v;
       __syncthreads();
@@ -198,12 +198,11 @@ __global__ __launch_bounds__(1024) void page_release_kernel(const unsigned char*
     // one wave a request: 16 waves copy the rows of the piece
     const int at0 = base;
     for (int r = tid >> 6; r < 1024 && b0 + r < B; r += 16) {
-      const int e = r ? cnt[r - 1] : 0, m = cnt[r] - e;
-      for (int i = lane; i < m; i += 64)
-        if ((long long)at0 + e + i < P) stack[at0 + e + i] = table[(long long)(b0 + r) * ld + i];
+      const long long e = r ? cnt[r - 1] : 0, m = min(cnt[r] - e, P - at0 - e);   // what the stack has room for
+      for (long long i = lane; i < m; i += 64) stack[at0 + e + i] = table[(long long)(b0 + r) * ld + i];
     }
     __syncthreads();
-    if (tid == 0) base = (int)min((long long)at0 + cnt[1023], (long long)P);
+    if (tid == 0) base = (int)min(at0 + cnt[1023], (long long)P);
   }
   __syncthreads();
   if (tid == 0) *nfree = base;

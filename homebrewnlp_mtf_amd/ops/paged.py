@@ -82,8 +82,8 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
     of ``tokens`` places. New pages come off the top of ``stack`` (int32 [P], ``nfree`` int32 [1] of them unused) and
     are entered into ``table`` (int32 [B, W]) in place.
 
-    Requests are served in order. One is refused -- no slots, its length unchanged -- if its pages pass W, its tokens
-    the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request that needs no new
+    Requests are served in order. One is refused -- no slots, its length unchanged -- if its pages pass W, its length
+    31 bits, its tokens the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request that needs no new
     page goes on). ``cached`` and ``nfree`` are not written: the plan holds their new values, and the same call again
     gives the same plan. ``out`` must not share memory with them."""
     dev, B = cached.get_device(), cached.numel()
@@ -125,7 +125,7 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
     for b, (c, n) in enumerate(zip(cached.clamp(min=0).tolist(), new.clamp(min=0).tolist())):
         out.start[b] = min(at, 2 ** 31 - 1)
         old, want = -(-c // page), -(-(c + n) // page)
-        ok = want <= W and at + n <= T
+        ok = want <= W and c + n < 2 ** 31 and at + n <= T
         if ok:
             asked += want - old
             ok = want == old or asked <= avail

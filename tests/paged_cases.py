@@ -3,6 +3,8 @@ import math
 
 import torch
 
+from homebrewnlp_mtf_amd.ops import paged
+
 U32 = 2.0 ** -24          # half a step of fp32, relative
 
 
@@ -121,3 +123,17 @@ def plan_loop(cached, new, table, stack, nfree, page, T):
                     slots[at + i] = p * page + (c + i) % page if 0 <= p < P else -1
         at += n
     return slots, pos, start + [at], lens, left, table
+
+
+def past_31_bits(device):
+    """a length that would pass 31 bits is refused, one that just fits is not"""
+    def i32(*v):
+        return torch.tensor(v, dtype=torch.int32, device=device)
+    top = 2 ** 31 - 1
+    for new, ok in ((9, True), (10, False)):
+        cached, table, stack = i32(top - 9, 3), i32(0, 0, 0, 0, 0, 0).reshape(2, 3), i32(0)
+        plan = paged.page_plan(cached, i32(new, 2), table, stack, i32(1), 2 ** 30, tokens=12)
+        n = 2 ** 30 - 10                       # offset of the first new token in the second page, whose id is 0
+        assert plan.lens.tolist() == [top if ok else top - 9, 5] and plan.nfree.tolist() == [1]
+        assert plan.slots.tolist() == ([n + i for i in range(9)] if ok else [-1] * 10) + [3, 4] + [-1] * (10 - new)
+        assert plan.start.tolist() == [0, new, new + 2]

@@ -7,7 +7,7 @@ import torch
 
 from homebrewnlp_mtf_amd.ops import _lib as L
 from homebrewnlp_mtf_amd.ops import paged, rotary
-from paged_cases import U32, attn64, half_step, make_cache, plan_loop, rotary64, rotary_grad64
+from paged_cases import U32, attn64, half_step, make_cache, past_31_bits, plan_loop, rotary64, rotary_grad64
 from test_rotary_paged_cpu import random_plan, run_plan
 
 pytestmark = pytest.mark.gpu
@@ -193,6 +193,23 @@ def test_plan_strided_table_and_overflow(cuda):
     p = paged.page_plan(i([0, 0, 3]), i([0, 20, 1]), table, i([5, 4, 3, 2, 1, 0]), i([6]), 16, tokens=50)
     assert wide[1, 2:4].tolist() == [0, 1] and bool((wide[:, :2] == -7).all()) and bool((wide[:, 6:] == -7).all())
     assert p.lens.tolist() == [0, 20, 4] and int(p.nfree) == 4
+
+
+def test_plan_refuses_lengths_past_31_bits(cuda):
+    past_31_bits(cuda)
+
+
+def test_release_more_pages_than_31_bits(cuda):
+    """1024 rows of 2^21 + 1 pages each: the stack takes what it has room for, what lies behind it stays"""
+    B, W, P = 1024, 2 ** 21 + 1, 1000
+    table = torch.zeros(B, W, dtype=torch.int32, device=cuda)
+    table[0, :P] = torch.arange(P, device=cuda).int() + 7
+    room = torch.full((P + 64,), -5, dtype=torch.int32, device=cuda)
+    lens = torch.full((B,), W, dtype=torch.int32, device=cuda)
+    nfree = torch.tensor([10], dtype=torch.int32, device=cuda)
+    paged.page_release(torch.ones(B, dtype=torch.bool, device=cuda), lens, table, room[:P], nfree, 1)
+    assert nfree.tolist() == [P] and bool((lens == 0).all())
+    assert room.tolist() == [-5] * 10 + [i + 7 for i in range(P - 10)] + [-5] * 64
 
 
 def test_release(cuda):

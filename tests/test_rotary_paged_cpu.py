@@ -8,7 +8,7 @@ import torch
 
 from homebrewnlp_mtf_amd.ops import _lib as L
 from homebrewnlp_mtf_amd.ops import paged, rotary
-from paged_cases import U32, attn64, half_step, make_cache, plan_loop, rotary64, rotary_grad64
+from paged_cases import U32, attn64, half_step, make_cache, past_31_bits, plan_loop, rotary64, rotary_grad64
 
 
 @pytest.mark.parametrize("inter", [False, True])
@@ -144,6 +144,10 @@ def test_plan_oracle():
     for _ in range(60):
         c = random_plan(r)
         assert run_plan("cpu", *c) == tuple(plan_loop(*c)), c
+
+
+def test_plan_refuses_lengths_past_31_bits():
+    past_31_bits("cpu")
 
 
 def test_plan_and_release_refusals():
