@@ -214,7 +214,9 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
     if len(qs) != 3 or v.shape != ks or v.dtype != q.dtype or v.get_device() != dev:
         raise L.KernelError(f"rotary_append: q [T, Hq, D], k and v [T, Hk, D] of one type, got {list(qs)}, {list(ks)}, "
                             f"{list(v.shape)}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_cache.requires_grad
+                                    or v_cache.requires_grad or (q_weight is not None and q_weight.requires_grad)
+                                    or (k_weight is not None and k_weight.requires_grad)):
         raise L.KernelError("rotary_append has no gradient: call it under torch.no_grad()")
     _, Hq, D = qs
     P, Hk, page = _pools("rotary_append", k_cache, v_cache, q, dev, D, ks[1])
@@ -250,7 +252,7 @@ def append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise L.KernelError(f"append: k and v [T, Hk, D] of one type, D up to {MAX_DIM}, got {list(ks)}, {list(v.shape)}")
     if dev >= 0 and k.dtype not in DTYPES:
         raise L.KernelError(f"append: bf16, fp16 or fp32 on the GPU, got {k.dtype}")
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise L.KernelError("append has no gradient: call it under torch.no_grad()")
     T, Hk, D = ks
     P, Hk, page = _pools("append", k_cache, v_cache, k, dev, D, Hk)

@@ -225,6 +225,7 @@ def test_append_oracle_and_refusals():
     for bad in (dict(v=v[:4]), dict(v=v.double()), dict(slots=slots.long()), dict(slots=slots[:4]), dict(k=k[:, :1]),
                 dict(k_cache=kc.double()), dict(v_cache=vc[:2]), dict(k_cache=kc[:, :1]), dict(pos=pos[:4]),
                 dict(k_cache=kc.transpose(0, 1)), dict(q=q.clone().requires_grad_()), dict(out=q[:3]),
+                dict(k_weight=w.clone().requires_grad_()), dict(v_cache=vc.clone().requires_grad_()),
                 dict(q=q.unsqueeze(0), k=k.unsqueeze(0), v=v.unsqueeze(0))):
         with pytest.raises(L.KernelError):
             paged.rotary_append(**{**args, **bad})
