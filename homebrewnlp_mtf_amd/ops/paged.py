@@ -83,9 +83,9 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
     are entered into ``table`` (int32 [B, W]) in place.
 
     Requests are served in order. One is refused -- no slots, its length unchanged -- if its pages pass W, its length
-    31 bits, its tokens the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request that needs no new
-    page goes on). ``cached`` and ``nfree`` are not written: the plan holds their new values, and the same call again
-    gives the same plan. ``out`` must not share memory with them."""
+    31 bits, its tokens the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request
+    that needs no new page goes on). ``cached`` and ``nfree`` are not written: the plan holds their new values, and
+    the same call again gives the same plan. ``out`` must not share memory with them."""
     dev, B = cached.get_device(), cached.numel()
     _ints("page_plan", dev, ("cached", cached), ("new", new), ("stack", stack), ("nfree", nfree))
     if cached.dim() != 1 or B < 1 or new.shape != cached.shape or nfree.numel() != 1 or stack.dim() != 1:
@@ -248,7 +248,8 @@ def append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """keys and values [T, Hk, D] as they are into the cache at ``slots`` (as ``rotary_append`` writes them): for prompts
     whose turned keys their own attention has read"""
     ks, dev = k.shape, k.get_device()
-    if len(ks) != 3 or v.shape != ks or v.dtype != k.dtype or v.get_device() != dev or ks[1] < 1 or not 1 <= ks[2] <= MAX_DIM:
+    if len(ks) != 3 or v.shape != ks or v.dtype != k.dtype or v.get_device() != dev or ks[1] < 1 \
+            or not 1 <= ks[2] <= MAX_DIM:
         raise L.KernelError(f"append: k and v [T, Hk, D] of one type, D up to {MAX_DIM}, got {list(ks)}, {list(v.shape)}")
     if dev >= 0 and k.dtype not in DTYPES:
         raise L.KernelError(f"append: bf16, fp16 or fp32 on the GPU, got {k.dtype}")
