@@ -355,16 +355,20 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
 def _splits(B: int, rows: int, cap: int) -> typing.Tuple[int, int, int]:
     """(splits of the length, tokens a split, ``most``) for B requests of ``rows`` blocks each without a split.
 
-    Up to 16 requests (``most`` > 0): the kernel sizes the splits from the lengths it finds, at least 256 tokens each and
-    two blocks a CU from all of them, so no request has more than ``most`` splits and the table's width hardly matters
-    (8 requests of 1 to 2000 tokens, 8 key heads: 12.8 us in a table of 2000, 13.9 in one of 131072; one of 131072, 4 key
-    heads: 47 us, 49 in four blocks a CU). More requests would start too many empty blocks that way (32 of 1 to 2000 in a
-    table of 131072: 42 us, 33 by the width), so the width decides: four blocks a CU, 384 to 2048 tokens a split (64 of
-    6144, 8 key heads: 248 us, 273 in splits of 512; 200 of 1 to 2000, 1 key head: 28 us, 35 in two blocks a CU), and
-    longer splits where that makes more than 65536 blocks (1000 of 1 to 500 in a table of 131072: 209 us, 397 in splits
-    of 2048; 256, one of them of 120000: 209, 170). At most 1024 splits (csrc/kernels/paged.hip MAX_SPLITS)."""
+    Up to 16 requests (``most`` > 0): the kernel sizes the splits from the lengths it finds, at least 256 tokens each
+    and three blocks a CU from all of them, so no request has more than ``most`` splits and the table's width hardly
+    matters (8 requests of 1 to 2000 tokens, 8 key heads: 12.8 us in a table of 2000, 13.9 in one of 131072; 4 of 1 to
+    30000: 46 us, 53 in two blocks a CU, 49 in four; one of 131072, 4 key heads: 48, 47, 48). A table so narrow that
+    its splits are the shortest either way spares the kernel that sum, 0.6 us.
+
+    More requests would start too many empty blocks that way (32 of 1 to 2000 in a table of 131072: 42 us, 33 by the
+    width), so the width decides: four blocks a CU, 384 to 2048 tokens a split (64 of 6144, 8 key heads: 248 us, 273
+    in splits of 512; 200 of 1 to 2000, 1 key head: 28 us, 35 in two blocks a CU), and longer splits where that makes
+    more than 65536 blocks (1000 of 1 to 500 in a table of 131072: 209 us, 397 in splits of 2048; 256, one of them of
+    120000: 209, 170). At most 1024 splits (csrc/kernels/paged.hip MAX_SPLITS)."""
     if B <= 16:
-        most, split = max(1, 512 // rows), max(256, -(-cap // 1024))
+        most = max(1, 768 // rows) if cap * rows * B > 768 * 256 else 0
+        split = max(256, -(-cap // 1024))
     else:
         most, split = 0, max(384, min(-(-cap * rows * B // 1024), 2048), -(-cap // max(1, 65536 // (B * rows))),
                              -(-cap // 1024))
