@@ -245,8 +245,8 @@ template <> struct Mat<2> {
 //
 // Blocks are ordered by key head, request, split, and the requests turn by one with each split. With the split first,
 // the blocks that have work in a table much wider than its requests' lengths all met one XCD (16 requests of 1 to 2000
-// tokens, 64 splits: 175 us, 24 now); without the turn the splits of one long request among short ones met the same CUs
-// (120000 tokens among 63 short: 239 us, 135 now).
+// tokens, 64 splits of 2048: 175 us, 24 in this order); without the turn the splits of one long request among short
+// ones met the same CUs (120000 tokens among 63 short: 239 us, 135 with it).
 //
 // Keys past the length, and pages whose id is not one, have weight 0 and a value of 0 whatever the cache holds there.
 //
