@@ -356,7 +356,7 @@ def run(state):
         return [qo.detach(), ko.detach(), dq, dwq, dk, dwk]
     if c["op"] == "plan":
         p = paged.page_plan(s["cached"], s["new"], s["table"], s["free"], s["nfree"], c["page"], out=s["out"])
-        return {"slots": p.slots, "pos": p.pos, "start": p.start, "lens": p.lens, "nfree": p.nfree,
+        return {"slots": p.slots, "pos": p.pos, "start": p.start, "lens": p.lens, "nfree": p.nfree[0],
                 "table": s["table"]}
     if c["op"] == "append":
         qo = paged.rotary_append(s["q"], s["k"], s["v"], s["kc"], s["vc"], s["slots"], s["pos"], s["freqs"],
