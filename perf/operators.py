@@ -177,7 +177,9 @@ def prepare(case, seed):
                  tokens=_cdiv(sum(new) + 1, 64) * 64)
         if own:
             from homebrewnlp_mtf_amd.ops import paged
-            s["out"] = paged.plan_buffers(c["B"], s["tokens"], DEV)
+            buf = paged.plan_buffers(c["B"], s["tokens"], DEV)
+            # run returns the first row of the height's buffer: [1], as the plain form has it
+            s["out"] = buf._replace(nfree=buf.nfree.view(1, 1))
         return s
     dt = TYPES[c["dtype"]]
     D, Hq, Hk = c["D"], c["Hq"], c["Hk"]
