@@ -215,6 +215,7 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 template <int TYPE> struct Mat;
 template <> struct Mat<1> {
   typedef bf16x8_t v;
+  static constexpr float UNIT = 1.f;
   static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -223,6 +224,7 @@ template <> struct Mat<1> {
 };
 template <> struct Mat<2> {
   typedef f16x8_t v;
+  static constexpr float UNIT = 32768.f;          // the largest power of two in fp16
   static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -240,8 +242,10 @@ template <> struct Mat<2> {
 // still a small part of the loads' (16 x 16-cycle products to 16 KB a tile and wave).
 //
 // Softmax in one pass with the running maximum; P enters the product as two summands of the cache's type (its value
-// and what that rounding left), so the weights keep at least 16 bits. Waves, then splits, are joined by their maxima
-// and sums.
+// and what that rounding left): 16 bits of a weight in bf16. In fp16, which ends at 2^-24, weights count in units of
+// 2^-15 (UNIT; the sum l too, so the quotient is the same): 22 bits of those above 2^-28 of the largest, 2^-40 of it for
+// the smaller ones. (In units of 1, a key 16 nats above 2047 others left these 6 % too heavy, 17.5 nats nothing.)
+// Waves, then splits, are joined by their maxima and sums.
 //
 // Blocks are ordered by key head, request, split, and the requests turn by one with each split. With the split first,
 // the blocks that have work in a table much wider than its requests' lengths all met one XCD (16 requests of 1 to 2000
@@ -366,8 +370,9 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
       for (int e = 0; e < 2; ++e) {
         const float x = __builtin_amdgcn_exp2f(p[2 * i + e] - m);
         l += x;
-        h2[e] = Mat<TYPE>::bits(x);
-        l2[e] = Mat<TYPE>::bits(x - Mat<TYPE>::back(h2[e]));
+        const float u = x * Mat<TYPE>::UNIT;
+        h2[e] = Mat<TYPE>::bits(u);
+        l2[e] = Mat<TYPE>::bits(u - Mat<TYPE>::back(h2[e]));
       }
       hi[i] = h2[0] | (uint32_t)h2[1] << 16;
       lo[i] = l2[0] | (uint32_t)l2[1] << 16;
@@ -380,7 +385,7 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
-  if (g == 0) { sm[w][n] = m; sl[w][n] = l; }
+  if (g == 0) { sm[w][n] = m; sl[w][n] = l * Mat<TYPE>::UNIT; }
   if (n < gc) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[(w * gc + n) * (D + 4) + 16 * j + 4 * g]) = acc[j];
