@@ -215,6 +215,7 @@ typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 template <int TYPE> struct Mat;
 template <> struct Mat<1> {
   typedef bf16x8_t v;
+  static constexpr int PARTS = 3;                 // summands of a softmax weight, and the unit that it counts in
   static constexpr float UNIT = 1.f;
   static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -224,6 +225,7 @@ template <> struct Mat<1> {
 };
 template <> struct Mat<2> {
   typedef f16x8_t v;
+  static constexpr int PARTS = 2;
   static constexpr float UNIT = 32768.f;          // the largest power of two in fp16
   static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -239,13 +241,14 @@ template <> struct Mat<2> {
 // of the two products of a tile is key 8 (m / 4) + 4 t + m % 4, so a lane ends up with the scores of eight
 // neighbouring keys 8 (lane / 16) + 0..7 of one query head: just what the P operand of O^T = V^T P takes from it. P
 // never leaves its lane. With one query head per key head 15 of the 16 columns are idle: the products' time is
-// still a small part of the loads' (16 x 16-cycle products to 16 KB a tile and wave).
+// still a small part of the loads' (32 products in bf16 to 16 KB a tile and wave, heads of 128: 8 for S, 24 for O).
 //
-// Softmax in one pass with the running maximum; P enters the product as two summands of the cache's type (its value
-// and what that rounding left): 16 bits of a weight in bf16. In fp16, which ends at 2^-24, weights count in units of
-// 2^-15 (UNIT; the sum l too, so the quotient is the same): 22 bits of those above 2^-28 of the largest, 2^-40 of it for
-// the smaller ones. (In units of 1, a key 16 nats above 2047 others left these 6 % too heavy, 17.5 nats nothing.)
-// Waves, then splits, are joined by their maxima and sums.
+// Softmax in one pass with the running maximum; P enters the product as summands of the cache's type, each what the
+// rounding of those before it left: in bf16 three, all 24 bits of a weight (two, 16 bits, are up to 2 % faster: 64 heads
+// x 96 64.4 -> 65.6 us). In fp16, which ends at 2^-24, two, and weights count in units of 2^-15 (UNIT; the sum l too, so
+// the quotient is the same): 22 bits of those above 2^-28 of the largest, 2^-40 of it for the smaller ones. (In units of
+// 1, a key 16 nats above 2047 others left these 6 % too heavy, 19.5 nats nothing.) Waves, then splits, are joined by
+// their maxima and sums.
 //
 // Blocks are ordered by key head, request, split, and the requests turn by one with each split. With the split first,
 // the blocks that have work in a table much wider than its requests' lengths all met one XCD (16 requests of 1 to 2000
@@ -362,25 +365,25 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
     l *= f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) acc[i] *= f;
-    u32x4_t hi, lo;
+    constexpr int NP = Mat<TYPE>::PARTS;
+    u32x4_t part[NP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint16_t h2[2], l2[2];
+    for (int i = 0; i < 8; ++i) {
+      float x = __builtin_amdgcn_exp2f(p[i] - m);
+      l += x;
+      x *= Mat<TYPE>::UNIT;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float x = __builtin_amdgcn_exp2f(p[2 * i + e] - m);
-        l += x;
-        const float u = x * Mat<TYPE>::UNIT;
-        h2[e] = Mat<TYPE>::bits(u);
-        l2[e] = Mat<TYPE>::bits(u - Mat<TYPE>::back(h2[e]));
+      for (int s = 0; s < NP; ++s) {
+        const uint16_t h = Mat<TYPE>::bits(x);
+        x -= Mat<TYPE>::back(h);
+        if (i & 1) part[s][i / 2] |= (uint32_t)h << 16;
+        else part[s][i / 2] = h;
       }
-      hi[i] = h2[0] | (uint32_t)h2[1] << 16;
-      lo[i] = l2[0] | (uint32_t)l2[1] << 16;
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, hi), acc[j]);
-      acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, lo), acc[j]);
+    for (int s = 0; s < NP; ++s) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, part[s]), acc[j]);
     }
   }
   l += __shfl_xor(l, 16, 64);

@@ -52,3 +52,37 @@ def test_small_weights(cuda, n, gap, spread, peak, dtype):
     rel = 2 * (3 * size + 8 + n / 16 + 64) * U32 + (2.0 ** -22 if dtype == HF else 0.0)
     tol = ref * (half_step(dtype) + rel) + (n * 2.0 ** -40 + 2.0 ** -25 if dtype == HF else 0.0)
     assert bool(((o.double() - ref).abs() <= tol).all()), (float(o[0, 0, 0]), ref)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n", [2, 600])
+def test_weights_that_cancel(cuda, n, dtype):
+    """values a and -b in turn, with weights x and 1 where x a is nearly b: what is left of them shows the bits that the
+    weights have (16 bits: up to 2^-17 of x a; an output of 8 bits sees that only where nothing else is left)"""
+    H, D, page = 64, 32, 16
+    g = torch.Generator(device=cuda).manual_seed(n)
+    s = (-1.5 + 1.45 * torch.rand(H, device=cuda, generator=g)).to(dtype).double()
+    x = s.exp()
+    steps = 2.0 ** (7 if dtype == BF else 10)
+    b = torch.arange(steps, 2 * steps, device=cuda, dtype=torch.float64) / steps       # every value in [1, 2)
+    a = ((b / x[:, None]) * steps / 2).round() / steps * 2                             # the nearest in [1, 16), coarser
+    a = a.to(dtype).double()
+    left = (x[:, None] * a - b).abs()
+    i = left.argmin(1, keepdim=True)
+    a, b = a.gather(1, i), b[i]
+    P = -(-n // page)
+    j = torch.arange(P * page, device=cuda) % 2
+    kc = torch.zeros(P, H, page, D, device=cuda, dtype=dtype)
+    kc[..., 0] = j.to(dtype).view(P, 1, page)
+    v = torch.where(j[None] == 1, a, -b).to(dtype)                                     # [H, tokens]
+    vc = v.view(H, P, page // 8, 1, 8).transpose(0, 1).expand(P, H, page // 8, D, 8).contiguous()
+    q = torch.zeros(1, H, D, device=cuda, dtype=dtype)
+    q[0, :, 0] = s.to(dtype)
+    table = torch.arange(P, dtype=torch.int32, device=cuda)[None]
+    o = paged.paged_attn(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device=cuda), 1.0)[0].double()
+    x = x[:, None]
+    ref = (x * a - b) / (1 + x)
+    # in roundings of fp32: the score's product and the scale by one each of 1.5 / ln 2, the exponential by two, its
+    # summands by one, each product's sum by one of b: of x a, which is b. The sum of weights by n / 16 + 64 of its own
+    tol = (half_step(dtype) + (n / 16 + 64) * U32) * ref.abs() + (2 * 1.5 + 4) * U32 * b / (1 + x)
+    assert bool(((o - ref).abs() <= tol).all()), float(((o - ref).abs() / tol).max())
