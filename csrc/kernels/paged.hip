@@ -217,6 +217,7 @@ template <> struct Mat<1> {
   typedef bf16x8_t v;
   static constexpr int PARTS = 3;                 // summands of a softmax weight, and the unit that it counts in
   static constexpr float UNIT = 1.f;
+  static constexpr uint16_t LEAST = 0x0080;       // a least number above 0
   static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -227,6 +228,7 @@ template <> struct Mat<2> {
   typedef f16x8_t v;
   static constexpr int PARTS = 2;
   static constexpr float UNIT = 32768.f;          // the largest power of two in fp16
+  static constexpr uint16_t LEAST = 0x0001;
   static __device__ __forceinline__ f32x4_t mul(v a, v b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -256,6 +258,11 @@ template <> struct Mat<2> {
 // ones met the same CUs (120000 tokens among 63 short: 239 us, 135 with it).
 //
 // Keys past the length, and pages whose id is not one, have weight 0 and a value of 0 whatever the cache holds there.
+// An infinite value that counts, times its weight's second summand, is NaN (0 is common there) or the other infinity: a
+// wave whose sums are not all finite goes over its keys once more with the first summands alone, and takes those of the
+// dims that are not. The code for it costs 150 short requests 0.2 us of 10.2; the waves a SIMD are asked for because the
+// compiler would give it registers of which heads of 128 leave room for two waves, where there are three (8 requests of
+// up to 2048 tokens 22.1 -> 20.8 us, 64 long grouped ones 272 -> 279).
 //
 // Bound by the read of the cache. V goes past the caches: a load takes whole lines of it. K's loads take half a line
 // of each key row, the next load the other half out of the cache; past it they cost 7 % more. At 64 x ~6100 tokens, 8
@@ -279,7 +286,7 @@ __device__ __forceinline__ int split_of(const PagedDesc& d) {
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
+__global__ __launch_bounds__(NTH, D <= 64 ? 4 : D <= 128 ? 3 : 1) void paged_attn_kernel(const PagedDesc d) {
   typedef typename Mat<TYPE>::v vec;
   constexpr int NK = D / 32, NV = D / 16, NW = NTH / 64;
   __shared__ float sm[NW][16], sl[NW][16];
@@ -298,9 +305,7 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
 #pragma unroll
   for (int j = 0; j < NK; ++j) q[j] = *reinterpret_cast<const vec*>(qp + 32 * j);
   f32x4_t acc[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = NEG, l = 0.f;
+  float m, l;
   const float sc = d.scale * LOG2E;
   const int* tb = d.table + (long long)b * d.ld;
   const uint16_t *K = (const uint16_t*)d.k, *V = (const uint16_t*)d.v;
@@ -317,82 +322,104 @@ __global__ __launch_bounds__(NTH) void paged_attn_kernel(const PagedDesc d) {
     ib = tb[min(t0 + ra + 4, d.cap - 1) >> d.shift];
     iv = tb[min(t0 + rv, d.cap - 1) >> d.shift];
   };
-  if (d.cap > 0) ids(k0 + 32 * w);
-  for (int t0 = k0 + 32 * w; t0 < k1; t0 += 32 * NW) {
-    const bool bad_v = (unsigned)iv >= (unsigned)d.P;
-    const long long ja = (unsigned)ia < (unsigned)d.P ? ia : 0, jb = (unsigned)ib < (unsigned)d.P ? ib : 0;
-    const long long jv = bad_v ? 0 : iv;
-    const uint16_t* pa = K + ja * pst + hoff + ((t0 + ra) & in_page) * D + 8 * g;
-    const uint16_t* pb = K + jb * pst + hoff + ((t0 + ra + 4) & in_page) * D + 8 * g;
-    const uint16_t* pv = V + jv * pst + hoff + ((t0 + rv) & in_page) * D + 8 * n;
-    f32x4_t s0{0.f, 0.f, 0.f, 0.f}, s1{0.f, 0.f, 0.f, 0.f};
-    vec a[NK], c[NK], v[NV];
+  // one pass over the wave's keys. INF: by the weights' first summands alone, 0 only where the weight is
+  auto pass = [&](auto which) {
+    constexpr bool INF = decltype(which)::value;
+    m = NEG;
+    l = 0.f;
 #pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      a[j] = *reinterpret_cast<const vec*>(pa + 32 * j);
-      c[j] = *reinterpret_cast<const vec*>(pb + 32 * j);
-    }
+    for (int i = 0; i < NV; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (d.cap > 0) ids(k0 + 32 * w);
+    for (int t0 = k0 + 32 * w; t0 < k1; t0 += 32 * NW) {
+      const bool bad_v = (unsigned)iv >= (unsigned)d.P;
+      const long long ja = (unsigned)ia < (unsigned)d.P ? ia : 0, jb = (unsigned)ib < (unsigned)d.P ? ib : 0;
+      const long long jv = bad_v ? 0 : iv;
+      const uint16_t* pa = K + ja * pst + hoff + ((t0 + ra) & in_page) * D + 8 * g;
+      const uint16_t* pb = K + jb * pst + hoff + ((t0 + ra + 4) & in_page) * D + 8 * g;
+      const uint16_t* pv = V + jv * pst + hoff + ((t0 + rv) & in_page) * D + 8 * n;
+      f32x4_t s0{0.f, 0.f, 0.f, 0.f}, s1{0.f, 0.f, 0.f, 0.f};
+      vec a[NK], c[NK], v[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(pv + 128 * j));
-    ids(t0 + 32 * NW);
-#pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      s0 = Mat<TYPE>::mul(a[j], q[j], s0);
-      s1 = Mat<TYPE>::mul(c[j], q[j], s1);
-    }
-    float p[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { p[i] = s0[i] * sc; p[4 + i] = s1[i] * sc; }
-    const int left = bad_v ? 0 : k1 - (t0 + 8 * g);         // how many of the lane's eight keys count
-    if (__any(left < 8)) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = i < left ? p[i] : -INFINITY;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        u32x4_t x = __builtin_bit_cast(u32x4_t, v[j]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = left >= 2 * i + 2 ? x[i] : left == 2 * i + 1 ? x[i] & 0xffffu : 0u;
-        v[j] = __builtin_bit_cast(vec, x);
+      for (int j = 0; j < NK; ++j) {
+        a[j] = *reinterpret_cast<const vec*>(pa + 32 * j);
+        c[j] = *reinterpret_cast<const vec*>(pb + 32 * j);
       }
-    }
-    float mx = p[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, p[i]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
-    const float f = __builtin_amdgcn_exp2f(m - mx);
-    m = mx;
-    l *= f;
+      for (int j = 0; j < NV; ++j) v[j] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(pv + 128 * j));
+      ids(t0 + 32 * NW);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) acc[i] *= f;
-    constexpr int NP = Mat<TYPE>::PARTS;
-    u32x4_t part[NP];
+      for (int j = 0; j < NK; ++j) {
+        s0 = Mat<TYPE>::mul(a[j], q[j], s0);
+        s1 = Mat<TYPE>::mul(c[j], q[j], s1);
+      }
+      float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float x = __builtin_amdgcn_exp2f(p[i] - m);
-      l += x;
-      x *= Mat<TYPE>::UNIT;
+      for (int i = 0; i < 4; ++i) { p[i] = s0[i] * sc; p[4 + i] = s1[i] * sc; }
+      const int left = bad_v ? 0 : k1 - (t0 + 8 * g);         // how many of the lane's eight keys count
+      if (__any(left < 8)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = i < left ? p[i] : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          u32x4_t x = __builtin_bit_cast(u32x4_t, v[j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = left >= 2 * i + 2 ? x[i] : left == 2 * i + 1 ? x[i] & 0xffffu : 0u;
+          v[j] = __builtin_bit_cast(vec, x);
+        }
+      }
+      float mx = p[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, p[i]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(m, fmaxf(mx, __shfl_xor(mx, 32, 64)));
+      const float f = __builtin_amdgcn_exp2f(m - mx);
+      m = mx;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) acc[i] *= f;
+      constexpr int NP = INF ? 1 : Mat<TYPE>::PARTS;
+      u32x4_t part[NP];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float x = __builtin_amdgcn_exp2f(p[i] - m);
+        l += x;
+        x *= Mat<TYPE>::UNIT;
+#pragma unroll
+        for (int s = 0; s < NP; ++s) {
+          uint16_t h = Mat<TYPE>::bits(x);
+          if (INF && x > 0.f && h < Mat<TYPE>::LEAST) h = Mat<TYPE>::LEAST;
+          x -= Mat<TYPE>::back(h);
+          if (i & 1) part[s][i / 2] |= (uint32_t)h << 16;
+          else part[s][i / 2] = h;
+        }
+      }
 #pragma unroll
       for (int s = 0; s < NP; ++s) {
-        const uint16_t h = Mat<TYPE>::bits(x);
-        x -= Mat<TYPE>::back(h);
-        if (i & 1) part[s][i / 2] |= (uint32_t)h << 16;
-        else part[s][i / 2] = h;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, part[s]), acc[j]);
       }
     }
+  };
+  float* const mine = &sacc[(w * gc + min(n, gc - 1)) * (D + 4) + 4 * g];
+  pass(std::false_type{});
+  f32x4_t odd{0.f, 0.f, 0.f, 0.f};                // NaN where a sum is not finite
 #pragma unroll
-    for (int s = 0; s < NP; ++s) {
+  for (int j = 0; j < NV; ++j) {
+    if (n < gc) *reinterpret_cast<f32x4_t*>(mine + 16 * j) = acc[j];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, part[s]), acc[j]);
-    }
+    for (int i = 0; i < 4; ++i) odd[i] = fmaf(acc[j][i], 0.f, odd[i]);
+  }
+  if (__any(!(odd[0] + odd[1] + odd[2] + odd[3] == 0.f))) {
+    pass(std::true_type{});
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n < gc && !(fabsf(mine[16 * j + i]) < INFINITY)) mine[16 * j + i] = acc[j][i];
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
   if (g == 0) { sm[w][n] = m; sl[w][n] = l * Mat<TYPE>::UNIT; }
-  if (n < gc) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) *reinterpret_cast<f32x4_t*>(&sacc[(w * gc + n) * (D + 4) + 16 * j + 4 * g]) = acc[j];
-  }
   __syncthreads();
   const bool whole = len <= split;
   for (int e = threadIdx.x; e < gc * D; e += NTH) {

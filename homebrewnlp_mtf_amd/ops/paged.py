@@ -293,7 +293,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
 
     ``max_len`` (default: what the table's width holds) is a bound on lens that the host knows; a close one spares a wide
     table some empty blocks and workspace. A page id outside the pool hides its tokens. What the cache holds behind a length
-    is never looked at. No gradient."""
+    is never looked at. Infinities and NaN among the values that count stay in their dims, as the formula has them (a weight
+    too small for 32 bits is 0, and makes an infinite value NaN). No gradient."""
     qs, dev = q.shape, q.get_device()
     if len(qs) != 3 or qs[1] < 1 or qs[2] < 1:
         raise L.KernelError(f"paged_attn: q must be [B, heads, D], got {list(qs)}")

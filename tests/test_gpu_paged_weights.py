@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from homebrewnlp_mtf_amd.ops import paged
-from paged_cases import U32, half_step
+from paged_cases import U32, attn64, half_step, make_cache
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -86,3 +86,33 @@ def test_weights_that_cancel(cuda, n, dtype):
     # summands by one, each product's sum by one of b: of x a, which is b. The sum of weights by n / 16 + 64 of its own
     tol = (half_step(dtype) + (n / 16 + 64) * U32) * ref.abs() + (2 * 1.5 + 4) * U32 * b / (1 + x)
     assert bool(((o - ref).abs() <= tol).all()), float(((o - ref).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("n,Hq,Hk,D", [(1, 1, 1, 32), (45, 2, 1, 64), (300, 4, 2, 128), (5000, 3, 1, 96), (700, 2, 2, 256)])
+def test_infinite_values(cuda, n, Hq, Hk, D, dtype):
+    """infinities among the values that count: infinite where the definition is, NaN where it is (both signs, or a NaN),
+    the other dims as ever"""
+    kc, vc, table, ln = make_cache([n, 7], 16, Hk, D, dtype, cuda, seed=n)
+    q = torch.randn(2, Hq, D, device=cuda, generator=torch.Generator(device=cuda).manual_seed(n)).to(dtype)
+    scale = D ** -0.5
+
+    def put(j, dim, x):
+        vc[int(table[0, j // 16]), :, j % 16 // 8, dim, j % 8] = x
+    put(0, 0, math.inf)
+    put(n - 1, 1, -math.inf)
+    put(n // 2, 2, math.nan)
+    put(n // 3, 3, math.inf)
+    put(n - 1, 3, -math.inf)
+    for j in range(0, n, 3):
+        put(j, 5, math.inf)
+    # the key of the largest weight: its second summand is 0
+    s = torch.stack([(kc[table[0].long(), h // (Hq // Hk)].reshape(-1, D)[:n].double() @ q[0, h].double())
+                     for h in range(Hq)])
+    put(int(s[0].argmax()), 6, -math.inf)
+    ref, err = attn64(q, kc, vc, table, ln, scale)
+    o = paged.paged_attn(q, kc, vc, table, ln, scale)
+    fine = torch.isfinite(ref)
+    assert bool(fine[1].all()) and bool(fine[0, :, 7:].all()) and not bool(fine[0, :, 0].any())
+    assert torch.equal(torch.nan_to_num(o.double()[~fine], nan=7.0), torch.nan_to_num(ref[~fine], nan=7.0))
+    assert bool(((o.double() - ref).abs()[fine] <= (half_step(dtype) * ref.abs() + err)[fine]).all())
