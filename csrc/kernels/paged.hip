@@ -16,6 +16,7 @@ struct PlanDesc {
   int *start, *lens, *nfree_out;       // [B + 1], [B], [1] out
   int B, W, ld, page, T, P;
 };
+static_assert(sizeof(PlanDesc) == 104);   // as ops/_lib.py packs it
 
 struct PagedDesc {
   const void *q, *k, *v;
@@ -27,6 +28,7 @@ struct PagedDesc {
   int most;                            // > 0: splits grow from `split` until all tokens together make at most so many
   float scale;
 };
+static_assert(sizeof(PagedDesc) == 128);  // as ops/_lib.py packs it
 
 namespace {
 constexpr int NTH = 256;

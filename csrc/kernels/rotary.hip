@@ -33,6 +33,7 @@ struct RotDesc {
   int Hq, Hk, D, R, inter, dtype, wtype, dwtype, dwacc, page;   // types: 0 fp32, 1 bf16, 2 fp16
   float mscale, eps;
 };
+static_assert(sizeof(RotDesc) == 272);    // as ops/_lib.py packs it
 
 namespace {
 constexpr int NTH = 256;

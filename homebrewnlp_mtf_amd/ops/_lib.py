@@ -85,10 +85,11 @@ class OptDesc(ctypes.Structure):
 
 
 # descriptors of the small latency-bound launches, packed in one call (a ctypes Structure of 40 fields takes 2.2 us to
-# fill, this 0.4): field order and types of the C structs in csrc/kernels/rotary.hip and paged.hip, natural alignment
-ROT_DESC = struct.Struct("@16P12q10i2f")      # RotDesc
-PLAN_DESC = struct.Struct("@10P6i")           # PlanDesc
-PAGED_DESC = struct.Struct("@7P2q12if")     # PagedDesc
+# fill, this 0.4): field order and types of the C structs in csrc/kernels/rotary.hip and paged.hip, natural alignment; 0P
+# pads the end as the struct's
+ROT_DESC = struct.Struct("@16P12q10i2f0P")    # RotDesc
+PLAN_DESC = struct.Struct("@10P6i0P")         # PlanDesc
+PAGED_DESC = struct.Struct("@7P2q12if0P")     # PagedDesc
 
 
 _SIGS = {
