@@ -175,11 +175,14 @@ __global__ __launch_bounds__(NTH) void page_plan_kernel(const PlanDesc d) {
   }
 }
 
-// pages of the requests that are done go back onto the stack, in request order; their lengths become 0. One block
+// pages of the requests that are done go back onto the stack, in request order; their lengths become 0. Ids outside the
+// pool are left out. One block, a piece of 1024 requests at a time: a thread a request for its length, a wave a request
+// for its row (once to count its ids, up to what the stack has room for; once to copy them)
 __global__ __launch_bounds__(1024) void page_release_kernel(const unsigned char* __restrict__ done, int* lens,
                                                            const int* __restrict__ table, int* stack, int* nfree, int B,
                                                            int W, int ld, int page, int P) {
-  __shared__ long long cnt[1024];                 // pages of 1024 rows as wide as memory holds pass 31 bits
+  __shared__ int rows[1024];                      // entries of a request's row
+  __shared__ long long cnt[1024];                 // its ids; 1024 times the stack's room may pass 31 bits
   __shared__ int base;
   const int tid = threadIdx.x, lane = tid & 63;
   if (tid == 0) base = min(max(*nfree, 0), P);
@@ -187,8 +190,20 @@ __global__ __launch_bounds__(1024) void page_release_kernel(const unsigned char*
     const int b = b0 + tid;
     int n = 0;
     if (b < B && done[b]) n = (int)min(((long long)max(lens[b], 0) + page - 1) / page, (long long)W);
-    __syncthreads();                              // the piece before this one has read cnt and base
-    cnt[tid] = n;
+    __syncthreads();                              // the piece before this one has read rows, cnt and base
+    rows[tid] = n;
+    cnt[tid] = 0;
+    __syncthreads();
+    const int at0 = base, room = P - at0;
+    for (int r = tid >> 6; r < 1024 && b0 + r < B; r += 16) {
+      const int m = rows[r];
+      if (m == 0) continue;
+      const int* row = table + (long long)(b0 + r) * ld;
+      int c = 0;
+      for (long long i = 0; i < m && c < room; i += 64)
+        c += __popcll(__ballot(i + lane < m && (unsigned)row[min(i + lane, m - 1LL)] < (unsigned)P));
+      if (lane == 0) cnt[r] = c;
+    }
     __syncthreads();
     for (int o = 1; o < 1024; o <<= 1) {          // inclusive prefix sums
       const long long v = tid >= o ? cnt[tid - o] : 0;
@@ -197,11 +212,17 @@ __global__ __launch_bounds__(1024) void page_release_kernel(const unsigned char*
       __syncthreads();
     }
     if (b < B && done[b]) lens[b] = 0;
-    // one wave a request: 16 waves copy the rows of the piece
-    const int at0 = base;
     for (int r = tid >> 6; r < 1024 && b0 + r < B; r += 16) {
-      const long long e = r ? cnt[r - 1] : 0, m = min(cnt[r] - e, P - at0 - e);   // what the stack has room for
-      for (long long i = lane; i < m; i += 64) stack[at0 + e + i] = table[(long long)(b0 + r) * ld + i];
+      long long at = r ? cnt[r - 1] : 0;          // where the row's ids go, behind at0
+      const int m = rows[r];
+      const int* row = table + (long long)(b0 + r) * ld;
+      for (long long i = 0; i < m && at < room; i += 64) {
+        const int id = row[min(i + lane, m - 1LL)];
+        const unsigned long long live = __ballot(i + lane < m && (unsigned)id < (unsigned)P);
+        const long long to = at + __popcll(live & ((1ULL << lane) - 1));
+        if (live >> lane & 1 && to < room) stack[at0 + to] = id;
+        at += __popcll(live);
+      }
     }
     __syncthreads();
     if (tid == 0) base = (int)min(at0 + cnt[1023], (long long)P);

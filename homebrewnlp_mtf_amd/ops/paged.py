@@ -79,8 +79,8 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
               page: int, tokens: typing.Optional[int] = None, out: typing.Optional[PagePlan] = None) -> PagePlan:
     """Pages, slots and positions of a step's new tokens, on the device: request b holds ``cached[b]`` tokens and
     appends ``new[b]`` (int32 [B], negative counts as 0); the step's tokens lie one request after the other in a buffer
-    of ``tokens`` places. New pages come off the top of ``stack`` (int32 [P], ``nfree`` int32 [1] of them unused) and
-    are entered into ``table`` (int32 [B, W]) in place.
+    of ``tokens`` places. New pages come off the top of ``stack`` (int32 [P], ``nfree`` int32 [1] ids of unused pages, 0 to
+    P - 1) and are entered into ``table`` (int32 [B, W]) in place.
 
     Requests are served in order. One is refused -- no slots, its length unchanged -- if its pages pass W, its length
     31 bits, its tokens the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request
@@ -151,7 +151,8 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
 def page_release(done: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, stack: torch.Tensor, nfree: torch.Tensor,
                  page: int) -> None:
     """Requests that are ``done`` (bool [B]) give their pages back: pushed onto ``stack`` in request order, ``nfree``
-    raised and their ``lens`` zeroed, all in place. (A stack that is full takes no more.)"""
+    raised and their ``lens`` zeroed, all in place. Ids outside the pool are left out, and a stack that is full takes no
+    more."""
     dev, B = lens.get_device(), lens.numel()
     _ints("page_release", dev, ("lens", lens), ("stack", stack), ("nfree", nfree))
     if lens.dim() != 1 or B < 1 or done.shape != lens.shape or done.dtype != torch.bool or done.get_device() != dev \
@@ -165,9 +166,10 @@ def page_release(done: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, st
         return
     at = min(max(int(nfree), 0), P)
     for b in done.nonzero().flatten().tolist():
-        n = min(-(-max(int(lens[b]), 0) // page), W, P - at)
-        stack[at:at + n] = table[b, :n]
-        at += n
+        ids = table[b, :min(-(-max(int(lens[b]), 0) // page), W)]
+        ids = ids[(ids >= 0) & (ids < P)][:P - at]
+        stack[at:at + ids.numel()] = ids
+        at += ids.numel()
         lens[b] = 0
     nfree[0] = at
 
