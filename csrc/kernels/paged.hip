@@ -588,10 +588,24 @@ int attn(const PagedDesc& d, hipStream_t st) {
   }
   return -2;
 }
+
+// whether a buffer that the plan writes shares memory with another of its buffers
+bool plan_overlaps(const PlanDesc& d) {
+  struct { uintptr_t a; size_t n; } s[10] = {
+      {(uintptr_t)d.table, 4 * ((size_t)(d.B - 1) * d.ld + d.W)}, {(uintptr_t)d.slots, 4 * (size_t)d.T},
+      {(uintptr_t)d.pos, 8 * (size_t)d.T}, {(uintptr_t)d.start, 4 * ((size_t)d.B + 1)}, {(uintptr_t)d.lens, 4 * (size_t)d.B},
+      {(uintptr_t)d.nfree_out, 4}, {(uintptr_t)d.cached, 4 * (size_t)d.B}, {(uintptr_t)d.nnew, 4 * (size_t)d.B},
+      {(uintptr_t)d.free, 4 * (size_t)d.P}, {(uintptr_t)d.nfree, 4}};
+  for (int i = 0; i < 6; ++i)
+    for (int j = i + 1; j < 10; ++j)
+      if (s[i].n && s[j].n && s[i].a < s[j].a + s[j].n && s[j].a < s[i].a + s[i].n) return true;
+  return false;
+}
 }  // namespace
 
 OBST_API int obst_page_plan(const PlanDesc* d, hipStream_t st) {
   if (!d || d->B < 1 || d->W < 1 || d->ld < d->W || d->page < 1 || d->T < 0 || d->P < 1) return -1;
+  if (plan_overlaps(*d)) return -2;
   const int gx = (d->B + GR - 1) / GR;
   long long gy = d->T / ((long long)d->B * GL * 4);      // a few rounds of a request's tokens per lane
   gy = gy < 1 ? 1 : gy > 64 ? 64 : gy;

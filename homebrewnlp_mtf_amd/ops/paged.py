@@ -75,6 +75,13 @@ def _table(what: str, table, B: int, dev: int) -> typing.Tuple[int, int]:
     return shape[1], st[0] if B > 1 else shape[1]
 
 
+def _shared(written, read) -> bool:
+    """whether one of the written tensors overlaps another one"""
+    spans = [(t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+             if t.numel() else None for t in (*written, *read)]
+    return any(a and b and a[0] < b[1] and b[0] < a[1] for i, a in enumerate(spans[:len(written)]) for b in spans[i + 1:])
+
+
 def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stack: torch.Tensor, nfree: torch.Tensor,
               page: int, tokens: typing.Optional[int] = None, out: typing.Optional[PagePlan] = None) -> PagePlan:
     """Pages, slots and positions of a step's new tokens, on the device: request b holds ``cached[b]`` tokens and
@@ -85,7 +92,8 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
     Requests are served in order. One is refused -- no slots, its length unchanged -- if its pages pass W, its length
     31 bits, its tokens the buffer, or the pages asked for by the requests up to and including it ``nfree`` (a request
     that needs no new page goes on). ``cached`` and ``nfree`` are not written: the plan holds their new values, and
-    the same call again gives the same plan. ``out`` must not share memory with them."""
+    the same call again gives the same plan. What is written (``out``, ``table``) must not share memory with anything else
+    here."""
     dev, B = cached.get_device(), cached.numel()
     _ints("page_plan", dev, ("cached", cached), ("new", new), ("stack", stack), ("nfree", nfree))
     if cached.dim() != 1 or B < 1 or new.shape != cached.shape or nfree.numel() != 1 or stack.dim() != 1:
@@ -106,8 +114,6 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
                 or out.lens.numel() != B or out.nfree.numel() != 1
                 or (tokens is not None and tokens != out.slots.numel())):
             raise L.KernelError("page_plan: out does not fit (plan_buffers)")
-        if out.lens.data_ptr() in (cached.data_ptr(), new.data_ptr()) or out.nfree.data_ptr() == nfree.data_ptr():
-            raise L.KernelError("page_plan: out shares memory with cached, new or nfree")
     T = out.slots.numel()
     if T >= 2 ** 31:
         raise L.KernelError(f"page_plan: {T} tokens")
@@ -118,6 +124,8 @@ def page_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, stac
             B, W, ld, page, T, P))
         return out
     # ---- torch oracle
+    if _shared((table, *out), (cached, new, stack, nfree)):
+        raise L.KernelError("page_plan: out or the table shares memory with another argument")
     avail = min(max(int(nfree), 0), P)
     out.slots.fill_(-1)
     out.pos.zero_()

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from homebrewnlp_mtf_amd.ops import paged
-from test_paged_edges_cpu import release_cases
+from test_paged_edges_cpu import plan_refuses_shared_memory, release_cases
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +20,7 @@ def test_release_row_without_ids(cuda):
     lens, nfree = torch.full((3,), 3200, dtype=torch.int32, device=cuda), torch.zeros(1, dtype=torch.int32, device=cuda)
     paged.page_release(torch.ones(3, dtype=torch.bool, device=cuda), lens, table, stack, nfree, 16)
     assert stack.tolist() == list(range(200)) and nfree.tolist() == [200] and lens.tolist() == [0, 0, 0]
+
+
+def test_plan_refuses_shared_memory(cuda):
+    plan_refuses_shared_memory(cuda)

@@ -50,3 +50,47 @@ def release_cases(dev, sizes):
 def test_release_leaves_out_ids_outside_the_pool():
     """an id that is no page would be handed out again, and its tokens lost"""
     release_cases("cpu", [(1, 1, 1), (5, 6, 20), (40, 3, 500)])
+
+
+def plan_refuses_shared_memory(dev):
+    """every buffer that the plan writes, each over the end of every other one: refused, nothing written"""
+    B, W, T, P = 3, 4, 6, 12
+    room = torch.zeros(256, dtype=torch.int32, device=dev)
+    sizes = dict(table=B * W, slots=T, pos=2 * T, start=B + 1, lens=B, nfree_out=1, cached=B, new=B, stack=P, nfree=1)
+    apart, at = {}, 0
+    for n, m in sizes.items():
+        apart[n] = at
+        at += m + m % 2
+
+    def call(first):
+        room.fill_(0)
+        v = {n: room[first[n]:first[n] + m] for n, m in sizes.items()}
+        v["new"].fill_(2)
+        v["stack"].copy_(torch.arange(P))
+        v["nfree"].fill_(P)
+        out = paged.PagePlan(v["slots"], v["pos"].view(torch.int64), v["start"], v["lens"], v["nfree_out"])
+        before = room.clone()
+        try:
+            return paged.page_plan(v["cached"], v["new"], v["table"].view(B, W), v["stack"], v["nfree"], 16, out=out)
+        finally:
+            if first is not apart:
+                assert torch.equal(room, before)
+    assert call(apart).lens.tolist() == [2] * B
+    written = ("table", "slots", "pos", "start", "lens", "nfree_out")
+    for w in written:
+        for x in sizes:
+            if x == w:
+                continue
+            # the last place of w over the first of x (pos by its 8 bytes)
+            to = apart[x] - sizes[w] + (2 if w == "pos" else 1)
+            if w == "pos":
+                to -= to % 2
+            if to >= 0:
+                with pytest.raises(L.KernelError):
+                    call({**apart, w: to})
+            with pytest.raises(L.KernelError):
+                call({**apart, w: apart[x]})
+
+
+def test_plan_refuses_shared_memory():
+    plan_refuses_shared_memory("cpu")
