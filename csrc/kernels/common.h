@@ -40,6 +40,12 @@ __device__ __forceinline__ void vm_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// host: whether n bytes at a and m bytes at b share any
+inline bool overlap(const void* a, size_t n, const void* b, size_t m) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return n && m && x < y + m && y < x + n;
+}
+
 __device__ __forceinline__ float bf2f(bf16_t v) {
   return __uint_as_float(((uint32_t)v) << 16);
 }

@@ -591,15 +591,23 @@ int attn(const PagedDesc& d, hipStream_t st) {
 
 // whether a buffer that the plan writes shares memory with another of its buffers
 bool plan_overlaps(const PlanDesc& d) {
-  struct { uintptr_t a; size_t n; } s[10] = {
-      {(uintptr_t)d.table, 4 * ((size_t)(d.B - 1) * d.ld + d.W)}, {(uintptr_t)d.slots, 4 * (size_t)d.T},
-      {(uintptr_t)d.pos, 8 * (size_t)d.T}, {(uintptr_t)d.start, 4 * ((size_t)d.B + 1)}, {(uintptr_t)d.lens, 4 * (size_t)d.B},
-      {(uintptr_t)d.nfree_out, 4}, {(uintptr_t)d.cached, 4 * (size_t)d.B}, {(uintptr_t)d.nnew, 4 * (size_t)d.B},
-      {(uintptr_t)d.free, 4 * (size_t)d.P}, {(uintptr_t)d.nfree, 4}};
+  struct { const void* p; size_t n; } s[10] = {
+      {d.table, 4 * ((size_t)(d.B - 1) * d.ld + d.W)}, {d.slots, 4 * (size_t)d.T}, {d.pos, 8 * (size_t)d.T},
+      {d.start, 4 * ((size_t)d.B + 1)}, {d.lens, 4 * (size_t)d.B}, {d.nfree_out, 4}, {d.cached, 4 * (size_t)d.B},
+      {d.nnew, 4 * (size_t)d.B}, {d.free, 4 * (size_t)d.P}, {d.nfree, 4}};
   for (int i = 0; i < 6; ++i)
     for (int j = i + 1; j < 10; ++j)
-      if (s[i].n && s[j].n && s[i].a < s[j].a + s[j].n && s[j].a < s[i].a + s[i].n) return true;
+      if (overlap(s[i].p, s[i].n, s[j].p, s[j].n)) return true;
   return false;
+}
+
+// the outputs may take the queries' own place (a block reads its rows first), but no other part of what the call reads
+bool out_overlaps(const PagedDesc& d) {
+  const size_t n = 2 * (size_t)d.B * d.Hq * d.D, pool = 2 * ((size_t)d.P << d.shift) * d.Hk * d.D;
+  const bool own = d.o == d.q && (d.q_hs == d.D || d.Hq == 1) && (d.q_bs == (long long)d.Hq * d.D || d.B == 1);
+  return (!own && overlap(d.o, n, d.q, 2 * ((d.B - 1) * d.q_bs + (d.Hq - 1) * d.q_hs + d.D))) ||
+         overlap(d.o, n, d.k, pool) || overlap(d.o, n, d.v, pool) || overlap(d.o, n, d.lens, 4 * (size_t)d.B) ||
+         overlap(d.o, n, d.table, 4 * ((size_t)(d.B - 1) * d.ld + ((d.cap - 1) >> d.shift) + 1));
 }
 }  // namespace
 
@@ -629,6 +637,7 @@ OBST_API int obst_paged_attn(const PagedDesc* d, hipStream_t st) {
   if (d->shift < 4 || d->shift > 8 || (long long)d->ld << d->shift < d->cap) return -3;
   if (d->most < 0 || (d->most > 0 && (d->B > MAX_SUM || d->split % 128))) return -6;
   if (d->cap > (long long)d->nsplit * d->split && (d->most == 0 || d->nsplit < d->most)) return -4;
+  if (out_overlaps(*d)) return -7;
   if (d->dtype == 1) return attn<1>(*d, st);
   if (d->dtype == 2) return attn<2>(*d, st);
   return -5;

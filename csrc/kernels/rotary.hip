@@ -632,6 +632,19 @@ int pow2_at_least(int n) {
   return p;
 }
 
+// the turned queries may take the queries' own place (a wave reads all of a row before it writes it), but no other part of
+// what the call reads or writes
+bool out_overlaps(const RotDesc& d) {
+  const size_t e = d.dtype == 0 ? 4 : 2, row = (size_t)d.Hq * d.D, n = d.qo ? e * d.T * row : 0;
+  const bool own = d.qo == d.q && (d.q_hs == d.D || d.Hq == 1) && (d.q_ts == (long long)row || d.T == 1);
+  auto span = [&](long long ts, int H, long long hs) { return e * ((d.T - 1) * ts + (H - 1) * hs + d.D); };
+  const size_t pool = e * (size_t)d.nslots * d.Hk * d.D;
+  return (!own && overlap(d.qo, n, d.q, span(d.q_ts, d.Hq, d.q_hs))) ||
+         overlap(d.qo, n, d.k, span(d.k_ts, d.Hk, d.k_hs)) || overlap(d.qo, n, d.v, span(d.v_ts, d.Hk, d.v_hs)) ||
+         overlap(d.qo, n, d.ko, pool) || overlap(d.qo, n, d.vo, pool) || overlap(d.qo, n, d.pos, 8 * d.T) ||
+         overlap(d.qo, n, d.slots, 4 * d.T);
+}
+
 // four blocks a CU; the backward's count also sizes its partials
 constexpr int FWD_BLOCKS = 1024, BWD_BLOCKS = 1024;
 
@@ -747,6 +760,7 @@ int run(const RotDesc* d, bool bwd, hipStream_t st) {
     hipLaunchKernelGGL(rotary_fold_kernel, dim3((2 * d->D + 15) / 16), dim3(1024), 0, st, *d, 0, 0);
     return (int)hipGetLastError();
   }
+  if (d->slots && out_overlaps(*d)) return -4;
   switch (d->dtype) {
     case 0: return dispatch<0>(*d, bwd, st);
     case 1: return dispatch<1>(*d, bwd, st);

@@ -210,6 +210,12 @@ def _out(what: str, out, q, shape, dev: int):
     return out
 
 
+def _apart(what: str, out, q, *others) -> None:
+    own = out.data_ptr() == q.data_ptr() and q.is_contiguous()
+    if _shared((out,), others if own else (q, *others)):
+        raise L.KernelError(f"{what}: out shares memory with another argument")
+
+
 def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   slots: torch.Tensor, pos: torch.Tensor, freqs: typing.Optional[torch.Tensor],
                   interleaved: bool = False, mscale: float = 1.0, q_weight: typing.Optional[torch.Tensor] = None,
@@ -218,7 +224,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
     """``rotary.rotary`` of a step's tokens with the turned keys and the values written into the cache: q [T, Hq, D],
     k and v [T, Hk, D] (any token and head strides), ``slots`` int32 [T] (outside the pool: neither key nor value is
     written), ``pos`` int64 [T]. Returns the turned queries [T, Hq, D]. ``freqs`` None and no weights: a plain append.
-    One launch, no gradient. Tokens of one call must have different slots."""
+    One launch, no gradient. Tokens of one call must have different slots. ``out`` may be q itself, and shares no memory
+    with anything else here."""
     pos, freqs, rot, T = check_args("rotary_append", q, k, pos, freqs, q_weight, k_weight, eps)
     qs, ks, dev = q.shape, k.shape, q.get_device()
     if len(qs) != 3 or v.shape != ks or v.dtype != q.dtype or v.get_device() != dev:
@@ -248,6 +255,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
             eps))
         return out
     # ---- torch oracle
+    _apart("rotary_append", out, q, k, v, k_cache, v_cache, slots, pos)
     _scatter_t(rotary_t(k, None if k_weight is None else k_weight.detach(), pos, freqs, interleaved, mscale, eps), v,
                k_cache, v_cache, slots)
     out.copy_(rotary_t(q, None if q_weight is None else q_weight.detach(), pos, freqs, interleaved, mscale, eps))
@@ -304,7 +312,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     ``max_len`` (default: what the table's width holds) is a bound on lens that the host knows; a close one spares a wide
     table some empty blocks and workspace. A page id outside the pool hides its tokens. What the cache holds behind a length
     is never looked at. Infinities and NaN among the values that count stay in their dims, as the formula has them (a weight
-    too small for 32 bits is 0, and makes an infinite value NaN). No gradient."""
+    too small for 32 bits is 0, and makes an infinite value NaN). ``out`` may be q itself, and shares no memory with anything
+    else here. No gradient."""
     qs, dev = q.shape, q.get_device()
     if len(qs) != 3 or qs[1] < 1 or qs[2] < 1:
         raise L.KernelError(f"paged_attn: q must be [B, heads, D], got {list(qs)}")
@@ -346,6 +355,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
             most, scale))
         return out
     # ---- torch oracle
+    _apart("paged_attn", out, q, k_cache, v_cache, table, lens)
     G = Hq // Hk
     for b in range(B):
         n = min(max(int(lens[b]), 0), cap)

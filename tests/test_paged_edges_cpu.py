@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from homebrewnlp_mtf_amd.ops import _lib as L
-from homebrewnlp_mtf_amd.ops import paged
+from homebrewnlp_mtf_amd.ops import paged, rotary
 
 KERNELS = pathlib.Path(__file__).resolve().parent.parent / "csrc" / "kernels"
 
@@ -94,3 +94,47 @@ def plan_refuses_shared_memory(dev):
 
 def test_plan_refuses_shared_memory():
     plan_refuses_shared_memory("cpu")
+
+
+def outputs_in_place_and_shared(dev):
+    """queries turned, and attended, in their own place; an output over any other part of a call's memory is refused"""
+    dt = torch.bfloat16
+    g = torch.Generator().manual_seed(5)
+    B, Hq, Hk, D, page = 4, 4, 2, 32, 16
+    room = torch.randn(4 * B * Hq * D, generator=g).to(dt).to(dev)
+    n = B * Hq * D
+    q = room[n:2 * n].view(B, Hq, D)
+    k, v = (torch.randn(B, Hk, D, generator=g).to(dt).to(dev) for _ in range(2))
+    kc, vc = paged.page_pools(4, page, Hk, D, dt, dev)
+    kc.normal_()
+    vc.normal_()
+    i32 = dict(dtype=torch.int32, device=dev)
+    slots, pos = torch.arange(B, device=dev).mul(page).int(), torch.arange(B, device=dev) * 100
+    table, lens = torch.arange(4, **i32).view(B, 1), torch.tensor([16, 3, 0, 9], **i32)
+    f = rotary.rotary_freqs(D, device=dev)[0]
+    calls = (lambda q, out=None, k=k, v=v, kc=kc, vc=vc: paged.rotary_append(q, k, v, kc, vc, slots, pos, f, out=out),
+             lambda q, out=None, kc=kc, vc=vc: paged.paged_attn(q, kc, vc, table, lens, 0.2, out=out))
+    for call in calls:
+        want = call(q.clone())
+        own = q.clone()
+        assert call(own, out=own).data_ptr() == own.data_ptr() and torch.equal(own, want)
+        before = room.clone()
+        for shift in (8, D, Hq * D, n - 8):
+            for at in (n - shift, n + shift):
+                with pytest.raises(L.KernelError):
+                    call(q, out=room[at:at + n].view(B, Hq, D))
+        with pytest.raises(L.KernelError):                 # the queries' place, in another order
+            call(q.view(Hq, B, D).transpose(0, 1), out=q)
+        assert torch.equal(room, before)
+        assert torch.equal(call(q, out=room[:n].view(B, Hq, D)), want)          # beside each other
+        room.copy_(before)
+        for cache in (kc, vc):
+            with pytest.raises(L.KernelError):
+                call(q, out=cache.view(-1)[:n].view(B, Hq, D))
+    for x in ("k", "v"):
+        with pytest.raises(L.KernelError):
+            calls[0](q, out=room[2 * n:3 * n].view(B, Hq, D), **{x: room[2 * n + 8:2 * n + 8 + B * Hk * D].view(B, Hk, D)})
+
+
+def test_outputs_in_place_and_shared():
+    outputs_in_place_and_shared("cpu")
