@@ -21,7 +21,7 @@ import torch
 
 from . import _lib as L
 from . import raw
-from .rotary import DTYPES, MAX_DIM, check_args, kernel_weights, rotary_t, tokens_view
+from .rotary import DTYPES, MAX_DIM, check_args, kernel_weights, refuse_tangents, rotary_t, tokens_view
 
 HEAD_DIMS = (32, 64, 96, 128, 256)
 PAGES = (16, 32, 64, 128, 256)
@@ -235,6 +235,7 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: to
                                     or v_cache.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
         raise L.KernelError("rotary_append has no gradient: call it under torch.no_grad()")
+    refuse_tangents("rotary_append", q, k, v, k_cache, v_cache, q_weight, k_weight)
     _, Hq, D = qs
     P, Hk, page = _pools("rotary_append", k_cache, v_cache, q, dev, D, ks[1])
     _ints("rotary_append", dev, ("slots", slots))
@@ -273,6 +274,7 @@ def append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
         raise L.KernelError(f"append: bf16, fp16 or fp32 on the GPU, got {k.dtype}")
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise L.KernelError("append has no gradient: call it under torch.no_grad()")
+    refuse_tangents("append", k, v, k_cache, v_cache)
     T, Hk, D = ks
     P, Hk, page = _pools("append", k_cache, v_cache, k, dev, D, Hk)
     _ints("append", dev, ("slots", slots))
@@ -323,6 +325,7 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
         raise L.KernelError(f"paged_attn: {Hq} query heads over {Hk} key heads")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise L.KernelError("paged_attn has no gradient: call it under torch.no_grad()")
+    refuse_tangents("paged_attn", q, k_cache, v_cache)
     W, ld = _table("paged_attn", table, B, dev)
     _ints("paged_attn", dev, ("lens", lens))
     if lens.dim() != 1 or lens.numel() != B:

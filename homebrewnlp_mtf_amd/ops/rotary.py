@@ -16,6 +16,7 @@ import math
 import typing
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from . import raw
@@ -128,6 +129,13 @@ def check_args(what: str, q, k, pos, freqs, wq, wk, eps: float):
     if not eps > 0:
         raise L.KernelError(f"{what}: eps must be positive, got {eps}")
     return pos, freqs, rot, math.prod(lead)
+
+
+def refuse_tangents(what: str, *tensors):
+    """the kernels carry no forward-mode derivative: a dual tensor is refused rather than its tangent dropped"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise L.KernelError(f"{what} has no forward-mode derivative")
 
 
 def kernel_weights(wq, wk):
@@ -303,4 +311,6 @@ def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, freqs: typing.Op
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)
                                     or (k_weight is not None and k_weight.requires_grad)):
         return _Rotary.apply(q, k, q_weight, k_weight, pos, freqs, cfg)
+    if q.get_device() >= 0:
+        refuse_tangents("rotary", q, k, q_weight, k_weight)
     return _forward(q, k, pos, freqs, q_weight, k_weight, *cfg)

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from homebrewnlp_mtf_amd.ops import paged
-from test_paged_edges_cpu import outputs_in_place_and_shared, plan_refuses_shared_memory, release_cases
+from test_paged_edges_cpu import outputs_in_place_and_shared, plan_refuses_shared_memory, release_cases, tangents
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,7 @@ def test_plan_refuses_shared_memory(cuda):
 
 def test_outputs_in_place_and_shared(cuda):
     outputs_in_place_and_shared(cuda)
+
+
+def test_tangents(cuda):
+    tangents(cuda)

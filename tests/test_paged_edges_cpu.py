@@ -5,6 +5,7 @@ import re
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from homebrewnlp_mtf_amd.ops import _lib as L
 from homebrewnlp_mtf_amd.ops import paged, rotary
@@ -138,3 +139,42 @@ def outputs_in_place_and_shared(dev):
 
 def test_outputs_in_place_and_shared():
     outputs_in_place_and_shared("cpu")
+
+
+def tangents(dev):
+    """forward-mode derivatives: what has none says so"""
+    g = torch.Generator().manual_seed(6)
+    f = rotary.rotary_freqs(32, device=dev)[0]
+    kc, vc = paged.page_pools(2, 16, 1, 32, torch.bfloat16, dev)
+    kc.zero_()
+    vc.zero_()
+    x, t, w = (torch.randn(*s, generator=g).to(torch.bfloat16).to(dev) for s in ((3, 1, 32), (3, 1, 32), (32,)))
+    i32 = dict(dtype=torch.int32, device=dev)
+    slots, pos = torch.arange(3, **i32), torch.arange(3, device=dev)
+    table, lens = torch.zeros(3, 1, **i32), torch.ones(3, **i32)
+    with torch.no_grad(), forward_ad.dual_level():
+        d, dw = forward_ad.make_dual(x, t), forward_ad.make_dual(w, w)
+        dk, dv = forward_ad.make_dual(kc, kc.clone()), forward_ad.make_dual(vc, vc.clone())
+        calls = [lambda: paged.rotary_append(d, x, x, kc, vc, slots, pos, f), lambda: paged.rotary_append(x, d, x, kc, vc, slots, pos, f),
+                 lambda: paged.rotary_append(x, x, d, kc, vc, slots, pos, f),
+                 lambda: paged.rotary_append(x, x, x, kc, vc, slots, pos, f, k_weight=dw),
+                 lambda: paged.append(d, x, kc, vc, slots), lambda: paged.append(x, d, kc, vc, slots),
+                 lambda: paged.append(x, x, dk, vc, slots), lambda: paged.paged_attn(d, kc, vc, table, lens, 1.0),
+                 lambda: paged.paged_attn(x, kc, dv, table, lens, 1.0)]
+        if x.is_cuda:
+            calls += [lambda: rotary.rotary(d, x, pos, f), lambda: rotary.rotary(x, d, pos, f),
+                      lambda: rotary.rotary(x, x, pos, f, q_weight=dw)]
+        else:
+            o = rotary.rotary(d, x, pos, f)[0]
+            assert torch.equal(forward_ad.unpack_dual(o).tangent, rotary.rotary(t, x, pos, f)[0])
+        for call in calls:
+            with pytest.raises(L.KernelError):
+                call()
+        assert not bool(kc.any()) and not bool(vc.any())
+        rotary.rotary(x, x, pos, f, q_weight=w)                       # none of them has a tangent
+        paged.rotary_append(x, x, x, kc, vc, slots, pos, f)
+        paged.paged_attn(x, kc, vc, table, lens, 1.0)
+
+
+def test_tangents():
+    tangents("cpu")
