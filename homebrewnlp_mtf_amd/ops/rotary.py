@@ -34,11 +34,12 @@ def rotary_freqs(rot_dim: int, theta: float = 10000.0, scaling: typing.Optional[
     the trained one: ``{"type": ..., "factor": s}`` with
 
     * ``"linear"``: positions are divided by s;
-    * ``"base"``: theta grows by ``s ** (rot_dim / (rot_dim - 2))``: the slowest pair turns s times slower, the fastest
-      as before;
-    * ``"ramp"``: pairs that turn more than ``fast`` (32) times over the trained ``length`` (2048) keep their frequency,
-      those under ``slow`` (1) turns are divided by s, linear in between over the pair's index; mscale is
-      ``0.1 ln s + 1``, sharpening the scores that the longer context flattens."""
+    * ``"base"`` (the "NTK-aware" base): theta grows by ``s ** (rot_dim / (rot_dim - 2))``: the slowest pair turns s times
+      slower, the fastest as before;
+    * ``"ramp"`` (YaRN, Peng et al. 2023): pairs that turn more than ``fast`` (32) times over the trained ``length`` (2048)
+      keep their frequency, those under ``slow`` (1) turns are divided by s, linear in between over the pair's index
+      (from the whole pair before the one to the whole pair after the other, pairs past the last one counted up to
+      ``rot_dim - 1``); mscale is ``0.1 ln s + 1``, sharpening the scores that the longer context flattens."""
     if rot_dim < 2 or rot_dim % 2:
         raise ValueError(f"rotary needs an even number of dims, got {rot_dim}")
     if not theta > 0:
@@ -67,8 +68,10 @@ def rotary_freqs(rot_dim: int, theta: float = 10000.0, scaling: typing.Optional[
 
         def pair_of(turns):     # the (fractional) pair that makes `turns` turns over the trained length
             return rot_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(theta))
-        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim // 2 - 1)
+        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim - 1)
         far = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        if pair_of(slow) < 0:                                   # also the fastest pair is under `slow` turns
+            far = torch.ones_like(i)
         freqs = freqs * (1 - far) + freqs / s * far
         mscale = 0.1 * math.log(s) + 1.0
     elif kind not in (None, "base"):

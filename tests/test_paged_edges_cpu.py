@@ -1,4 +1,5 @@
 """Rotary and paged-cache operators on the CPU: calls at the edge of what they take."""
+import math
 import pathlib
 import random
 import re
@@ -178,3 +179,29 @@ def tangents(dev):
 
 def test_tangents():
     tangents("cpu")
+
+
+@pytest.mark.parametrize("theta", [500.0, 10000.0, 500000.0])
+@pytest.mark.parametrize("rot,length,fast,slow", [(64, 2048, 32, 1), (128, 4096, 32, 1), (8, 32768, 32, 1), (16, 10 ** 6, 32, 1),
+                                                  (64, 4, 32, 1), (64, 2, 2, 0.5), (32, 6, 8, 2), (8, 100, 4, 3.9)])
+def test_ramp_keeps_and_divides_as_it_says(rot, length, fast, slow, theta):
+    """every pair by its own turns over the trained length: as it was above `fast`, divided below `slow`, in between on
+    a line over the pair's index that spans the two (their whole pairs around it)"""
+    s = 8.0
+    f, _ = rotary.rotary_freqs(rot, theta)
+    r, m = rotary.rotary_freqs(rot, theta, {"type": "ramp", "factor": s, "length": length, "fast": fast, "slow": slow})
+    assert math.isclose(m, 0.1 * math.log(s) + 1)
+    turns = f * length / (2 * math.pi)
+    part = (r / f - 1) / (1 / s - 1)                     # 0: kept, 1: divided
+    assert bool((part >= -1e-12).all()) and bool((part <= 1 + 1e-12).all())
+    assert bool((part[turns < slow] > 1 - 1e-9).all()) and bool((part[turns > fast] < 1e-9).all())
+    step = part.diff()
+    assert bool((step > -1e-9).all())
+    # the line: equal steps between the pairs that are on it
+    on = (part > 1e-9) & (part < 1 - 1e-9)
+    both = on[1:] & on[:-1]
+    if int(both.sum()) > 1:
+        assert float(step[both].max() - step[both].min()) < 1e-9
+    # the slowest pair is divided in full only where it turns less than the pair after it, at most `slow` times
+    if float(turns[-1]) > slow * theta ** (2 / rot):
+        assert float(part[-1]) < 1 - 1e-9
