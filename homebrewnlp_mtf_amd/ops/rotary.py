@@ -24,6 +24,7 @@ from .functional import _acc_grad, _done, _param32
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_DIM = 512
+MIN_EPS, MAX_EPS = 2.0 ** -126, 2.0 ** 127
 
 
 def rotary_freqs(rot_dim: int, theta: float = 10000.0, scaling: typing.Optional[dict] = None,
@@ -129,8 +130,8 @@ def check_args(what: str, q, k, pos, freqs, wq, wk, eps: float):
     for w in (wq, wk):
         if w is not None and (w.numel() != D or w.get_device() != dev or not w.dtype.is_floating_point):
             raise L.KernelError(f"{what}: norm weights must be [{D}] on the device of q")
-    if not eps > 0:
-        raise L.KernelError(f"{what}: eps must be positive, got {eps}")
+    if not MIN_EPS <= eps < MAX_EPS and not (q.dtype == torch.float64 and eps > 0):
+        raise L.KernelError(f"{what}: eps must be positive and a normal number of 32 bits, got {eps}")
     return pos, freqs, rot, math.prod(lead)
 
 

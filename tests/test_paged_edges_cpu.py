@@ -205,3 +205,21 @@ def test_ramp_keeps_and_divides_as_it_says(rot, length, fast, slow, theta):
     # the slowest pair is divided in full only where it turns less than the pair after it, at most `slow` times
     if float(turns[-1]) > slow * theta ** (2 / rot):
         assert float(part[-1]) < 1 - 1e-9
+
+
+def test_eps_that_vanishes_in_32_bits():
+    """added in 32 bits, it is 0: rows of zeros would be 0 times infinity. 64 bits hold it"""
+    f = rotary.rotary_freqs(8)[0]
+    pos = torch.arange(2)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        x, w = torch.zeros(2, 1, 8, dtype=dtype), torch.ones(8, dtype=dtype)
+        kc, vc = paged.page_pools(1, 16, 1, 8, dtype, "cpu")
+        for eps in (1e-50, 1e-39, math.inf, math.nan, 1e39, -1.0):
+            with pytest.raises(L.KernelError):
+                rotary.rotary(x, x, pos, f, q_weight=w, eps=eps)
+            with pytest.raises(L.KernelError):
+                paged.rotary_append(x, x, x, kc, vc, pos.int(), pos, f, k_weight=w, eps=eps)
+        for eps in (2.0 ** -126, 1e-30, 1e-5, 1e38):
+            assert not bool(rotary.rotary(x, x, pos, f, q_weight=w, eps=eps)[0].any())
+    x = torch.zeros(2, 1, 8, dtype=torch.float64)
+    assert not bool(rotary.rotary(x, x, pos, f, q_weight=torch.ones(8), eps=1e-50)[0].any())
