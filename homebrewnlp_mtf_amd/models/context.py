@@ -46,7 +46,7 @@ class Pages:
             old = persist["bufs"]["pages"] = {"key": (B, S, page, dev), "count": max(total, 1), "table": torch.empty(
                 B, -(-S // page), dtype=torch.int32, device=dev)}
             persist["graph"] = None
-        self.page, self.count, self.table = page, old["count"], old["table"]
+        self.page, self.context, self.count, self.table = page, S, old["count"], old["table"]
         self.table.fill_(-1)          # a position that was not reserved has no slot
 
         def i32(v):
@@ -62,10 +62,12 @@ class Pages:
         self.lens: typing.Optional[torch.Tensor] = None
 
     def step(self, pos: torch.Tensor):
-        """slots and lengths of the decode step's tokens, one a request at ``pos`` (on the device, once a step)"""
-        ids = self.table.gather(1, torch.div(pos, self.page, rounding_mode="floor").unsqueeze(1)).squeeze(1).long()
-        self.slots = (ids * self.page + pos % self.page).int()
-        self.lens = (pos + 1).int()
+        """slots and lengths of the decode step's tokens, one a request at ``pos`` (on the device, once a step). As with
+        dense caches, a token outside the context is kept nowhere and attends to what the context holds"""
+        at = pos.clamp(0, self.context - 1)
+        ids = self.table.gather(1, torch.div(at, self.page, rounding_mode="floor").unsqueeze(1)).squeeze(1).long()
+        self.slots = torch.where(at == pos, ids * self.page + at % self.page, -1).int()
+        self.lens = (pos + 1).clamp(0, self.context).int()
 
 
 class KVCache:

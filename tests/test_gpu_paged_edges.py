@@ -32,3 +32,21 @@ def test_outputs_in_place_and_shared(cuda):
 
 def test_tangents(cuda):
     tangents(cuda)
+
+
+def test_decoding_outside_the_context(cuda):
+    """positions before and behind the context, eager and replayed: as dense caches, nothing kept and nothing read outside"""
+    from test_gpu_rotary_paged import _model
+    m, p = _model(cuda, kv_page_size=16)
+    x = torch.randint(0, 256, (3, 96, 1), generator=torch.Generator().manual_seed(1)).to(cuda)
+    steps = [torch.tensor(v, device=cuda) for v in ([96, 4, 50], [97, 5, -1], [10 ** 6, 6, -10 ** 6], [111, 7, 112])]
+    out = []
+    for page, graphs in ((0, False), (16, False), (16, True)):
+        p.kv_page_size, p.decode_hip_graphs = page, graphs
+        m.prefill(x, torch.tensor([95, 3, 95], device=cuda))
+        out.append(torch.stack([m.decode(x[:, :1], s).clone() for s in steps]))
+        m.end_decode()
+    assert torch.equal(out[1], out[2])
+    # two layers of about ten bf16 roundings each, every one off by 2^-8 of what it rounds at most
+    a, b = out[0].flatten(2), out[1].flatten(2)
+    assert bool(((a - b).norm(dim=-1) <= 20 * 2.0 ** -8 * a.norm(dim=-1)).all())

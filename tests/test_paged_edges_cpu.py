@@ -10,6 +10,7 @@ from torch.autograd import forward_ad
 
 from homebrewnlp_mtf_amd.ops import _lib as L
 from homebrewnlp_mtf_amd.ops import paged, rotary
+from test_rotary_paged_cpu import ROTARY, _params
 
 KERNELS = pathlib.Path(__file__).resolve().parent.parent / "csrc" / "kernels"
 
@@ -223,3 +224,26 @@ def test_eps_that_vanishes_in_32_bits():
             assert not bool(rotary.rotary(x, x, pos, f, q_weight=w, eps=eps)[0].any())
     x = torch.zeros(2, 1, 8, dtype=torch.float64)
     assert not bool(rotary.rotary(x, x, pos, f, q_weight=torch.ones(8), eps=1e-50)[0].any())
+
+
+# ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("extras", ["-rotary", ""])
+def test_decoding_outside_the_context(extras):
+    """a position before or behind the context: paged caches give what dense ones do, and hold what they held"""
+    from homebrewnlp_mtf_amd.models.model import Model
+    from homebrewnlp_mtf_amd.parallel import state as pstate
+    pstate.set_mesh(pstate.Mesh())
+    torch.manual_seed(0)
+    p = _params(sequence_length=40, **ROTARY, block_config=[
+        {"layer": ["norm-shift-scale", "attention-dot_product-context" + extras], "skip": True}])
+    m = Model(p, "cpu")
+    x = torch.randint(0, 64, (3, 40, 1), generator=torch.Generator().manual_seed(1))
+    for pos in (40, 47, 48, 10 ** 6, -1, -17, -10 ** 6):
+        out = []
+        for page in (0, 16):
+            p.kv_page_size = page
+            m.prefill(x, torch.tensor([39, 39, 5]))          # rows 0 and 1 hold the whole context
+            out.append([m.decode(x[:, :1], torch.tensor([pos, pos, at])) for at in (6, 7)])
+            m.end_decode()
+        for a, b in zip(*out):
+            assert torch.allclose(a, b, rtol=1e-4, atol=1e-5)       # fp32, sums in another order
