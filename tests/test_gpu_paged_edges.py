@@ -4,6 +4,7 @@ import torch
 
 from homebrewnlp_mtf_amd.ops import paged
 from test_paged_edges_cpu import outputs_in_place_and_shared, plan_refuses_shared_memory, release_cases, tangents
+from test_rotary_paged_cpu import _params
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,29 @@ def test_decoding_outside_the_context(cuda):
     # two layers of about ten bf16 roundings each, every one off by 2^-8 of what it rounds at most
     a, b = out[0].flatten(2), out[1].flatten(2)
     assert bool(((a - b).norm(dim=-1) <= 20 * 2.0 ** -8 * a.norm(dim=-1)).all())
+
+
+@pytest.mark.parametrize("strategy", ["checkpoint", "revnet", "momentum"])
+def test_training_strategies(cuda, strategy):
+    """gradients of recomputed and reconstructed blocks point where the CPU's do (bf16 activations through two layers)"""
+    from homebrewnlp_mtf_amd.models.model import Model
+    p = _params(calculation_dtype="bfloat16", storage_dtype="bfloat16", memory_reduction_strategy=strategy,
+                features_per_head=64, sequence_length=96, vocab_size=256, rotary_fraction=0.5)
+    grads = []
+    t = torch.randint(0, 256, (3, 97, 1), generator=torch.Generator().manual_seed(3))
+    for dev in (cuda, torch.device("cpu")):
+        torch.manual_seed(0)
+        m = Model(p, dev)
+        if grads:
+            m.store.master.copy_(master)
+            if m.store.compute.data_ptr() != m.store.master.data_ptr():
+                m.store.compute.copy_(master)
+        master = m.store.master
+        m.store.zero_grad()
+        m(token_x=t[:, :-1].contiguous().to(dev), token_y=t[:, 1:].contiguous().to(dev))["loss"].backward()
+        grads.append(m.store.grad.cpu())
+    cos = torch.nn.functional.cosine_similarity
+    assert cos(*grads, dim=0) > 0.97
+    for n in [n for n in m.store.order if "qk_norm" in n]:
+        sp = m.store.specs[n]
+        assert cos(*(g[sp.offset:sp.offset + sp.numel] for g in grads), dim=0) > 0.97, n

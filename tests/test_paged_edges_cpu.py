@@ -247,3 +247,42 @@ def test_decoding_outside_the_context(extras):
             m.end_decode()
         for a, b in zip(*out):
             assert torch.allclose(a, b, rtol=1e-4, atol=1e-5)       # fp32, sums in another order
+
+
+@pytest.mark.parametrize("extras", ["-rotary-qk_norm", "-rotary", "-qk_norm"])
+@pytest.mark.parametrize("strategy", ["none", "checkpoint", "revnet", "momentum"])
+def test_training_gradients(strategy, extras):
+    """every strategy's gradients -- recomputed blocks, reconstructed streams -- against differences of the loss, along
+    random directions of each weight that lies before or in the turned attention"""
+    from homebrewnlp_mtf_amd.parallel import state as pstate
+    from homebrewnlp_mtf_amd.run.trainer import Trainer
+    pstate.set_mesh(pstate.Mesh())
+    torch.manual_seed(0)
+    tr = Trainer(_params(memory_reduction_strategy=strategy, **ROTARY, block_config=[
+        {"layer": ["norm-shift-scale", "attention-dot_product-context" + extras], "skip": True},
+        {"layer": ["norm-shift-scale", "feed_forward-in:gelu"], "skip": True}]), "cpu")
+    st = tr.model.store
+    t = torch.randint(0, 64, (3, 17, 1), generator=torch.Generator().manual_seed(2))
+    batch = {"token_x": t[:, :-1].contiguous(), "token_y": t[:, 1:].contiguous()}
+    st.zero_grad()
+    tr.model(**batch)["loss"].backward()
+    grads = st.grad.clone()
+    names = [n for n in st.order if "qk_norm" in n or "attention" in n]
+    assert len(names) >= 4 and ("qk_norm" not in extras or sum("qk_norm" in n for n in names) == 4)
+    g = torch.Generator().manual_seed(3)
+    bufs = {b.data_ptr(): b for b in (st.master, st.compute)}.values()
+    for name in names:
+        sp = st.specs[name]
+        grad = grads[sp.offset:sp.offset + sp.numel]
+        d = torch.sign(grad) + 0.5 * torch.randn(sp.numel, generator=g)     # a direction in which the loss moves
+        d *= 3e-2 / d.norm()
+        vals = []
+        for sign in (1, -2, 1):
+            for b in bufs:
+                b[sp.offset:sp.offset + sp.numel] += sign * d
+            with torch.no_grad():
+                vals.append(float(tr.model(**batch)["loss"]))
+        got, want = float(grad @ d), (vals[0] - vals[1]) / 2
+        # the losses (~4) are fp32 sums, each off by some half steps of 2.4e-7; the difference's third order, of a step
+        # of 3e-2, is 1e-3 of it
+        assert got > 0 and abs(got - want) < 4e-6 + 0.02 * abs(want), (name, got, want)
