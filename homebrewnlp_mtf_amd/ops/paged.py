@@ -309,7 +309,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
     ``page_pools`` makes them with Hq a multiple of their heads (query heads h * G .. h * G + G - 1 read key head h),
     ``table`` int32 [B, W], ``lens`` int32 [B] the tokens that count, the new one among them:
 
-        out[b, h] = softmax_j(scale * q[b, h] . k_j) @ v,  j < min(lens[b], max_len);  0 for a request without tokens
+        out[b, h] = softmax_j(scale * q[b, h] . k_j) @ v,  j < min(lens[b], max_len)
+        0 for a request without tokens, or with -inf for every score
 
     ``max_len`` (default: what the table's width holds) is a bound on lens that the host knows; a close one spares a wide
     table some empty blocks and workspace. A page id outside the pool hides its tokens. What the cache holds behind a length
@@ -372,7 +373,8 @@ def paged_attn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ta
             out[b] = 0
             continue
         s = torch.einsum("hgd,jhd->hgj", raw._f(q[b]).reshape(Hk, G, D), raw._f(kk)) * scale
-        out[b] = torch.einsum("hgj,jhd->hgd", torch.softmax(s, -1), raw._f(vv)).reshape(Hq, D)
+        o = torch.einsum("hgj,jhd->hgd", torch.softmax(s, -1), raw._f(vv))
+        out[b] = o.masked_fill(s.amax(-1, keepdim=True) == float("-inf"), 0).reshape(Hq, D)
     return out
 
 

@@ -3,7 +3,8 @@ import pytest
 import torch
 
 from homebrewnlp_mtf_amd.ops import paged
-from test_paged_edges_cpu import outputs_in_place_and_shared, plan_refuses_shared_memory, release_cases, tangents
+from test_paged_edges_cpu import (outputs_in_place_and_shared, plan_refuses_shared_memory, release_cases,
+                                  scores_of_minus_infinity, tangents)
 from test_rotary_paged_cpu import _params
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +78,7 @@ def test_training_strategies(cuda, strategy):
     for n in [n for n in m.store.order if "qk_norm" in n]:
         sp = m.store.specs[n]
         assert cos(*(g[sp.offset:sp.offset + sp.numel] for g in grads), dim=0) > 0.97, n
+
+
+def test_scores_of_minus_infinity(cuda):
+    scores_of_minus_infinity(cuda)

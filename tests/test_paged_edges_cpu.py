@@ -226,6 +226,30 @@ def test_eps_that_vanishes_in_32_bits():
     assert not bool(rotary.rotary(x, x, pos, f, q_weight=torch.ones(8), eps=1e-50)[0].any())
 
 
+def scores_of_minus_infinity(dev):
+    """a request all of whose scores are -inf has no weights: 0, as one without tokens; some of them hide their keys"""
+    g = torch.Generator().manual_seed(8)
+    kc, vc = paged.page_pools(4, 16, 1, 32, torch.bfloat16, dev)
+    kc.copy_(torch.randn(kc.shape, generator=g))
+    vc.copy_(torch.randn(vc.shape, generator=g))
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([20, 20], dtype=torch.int32, device=dev)
+    q = torch.ones(2, 3, 32, dtype=torch.bfloat16, device=dev)
+    kc[:2, :, :, 5] = -math.inf
+    kc[2, :, :, 5] = -math.inf                 # the second request's keys 16 to 19 are left
+    o = paged.paged_attn(q, kc, vc, table, lens, 0.1)
+    w = torch.softmax(0.1 * kc[3, 0, :4].double().sum(-1), 0)
+    ref = (w[:, None] * vc[3, 0, 0, :, :4].double().t()).sum(0)
+    assert not bool(o[0].any())
+    # a score of 32 products within (32 + 4) roundings of its size, twice; half a step of bf16
+    err = 2 * 36 * 2.0 ** -24 * float(0.1 * kc[3, 0, :4].double().abs().sum(-1).max()) + 2.0 ** -20
+    assert bool(((o[1].double() - ref).abs() <= 2.0 ** -8 * ref.abs() + err * vc[3].double().abs().max()).all())
+
+
+def test_scores_of_minus_infinity():
+    scores_of_minus_infinity("cpu")
+
+
 # ----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("extras", ["-rotary", ""])
 def test_decoding_outside_the_context(extras):
