@@ -313,6 +313,10 @@ static int g4w_queue_tri_env() {   // the triangular (token-mixer) products on t
   static int v = [] { const char* e = getenv("OBST_G4W_QUEUE_TRI"); return e ? atoi(e) : 1; }();
   return v;
 }
+// by a kernel, not hipMemsetAsync: recorded into a hipGraph, memset nodes left counters as they were on later replays,
+// and the product skipped tiles (a 2-layer GPT-Neo-1.3B step: losses off in the fourth digit, or NaN)
+__global__ void g4w_queue_clear_kernel(unsigned* q) { q[threadIdx.x] = 0; }
+
 static unsigned* g4w_queue_slot(hipStream_t stream) {
   constexpr int RING = 256;
   static unsigned* ring = nullptr;
@@ -322,8 +326,8 @@ static unsigned* g4w_queue_slot(hipStream_t stream) {
     return nullptr;
   }
   unsigned* q = ring + (next++ % RING) * 8;
-  if (hipMemsetAsync(q, 0, 8 * sizeof(unsigned), stream) != hipSuccess) return nullptr;
-  return q;
+  hipLaunchKernelGGL(g4w_queue_clear_kernel, dim3(1), dim3(8), 0, stream, q);
+  return hipGetLastError() == hipSuccess ? q : nullptr;
 }
 
 // Every GEMM of the framework is one of two hand-written kernels: gemm4w (gemm4w.h: the one-wave-per-SIMD 256x256

@@ -72,6 +72,15 @@ __global__ __launch_bounds__(NTH) void tril_kernel(const bf16_t* __restrict__ X,
   }
 }
 
+// 16-byte stores of the aligned middle, grid-stride; single bytes of the ends
+__global__ __launch_bounds__(NTH) void zero_kernel(unsigned char* p, long long head, long long nvec, long long bytes) {
+  const long long tid = (long long)blockIdx.x * NTH + threadIdx.x;
+  uint4* v = reinterpret_cast<uint4*>(p + head);
+  for (long long i = tid; i < nvec; i += (long long)gridDim.x * NTH) v[i] = make_uint4(0, 0, 0, 0);
+  if (tid < head) p[tid] = 0;
+  if (head + nvec * 16 + tid < bytes) p[head + nvec * 16 + tid] = 0;      // fewer than 16
+}
+
 }  // namespace
 
 // rows/cols of X; ldx/ldy row strides (elements); sx/sy batch strides. rows, cols, ldx, ldy multiples of 8.
@@ -109,7 +118,13 @@ OBST_API int obst_tril(const void* X, void* Y, long long S, long long batch, hip
   return (int)hipGetLastError();
 }
 
-// bytes of zeros (the flat gradient buffer at the start of a step): the runtime's fill, not a framework kernel
+// bytes of zeros (the flat gradient buffer at the start of a step). A kernel, not hipMemsetAsync: the training step is
+// captured, and memset nodes of a hipGraph have cleared nothing on later replays
 OBST_API int obst_zero(void* p, long long bytes, hipStream_t st) {
-  return (int)hipMemsetAsync(p, 0, (size_t)bytes, st);
+  if (bytes < 0) return -1;
+  if (bytes == 0) return 0;
+  const long long head = (16 - ((uintptr_t)p & 15)) % 16, nvec = bytes > head ? (bytes - head) / 16 : 0;
+  const unsigned g = (unsigned)(nvec / NTH + 1 < 8192 ? nvec / NTH + 1 : 8192);
+  hipLaunchKernelGGL(zero_kernel, dim3(g), dim3(NTH), 0, st, (unsigned char*)p, head < bytes ? head : bytes, nvec, bytes);
+  return (int)hipGetLastError();
 }

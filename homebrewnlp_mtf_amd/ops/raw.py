@@ -766,12 +766,9 @@ def tril(x):
     return torch.tril(x)
 
 
-_ZERO_MEMSET = __import__("os").environ.get("OBST_ZERO_MEMSET", "1") != "0"
-
-
 def zero_(t):
-    """t[:] = 0 (contiguous): the runtime's memset on the GPU (OBST_ZERO_MEMSET=0: torch's fill)"""
-    if _ZERO_MEMSET and on_gpu(t) and t.is_contiguous():
+    """t[:] = 0, by a kernel: hipMemsetAsync is no part of a captured step"""
+    if on_gpu(t) and t.is_contiguous():
         L.check(L.lib().obst_zero(t.data_ptr(), t.numel() * t.element_size(), L.stream_ptr()), "zero")
         return t
     return t.zero_()
