@@ -283,13 +283,14 @@ template <> struct Mat<2> {
 // Keys past the length, and pages whose id is not one, have weight 0 and a value of 0 whatever the cache holds there.
 // An infinite value that counts, times its weight's second summand, is NaN (0 is common there) or the other infinity: a
 // wave whose sums are not all finite goes over its keys once more with the first summands alone, and takes those of the
-// dims that are not. The code for it costs 150 short requests 0.2 us of 10.2; the waves a SIMD are asked for because the
-// compiler would give it registers of which heads of 128 leave room for two waves, where there are three (8 requests of
-// up to 2048 tokens 22.1 -> 20.8 us, 64 long grouped ones 272 -> 279).
+// dims that are not. The check costs 150 short requests 0.3 us of 10. The waves a SIMD are asked for because the compiler
+// would take registers that leave room for two waves with heads of 128, where there are three (8 requests of up to 2048
+// tokens 22.1 -> 20.7 us).
 //
 // Bound by the read of the cache. V goes past the caches: a load takes whole lines of it. K's loads take half a line
 // of each key row, the next load the other half out of the cache; past it they cost 7 % more. At 64 x ~6100 tokens, 8
-// key heads x 128, 4 query heads each (1.6 GB): 258 us, 6.2 TB/s, where a bare read of such data reaches 7.1.
+// key heads x 128, 4 query heads each (1.6 GB): 262 us with the join, 6.1 TB/s, where a bare read of such data reaches
+// 7.1.
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float NEG = -3.0e38f;                   // a running maximum before any key
 
@@ -370,6 +371,9 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 4 : D <= 128 ? 3 : 1) void paged_att
 #pragma unroll
       for (int j = 0; j < NV; ++j) v[j] = __builtin_nontemporal_load(reinterpret_cast<const vec*>(pv + 128 * j));
       ids(t0 + 32 * NW);
+      // all loads before the products: within the registers of three waves a SIMD the compiler starts some behind them
+      // (64 long grouped contexts x 128: 255 us, 248 so; heads of 256, one wave a SIMD: 213 us, 223 so)
+      if constexpr (D <= 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < NK; ++j) {
         s0 = Mat<TYPE>::mul(a[j], q[j], s0);
@@ -400,26 +404,29 @@ __global__ __launch_bounds__(NTH, D <= 64 ? 4 : D <= 128 ? 3 : 1) void paged_att
       l *= f;
 #pragma unroll
       for (int i = 0; i < NV; ++i) acc[i] *= f;
-      constexpr int NP = INF ? 1 : Mat<TYPE>::PARTS;
-      u32x4_t part[NP];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float x = __builtin_amdgcn_exp2f(p[i] - m);
-        l += x;
-        x *= Mat<TYPE>::UNIT;
-#pragma unroll
-        for (int s = 0; s < NP; ++s) {
-          uint16_t h = Mat<TYPE>::bits(x);
-          if (INF && x > 0.f && h < Mat<TYPE>::LEAST) h = Mat<TYPE>::LEAST;
-          x -= Mat<TYPE>::back(h);
-          if (i & 1) part[s][i / 2] |= (uint32_t)h << 16;
-          else part[s][i / 2] = h;
-        }
+        p[i] = __builtin_amdgcn_exp2f(p[i] - m);
+        l += p[i];
+        p[i] *= Mat<TYPE>::UNIT;
       }
 #pragma unroll
-      for (int s = 0; s < NP; ++s) {
+      for (int s = 0; s < (INF ? 1 : Mat<TYPE>::PARTS); ++s) {
+        u32x4_t part;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, part[s]), acc[j]);
+        for (int i = 0; i < 4; ++i) {
+          uint16_t h[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = p[2 * i + e];
+            h[e] = Mat<TYPE>::bits(x);
+            if (INF && x > 0.f && h[e] < Mat<TYPE>::LEAST) h[e] = Mat<TYPE>::LEAST;
+            x -= Mat<TYPE>::back(h[e]);
+          }
+          part[i] = h[0] | (uint32_t)h[1] << 16;
+        }
+#pragma unroll
+        for (int j = 0; j < NV; ++j) acc[j] = Mat<TYPE>::mul(v[j], __builtin_bit_cast(vec, part), acc[j]);
       }
     }
   };

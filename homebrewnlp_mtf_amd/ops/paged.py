@@ -383,16 +383,16 @@ def _splits(B: int, rows: int, cap: int) -> typing.Tuple[int, int, int]:
 
     Up to 16 requests (``most`` > 0): the kernel sizes the splits from the lengths it finds, at least 256 tokens each
     and three blocks a CU from all of them, so no request has more than ``most`` splits and the table's width hardly
-    matters (8 requests of 1 to 2000 tokens, 8 key heads: 12.8 us in a table of 2000, 13.9 in one of 131072; 4 of 1 to
-    30000: 46 us, 53 in two blocks a CU, 49 in four). One request's splits are all alike: two blocks a CU (131072
-    tokens, 4 key heads: 44 us + 5 to join, 47 + 6 in three). A table so narrow that its splits are the shortest either
+    matters (8 requests of 1 to 2000 tokens, 8 key heads: 12.3 us in a table of 2000, 14.7 in one of 131072; 4 of 1 to
+    30000: 53 us, 59 in two blocks a CU, 57 in four). One request's splits are all alike: two blocks a CU (131072
+    tokens, 4 key heads: 46.7 us with the join, 48.3 in three). A table so narrow that its splits are the shortest either
     way spares the kernel that sum, 0.6 us.
 
     More requests would start too many empty blocks that way (32 of 1 to 2000 in a table of 131072: 42 us, 33 by the
-    width), so the width decides: four blocks a CU, 384 to 2048 tokens a split (64 of 6144, 8 key heads: 248 us, 273
-    in splits of 512; 200 of 1 to 2000, 1 key head: 28 us, 35 in two blocks a CU), and longer splits where that makes
-    more than 65536 blocks (1000 of 1 to 500 in a table of 131072: 209 us, 397 in splits of 2048; 256, one of them of
-    120000: 209, 170). At most 1024 splits (csrc/kernels/paged.hip MAX_SPLITS)."""
+    width), so the width decides: four blocks a CU, 384 to 2048 tokens a split (64 of 6144, 8 key heads: 248 us, 275
+    in splits of 512; 200 of 1 to 2000, 1 key head: 28 us, 31 in two blocks a CU), and longer splits where that makes
+    more than 65536 blocks (1000 of 1 to 500 in a table of 131072: 201 us, 395 in splits of 2048; 256, one of them of
+    120000: 209, 168). At most 1024 splits (csrc/kernels/paged.hip MAX_SPLITS)."""
     if B <= 16:
         blocks = 512 if B == 1 else 768
         most = max(1, blocks // rows) if cap * rows * B > blocks * 256 else 0
