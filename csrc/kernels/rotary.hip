@@ -8,7 +8,9 @@
 // dx = r (h - u mean(h u)),  dw = sum over tokens and heads of g u.
 //
 // Angles are formed in 64 bits as turns (pos * freq / 2 pi, minus its nearest integer): at position 10^5 a 32-bit
-// product is off by 10^-2 radians. sin and cos then see an argument within half a turn.
+// product is off by 10^-2 radians, this one by three roundings of 2^-53 of the turns made, 2e-15 radians a turn: less
+// than a rounding of 32 bits up to 3e7 turns (position 1.8e8 of a pair of frequency 1). sin and cos then see an argument
+// within half a turn.
 //
 // A head's elements are cut into items of two chunks of VEC elements (16 bytes): one lane holds both members of its
 // pairs, so the rotation needs no exchange between lanes. LPH lanes hold a head, a wave 64 / LPH heads of one token.

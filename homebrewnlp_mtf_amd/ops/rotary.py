@@ -35,10 +35,10 @@ def rotary_freqs(rot_dim: int, theta: float = 10000.0, scaling: typing.Optional[
     the trained one: ``{"type": ..., "factor": s}`` with
 
     * ``"linear"``: positions are divided by s;
-    * ``"base"`` (the "NTK-aware" base): theta grows by ``s ** (rot_dim / (rot_dim - 2))``: the slowest pair turns s times
-      slower, the fastest as before;
-    * ``"ramp"`` (YaRN, Peng et al. 2023): pairs that turn more than ``fast`` (32) times over the trained ``length`` (2048)
-      keep their frequency, those under ``slow`` (1) turns are divided by s, linear in between over the pair's index
+    * ``"base"`` (the "NTK-aware" base): theta grows by ``s ** (rot_dim / (rot_dim - 2))``: the slowest pair turns s
+      times slower, the fastest as before;
+    * ``"ramp"`` (YaRN, Peng et al. 2023): pairs that turn more than ``fast`` (32) times over the trained ``length``
+      (2048) keep their frequency, those under ``slow`` (1) turns are divided by s, linear in between over the pair's index
       (from the whole pair before the one to the whole pair after the other, pairs past the last one counted up to
       ``rot_dim - 1``); mscale is ``0.1 ln s + 1``, sharpening the scores that the longer context flattens."""
     if rot_dim < 2 or rot_dim % 2:
@@ -307,9 +307,11 @@ def rotary(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, freqs: typing.Op
            k_weight: typing.Optional[torch.Tensor] = None, eps: float = 1e-5
            ) -> typing.Tuple[torch.Tensor, torch.Tensor]:
     """Queries [..., Hq, D] and keys [..., Hk, D] of the same tokens, normed (each where its weight [D] is given) and
-    turned (module docstring); any token and head strides. ``pos`` int64 over the tokens (or broadcastable to them, any
-    value), ``freqs`` float64 from ``rotary_freqs`` (None: no rotation). Returns new contiguous tensors; differentiable
-    in q, k and the weights, sums in fp32, weight gradients in a fixed order (the same bits each run)."""
+    turned (module docstring); any token and head strides. ``pos`` int64 over the tokens (or broadcastable to them; angles
+    are off by up to 2e-15 radians a turn made: a rounding of 32 bits at position 1.8e8 of a pair of frequency 1),
+    ``freqs`` float64 from ``rotary_freqs`` (None: no rotation). Returns new contiguous tensors; differentiable in q, k
+    and the weights, sums in fp32, weight gradients in a fixed order (the same bits each run). No forward-mode derivative
+    on the GPU."""
     pos, freqs, rot, T = check_args("rotary", q, k, pos, freqs, q_weight, k_weight, eps)
     cfg = (rot, T, bool(interleaved), float(mscale), float(eps))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and q_weight.requires_grad)

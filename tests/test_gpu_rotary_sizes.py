@@ -109,3 +109,18 @@ def test_append_sizes(cuda, T, Hq, Hk, D, rot, inter, norm, dtype):
     s = slots.long()
     rows_within(kc.permute(0, 2, 1, 3).reshape(P * page, Hk, D)[s], rotary64(k, w[1], pos, freqs, inter, 1.1, 1e-5), dtype)
     assert torch.equal(vc.permute(0, 2, 4, 1, 3).reshape(P * page, Hk, D)[s], v)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("Hq,D", [(1, 64), (16, 64), (3, 34)])
+def test_far_positions(cuda, Hq, D, inter):
+    """angles formed in 64 bits, off by three roundings of 2^-53 of the turns made, the definition's by one"""
+    g = torch.Generator(device=cuda).manual_seed(D)
+    pos = torch.tensor([0, 1, 10 ** 6, 10 ** 7 + 1, 150000001, -150000001, 2 ** 31 - 1, -2 ** 31, 10 ** 11 + 7], device=cuda)
+    q = torch.randn(pos.numel(), Hq, D, device=cuda, generator=g)
+    freqs = rotary.rotary_freqs(D, device=cuda)[0]
+    y = rotary.rotary(q, q, pos, freqs, interleaved=inter)[0]
+    ref = rotary64(q, None, pos, freqs, inter, 1.0, 1e-5)
+    angle = 4 * 2.0 ** -53 * pos.double().abs()[:, None, None]                 # the fastest pair's, in radians
+    tol = ((32 + D) * U32 + angle) * 2 ** 0.5 * ref.abs().amax(-1, keepdim=True)
+    assert bool(((y.double() - ref).abs() <= tol).all())
