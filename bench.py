@@ -54,9 +54,8 @@ def _self_launch(n: int) -> int:
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--gpus", type=int, default=1)
-    # defaults as the driver's command (--steps 20 --warmup 5): with 3 warm-up steps (the eager first step and the two
-    # captures) the timed window starts on the first graph replays, which run slower -- 140.2k vs 150.6k tokens/s at
-    # 10 / 3 vs 20 / 5 on one box (profiles/r6s/bench_defaults_ab.txt)
+    # five warm-up steps: two eager ones, the two captures with their first replays, and one more replay, so that the
+    # timed window holds replays only
     ap.add_argument("--steps", type=int, default=20)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--config", default=os.path.join(os.path.dirname(os.path.abspath(__file__)), "configs",
